@@ -592,6 +592,89 @@ typedef struct {
 int vitmi_transpose_cast_multi(const vitmi_transpose_job* jobs, const long long* tile_start, int n_jobs,
                                long long total_tiles, void* stream);
 
+/* ---- decoder-block operators over image and video tokens -------------------------------------------------------
+ * The reference has absolute positional tables, self-attention over one packed qkv and pre-norm residuals only; these
+ * entry points are what a block that reads the states of ANOTHER sequence needs beside them.  Their arguments travel in
+ * a host struct that is read during the call and not kept. */
+
+/* Rotary positions with several axes on one or two tensors [B, N, heads, DH] (queries and keys of one token set) in one
+ * launch.  Pair p of a head, p = 0 .. P-1 with P = sum of sections[], belongs to the axis whose section holds it; its
+ * angle is pos[b][n][axis] * base^(-j / sections[axis]), j the pair's index within the axis (shared_ladder: base^(-p / P)),
+ * formed in 64 bits.  The pair's two elements are dims p and P + p, or 2p and 2p + 1 (interleaved); dims from 2P on pass
+ * through.  inverse turns the other way: the gradient.  y may be x with the same strides (in place; the dims that pass
+ * through are then not touched).  Strides are in elements (batch, token, head), the head dim has stride 1; a position
+ * stride may be 0.  Up to 4 axes and 256 pairs. */
+#define VITMI_POS_I32 0
+#define VITMI_POS_I64 1
+#define VITMI_POS_F32 2
+typedef struct {
+    const void* x;
+    void* y;
+    long long xs[3], ys[3];
+    int heads, pad;
+} vitmi_rope_tensor;
+typedef struct {
+    vitmi_rope_tensor t[2];      /* t[1].x == NULL: one tensor */
+    const void* pos;
+    long long pos_stride[3];     /* batch, token, axis */
+    double log2_base[4];         /* log2 of each axis's base */
+    int sections[4];
+    int axes, pos_type, dt, B, N, DH, interleaved, shared_ladder, inverse, pad;
+} vitmi_rope_args;
+int vitmi_rope_axes(const vitmi_rope_args* args, void* stream);
+
+/* Attention of q [B, Nq, Hq, D] over k, v [B, Nk, Hk, D]; query heads h * Hq/Hk .. share key head h.  o and the
+ * gradients are dense in the same shapes; q, k, v, dout have strides in elements (batch, row, head; 0 allowed) and unit
+ * stride over D <= 128.  kv_len [B] (int32, or int64 with kv_len_i64; clamped to 0 .. Nk) or key_mask [B, Nk] bytes
+ * (0 = not attended to; rows mask_stride apart, unit stride), or neither.  Masked keys count as absent whatever their
+ * rows hold, their gradients are zero; a sample without an allowed key gives o = 0 and zero gradients.
+ * lse [B, Hq * Nq] fp32 (log2 domain, +inf for an empty row) is written by the forward call (NULL: not kept) and read by
+ * the backward call.  dq may be NULL, and dk with dv. */
+typedef struct {
+    const void *q, *k, *v;
+    void* o;
+    long long qs[3], ks[3], vs[3];
+    const void *kv_len, *key_mask;
+    long long mask_stride;
+    float* lse;
+    const void* dout;
+    long long dos[3];
+    void *dq, *dk, *dv;
+    int kv_len_i64, dt, B, Nq, Nk, Hq, Hk, D;
+    float scale;
+    int pad;
+} vitmi_xattn_args;
+long long vitmi_cross_attn_fwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D);
+int vitmi_cross_attn_fwd(const vitmi_xattn_args* args, void* workspace, void* stream);
+long long vitmi_cross_attn_bwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D);
+int vitmi_cross_attn_bwd(const vitmi_xattn_args* args, void* workspace, void* stream);
+
+/* The residual update with the norms on both sides, for x (residual stream, dt_x) and u (the branch's output, dt_u no
+ * wider than dt_x) [B, N, D]:   p = post(u),  y = res_scale * x + branch_scale[b] * gate * p,  h = pre(y).
+ * post / pre: 0 = nothing, 1 = LayerNorm, 2 = RMS norm, over D <= 8192 with eps, affine parameters fp32 or NULL.  gate [D]
+ * (gate_stride 0) or [B, D], fp32 or bf16 (gate_dt), or NULL.  branch_scale fp32 [B] or NULL; where it is 0 the branch is
+ * absent: y = res_scale * x and u is not read.  x, u have strides in elements (batch, row) and unit stride over D; y, h, dy,
+ * dh, dx, du are dense (y, dy, dx of dt_x; h, dh, du of dt_u).  stats fp32 [4][B * N] is written by the forward call (NULL:
+ * not kept) and read by the backward call.  Backward: dy or dh may be NULL (zero), any output may be NULL; dgate has the
+ * gate's shape (dense) and type. */
+typedef struct {
+    const void *x, *u;
+    long long xs[2], us[2];
+    void *y, *h;
+    const void* gate;
+    long long gate_stride;
+    const float *branch_scale, *post_w, *post_b, *pre_w, *pre_b;
+    float* stats;
+    const void *dy, *dh;
+    void *dx, *du, *dgate;
+    float *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    int gate_dt, dt_x, dt_u, B, N, D, post, pre;
+    float res_scale, eps;
+} vitmi_ngr_args;
+int vitmi_norm_gate_residual_fwd(const vitmi_ngr_args* args, void* stream);
+long long vitmi_norm_gate_residual_bwd_workspace_bytes(int B, int N, int D, int gate_per_sample);
+int vitmi_norm_gate_residual_bwd(const vitmi_ngr_args* args, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

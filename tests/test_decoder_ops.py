@@ -1,0 +1,267 @@
+"""The decoder-block operators on the CPU: the oracle's gradients against differences, the refusals of the Python entry
+points (shapes and types are checked before the device), and the argument checks and size queries of the C ABI, which
+return before any device call -- those also under the host-sanitized build where it exists."""
+import ctypes
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from oracle import decoder_oracle as orc
+from visiontransformer_amd import _lib, ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def rnd(*s, seed=0):
+    return torch.randn(*s, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shared", [False, True])
+def test_oracle_rope_against_differences(interleaved, shared):
+    x = rnd(2, 3, 2, 11).requires_grad_()
+    pos = torch.tensor([[0, 0], [3, -2], [1000003, 7]])
+    f = lambda t: orc.rope_axes(t, pos, (2, 3), 100.0, interleaved, shared)
+    assert torch.autograd.gradcheck(f, (x,))
+    y = f(x)
+    assert torch.equal(y[:, 0], x[:, 0])                                   # the origin turns by nothing
+    assert torch.allclose(y.square().sum(-1), x.square().sum(-1))          # a rotation keeps lengths
+    assert torch.equal(y[..., 10:], x[..., 10:])
+
+
+def test_oracle_rope_scores_depend_on_distance_alone():
+    q, k = rnd(1, 1, 1, 8), rnd(1, 1, 1, 8, seed=1)
+    at = lambda t, p: orc.rope_axes(t, torch.tensor([[p, 2 * p]]), (2, 2))
+    a = (at(q, 5) * at(k, 3)).sum()
+    b = (at(q, 1005) * at(k, 1003)).sum()
+    assert abs(a - b) < 1e-9
+
+
+def test_oracle_cross_attention_against_differences():
+    q, k, v = (rnd(2, 3, 4, 5).requires_grad_(), rnd(2, 6, 2, 5, seed=1).requires_grad_(), rnd(2, 6, 2, 5, seed=2).requires_grad_())
+    keep = torch.ones(2, 6, dtype=torch.bool)
+    keep[0, 2] = False
+    keep[1] = False
+    assert torch.autograd.gradcheck(lambda *t: orc.cross_attn(*t, keep), (q, k, v))
+    full = torch.ones(2, 6, dtype=torch.bool)
+    ref = torch.nn.functional.scaled_dot_product_attention(*(t.detach().transpose(1, 2) for t in (q, k.repeat_interleave(2, 2),
+                                                                                                 v.repeat_interleave(2, 2))))
+    assert torch.allclose(orc.cross_attn(q, k, v, full).detach(), ref.transpose(1, 2))
+
+
+@pytest.mark.parametrize("post", [None, "layer", "rms"])
+@pytest.mark.parametrize("pre", [None, "layer", "rms"])
+@pytest.mark.parametrize("per_sample", [False, True])
+def test_oracle_norm_gate_residual_against_differences(post, pre, per_sample):
+    B, N, D = 3, 2, 5
+    x, u = rnd(B, N, D).requires_grad_(), rnd(B, N, D, seed=1).requires_grad_()
+    gate = (rnd(B, D, seed=2) if per_sample else rnd(D, seed=2)).requires_grad_()
+    kw = {}
+    for side, kind in (("post", post), ("pre", pre)):
+        if kind:
+            kw[side + "_weight"] = rnd(D, seed=3).requires_grad_()
+            kw[side + "_bias"] = rnd(D, seed=4).requires_grad_()
+    keys = list(kw)
+    s = torch.tensor([1.0, 0.0, 1.25], dtype=torch.float64)
+
+    def f(x, u, gate, *p):
+        y, h = orc.norm_gate_residual(x, u, gate, s, 0.75, post, pre=pre, **dict(zip(keys, p)))
+        return y if h is None else (y, h)
+    assert torch.autograd.gradcheck(f, (x, u, gate, *kw.values()))
+
+
+# ---------------------------------------------------------------------------------------------- refusals
+def test_rope_refusals():
+    q, k = torch.zeros(2, 3, 4, 16), torch.zeros(2, 3, 2, 16)
+    pos = torch.zeros(3, 2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="batch, tokens, heads"):
+        ops.rope_axes(q[0], k, pos, (4, 4))
+    with pytest.raises(ValueError, match="agree"):
+        ops.rope_axes(q, k[:, :2], pos, (4, 4))
+    with pytest.raises(ValueError, match="agree"):
+        ops.rope_axes(q, k.bfloat16(), pos, (4, 4))
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        ops.rope_axes(q.half(), None, pos, (4, 4))
+    for sections in ((), (0, 4), (1, 1, 1, 1, 1)):
+        with pytest.raises(ValueError, match="sections"):
+            ops.rope_axes(q, k, pos, sections)
+    with pytest.raises(ValueError, match="the head has 16"):
+        ops.rope_axes(q, k, pos, (4, 5))
+    with pytest.raises(TypeError, match="positions are"):
+        ops.rope_axes(q, k, pos.double(), (4, 4))
+    with pytest.raises(ValueError, match="must be"):
+        ops.rope_axes(q, k, pos[:, :1], (4, 4))
+    for base in (1.0, 0.5, (100.0,), float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="base"):
+            ops.rope_axes(q, k, pos, (4, 4), base=base)
+    with pytest.raises(ValueError, match="one base"):
+        ops.rope_axes(q, k, pos, (4, 4), base=(10.0, 100.0), shared_ladder=True)
+    with pytest.raises(RuntimeError, match="outside of autograd"):
+        ops.rope_axes(q.clone().requires_grad_(), k, pos, (4, 4), inplace=True)
+    with pytest.raises(ValueError, match="broadcast"):
+        ops.rope_axes(q[:1].expand(2, 3, 4, 16), k, pos, (4, 4), inplace=True)
+    with pytest.raises(ValueError, match="unit stride"):
+        ops.rope_axes(q.transpose(2, 3), None, torch.zeros(3, 1, dtype=torch.int64), (2,), inplace=True)
+    with pytest.raises(ValueError, match="apart"):
+        ops.rope_axes(q, q, pos, (4, 4), inplace=True)
+    for inplace in (False, True):
+        with pytest.raises(RuntimeError, match="ROCm device tensors"):
+            ops.rope_axes(q, k, pos, (4, 4), inplace=inplace)
+
+
+def test_cross_attn_refusals():
+    q, k = torch.zeros(2, 3, 4, 16), torch.zeros(2, 5, 2, 16)
+    with pytest.raises(ValueError, match="batch, tokens, heads"):
+        ops.cross_attn(q[0], k, k)
+    with pytest.raises(TypeError, match="share a dtype"):
+        ops.cross_attn(q, k, k.bfloat16())
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        ops.cross_attn(q.half(), k.half(), k.half())
+    for kk, vv in ((k, k[:, :4]), (k[:1], k[:1]), (k[..., :8], k[..., :8])):
+        with pytest.raises(ValueError, match="must be"):
+            ops.cross_attn(q, kk, vv)
+    with pytest.raises(ValueError, match="cannot share"):
+        ops.cross_attn(q, torch.zeros(2, 5, 3, 16), torch.zeros(2, 5, 3, 16))
+    big = torch.zeros(1, 1, 1, 129)
+    with pytest.raises(ValueError, match="exceed"):
+        ops.cross_attn(big, big, big)
+    keep, lens = torch.ones(2, 5, dtype=torch.bool), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not both"):
+        ops.cross_attn(q, k, k, kv_len=lens, key_mask=keep)
+    for bad in (lens.float(), lens[:1], lens[:, None]):
+        with pytest.raises(ValueError, match="kv_len"):
+            ops.cross_attn(q, k, k, kv_len=bad)
+    for bad in (keep.int(), keep[:, :4], keep[0]):
+        with pytest.raises(ValueError, match="key_mask"):
+            ops.cross_attn(q, k, k, key_mask=bad)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            ops.cross_attn(q, k, k, scale=scale)
+    with pytest.raises(RuntimeError, match="ROCm device tensors"):
+        ops.cross_attn(q, k, k)
+
+
+def test_norm_gate_residual_refusals():
+    x = torch.zeros(2, 3, 8)
+    w = torch.ones(8)
+    with pytest.raises(ValueError, match="alike"):
+        ops.norm_gate_residual(x, x[:, :2])
+    with pytest.raises(ValueError, match="alike"):
+        ops.norm_gate_residual(x[0], x[0])
+    with pytest.raises(TypeError, match="bf16 residual"):
+        ops.norm_gate_residual(x.bfloat16(), x)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        ops.norm_gate_residual(x.half(), x.half())
+    wide = torch.zeros(1, 1, 8193)
+    with pytest.raises(ValueError, match="outside"):
+        ops.norm_gate_residual(wide, wide)
+    with pytest.raises(ValueError, match="layer"):
+        ops.norm_gate_residual(x, x, post="batch")
+    with pytest.raises(ValueError, match="without post"):
+        ops.norm_gate_residual(x, x, post_weight=w)
+    with pytest.raises(ValueError, match="pre_bias must be"):
+        ops.norm_gate_residual(x, x, pre="layer", pre_bias=w[:4])
+    with pytest.raises(ValueError, match="pre_weight must be"):
+        ops.norm_gate_residual(x, x, pre="layer", pre_weight=w.bfloat16())
+    with pytest.raises(ValueError, match="gate"):
+        ops.norm_gate_residual(x, x, gate=torch.zeros(3, 8))
+    with pytest.raises(ValueError, match="branch_scale"):
+        ops.norm_gate_residual(x, x, branch_scale=torch.ones(3))
+    with pytest.raises(ValueError, match="not differentiated"):
+        ops.norm_gate_residual(x, x, branch_scale=torch.ones(2).requires_grad_())
+    with pytest.raises(RuntimeError, match="ROCm device tensors"):
+        ops.norm_gate_residual(x, x)
+
+
+# ---------------------------------------------------------------------------------------------- C ABI without a device
+CHECKS = r"""
+import ctypes, os, sys
+sys.path.insert(0, sys.argv[2])
+if sys.argv[1]:
+    os.environ["VITMI_LIB"] = sys.argv[1]
+from visiontransformer_amd import _lib, ops
+lib, at = _lib.lib, ctypes.addressof
+big = 2 ** 31 - 1
+assert lib.vitmi_rope_axes(None, None) == -1
+a = ops._RopeArgs()
+def rope(**kw):
+    for k, v in dict(dict(dt=1, axes=1, pos_type=1, B=1, N=1, DH=64), **kw).items():
+        setattr(a, k, v)
+    return lib.vitmi_rope_axes(at(a), None)
+a.t[0].heads = 1
+a.sections[0] = 16
+a.log2_base[0] = 13.3
+assert rope(N=0) == 0 and rope(B=0) == 0
+for bad in (dict(dt=2), dict(axes=0), dict(axes=5), dict(pos_type=3), dict(B=-1), dict(DH=31), dict()):
+    assert rope(**bad) == -1, bad               # dict(): null pointers
+a.sections[0] = big
+assert rope(DH=big) == -1
+a.sections[0], a.log2_base[0] = 16, 0.0
+assert rope() == -1
+x = ops._XattnArgs()
+def xattn(fn, **kw):
+    base = dict(dt=1, B=1, Nq=1, Nk=1, Hq=2, Hk=1, D=64, scale=1.0)
+    for k, v in dict(base, **kw).items():
+        setattr(x, k, v)
+    return fn(at(x), None, None)
+f, b = lib.vitmi_cross_attn_fwd, lib.vitmi_cross_attn_bwd
+assert f(None, None, None) == -1 and b(None, None, None) == -1
+assert xattn(f, B=0) == 0 and xattn(f, Nq=0) == 0
+for fn in (f, b):
+    for bad in (dict(dt=2), dict(Nq=-1), dict(Hq=3, Hk=2), dict(Hk=0), dict(scale=0.0), dict(scale=float("inf")),
+                dict(scale=float("nan")), dict(Nk=big), dict(Nq=big), dict(Hq=big - 1, Nq=4), dict()):
+        assert xattn(fn, **bad) == -1, bad
+    assert xattn(fn, D=129) == -3
+assert xattn(b, Nk=0) == -1
+for dt in (0, 1):
+    for s in ((1, 1, 1, 1, 1, 1), (2, 4096, 4609, 16, 4, 128), (8, 1, 16411, 32, 8, 128), (1, 1, big - 300, 1, 1, 128),
+              (4096, 197, 197, 12, 12, 64), (1, big - 300, 1, 1, 1, 1), (65535, 1, 1, 128, 1, 128)):
+        assert lib.vitmi_cross_attn_fwd_workspace_bytes(dt, *s) >= 0
+        assert lib.vitmi_cross_attn_bwd_workspace_bytes(dt, *s) > 0
+    assert lib.vitmi_cross_attn_bwd_workspace_bytes(dt, 1, big, 1, 2, 1, 1) == 0
+    assert lib.vitmi_cross_attn_fwd_workspace_bytes(dt, 1, 1, 1, 3, 2, 1) == 0
+n = ops._NgrArgs()
+def ngr(fn, **kw):
+    for k, v in dict(dict(dt_x=1, dt_u=1, B=1, N=1, D=8, post=1, pre=1, eps=1e-6, res_scale=1.0), **kw).items():
+        setattr(n, k, v)
+    return fn(at(n), None) if fn is nf else fn(at(n), None, None)
+nf, nb = lib.vitmi_norm_gate_residual_fwd, lib.vitmi_norm_gate_residual_bwd
+assert nf(None, None) == -1 and nb(None, None, None) == -1
+assert ngr(nf, B=0) == 0 and ngr(nf, N=0) == 0
+for fn in (nf, nb):
+    for bad in (dict(dt_x=2), dict(dt_x=1, dt_u=0), dict(D=0), dict(N=-1), dict(post=3), dict(pre=-1), dict()):
+        assert ngr(fn, **bad) == -1, bad
+    assert ngr(fn, D=8193) == -3
+for s in ((1, 1, 1, 0), (256, 197, 768, 0), (65536, 1, 8192, 1), (big, 1, 8192, 0), (1, big, 8192, 1)):
+    assert lib.vitmi_norm_gate_residual_bwd_workspace_bytes(*s) > 0
+print("ok")
+"""
+
+
+@pytest.mark.parametrize("sanitized", [False, True])
+def test_c_abi_checks_and_sizes(sanitized):
+    path = os.path.join(ROOT, "visiontransformer_amd", "libvitmi_hip_hostsan.so") if sanitized else ""
+    if sanitized and not os.path.exists(path):
+        pytest.skip("host-sanitized library not built")
+    r = subprocess.run([sys.executable, "-c", CHECKS, path, ROOT], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), (r.returncode, r.stdout, r.stderr[-2000:])
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "%s/include/vitmi.h"\nint main(void) { printf("%%zu %%zu %%zu %%zu", '
+                   'sizeof(vitmi_rope_tensor), sizeof(vitmi_rope_args), sizeof(vitmi_xattn_args), sizeof(vitmi_ngr_args)); '
+                   'return 0; }\n' % ROOT)
+    exe = str(tmp_path / "sizes")
+    subprocess.run(["gcc", str(src), "-o", exe], check=True)
+    sizes = [int(v) for v in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert sizes == [ctypes.sizeof(t) for t in (ops._RopeTensor, ops._RopeArgs, ops._XattnArgs, ops._NgrArgs)]
+
+
+def test_entry_points_are_bound():
+    for name in ("vitmi_rope_axes", "vitmi_cross_attn_fwd", "vitmi_cross_attn_bwd", "vitmi_norm_gate_residual_fwd",
+                 "vitmi_norm_gate_residual_bwd"):
+        assert name in _lib.SIGNATURES and hasattr(_lib.lib, name)

@@ -1,0 +1,653 @@
+"""The decoder-block operators on the GPU against their definitions in 64 bits (oracle/decoder_oracle.py, pinned to
+differences by tests/test_decoder_ops.py).
+
+Tolerances are error bounds, element by element, built from the operator's own terms in 64 bits: a rounding to the output
+type is off by half a step (eps / 2 of the value), 32-bit arithmetic by 2^-24 of every term per operation along the
+longest chain of operations, and in the bf16 attention the probabilities and score gradients are rounded to bf16
+(2^-8 of each) before their products."""
+import math
+
+import pytest
+import torch
+
+from oracle import decoder_oracle as orc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+F, H = torch.float32, torch.bfloat16
+
+
+def ops():
+    from visiontransformer_amd import ops as o
+    return o
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def half_step(t):
+    return torch.finfo(t.dtype).eps / 2
+
+
+def within(name, got, ref, tol):
+    """got against ref with an elementwise bound on its 32-bit arithmetic, plus half a step of its type."""
+    got64 = got.detach().double().cpu()
+    assert got64.shape == ref.shape, (name, got64.shape, ref.shape)
+    assert torch.isfinite(got64).all(), f"{name}: not finite"
+    h = half_step(got)
+    bound = h * ref.abs() + (1 + h) * tol + 1e-37
+    bad = (got64 - ref).abs() > bound
+    assert not bad.any(), (f"{name}: {int(bad.sum())} of {bad.numel()} beyond the bound, worst "
+                           f"{((got64 - ref).abs() / bound).max().item():.3g} of it")
+
+
+# ---------------------------------------------------------------------------------------------- rotary positions
+def rope_tol(x, P, interleaved):
+    """The reduced angle is off by 2^-25 of at most an eighth of a turn and sincospi by 2 ulp, so cos and sin by under 2^-22;
+    two products and a sum add 2 U: in all under 2^-21 of |x1| + |x2|."""
+    a = x.abs()
+    t = torch.zeros_like(a)
+    i1 = slice(0, 2 * P, 2) if interleaved else slice(0, P)
+    i2 = slice(1, 2 * P, 2) if interleaved else slice(P, 2 * P)
+    t[..., i1] = t[..., i2] = (a[..., i1] + a[..., i2]) * 2.0 ** -21
+    return t
+
+
+ROPE = [  # B, N, Hq, Hk, D, sections, positions
+    (1, 1, 1, 0, 2, (1,), "i64"), (2, 5, 3, 1, 64, (16, 16), "i32"), (3, 197, 2, 2, 64, (16, 16), "f32"),
+    (2, 33, 2, 1, 66, (5, 7), "i64"), (1, 9, 2, 2, 40, (10, 10), "i64"), (2, 7, 4, 1, 80, (8, 16, 16), "far"),
+    (1, 3, 1, 1, 512, (256,), "far"), (2, 17, 3, 3, 9, (2, 1), "i32"), (2, 65, 1, 0, 128, (4, 4, 4, 4), "f32"),
+    (1, 1030, 2, 1, 32, (16,), "far"), (40, 3, 1, 1, 24, (3, 1), "i64"),
+]
+
+
+@pytest.mark.parametrize("case", ROPE, ids=str)
+@pytest.mark.parametrize("dtype", [F, H], ids=["f32", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_axes(case, dtype, interleaved):
+    B, N, Hq, Hk, D, sections, kind = case
+    g = gen(B * 1000 + N)
+    per_batch = kind in ("i32", "far")
+    shared = kind == "far"
+    shape = (B, N, len(sections)) if per_batch else (N, len(sections))
+    if kind == "f32":
+        pos = torch.rand(shape, generator=g) * 60 - 20
+    else:
+        hi = 2_000_000 if kind == "far" else 50
+        pos = torch.randint(-hi, hi, shape, generator=g).to(torch.int32 if kind == "i32" else torch.int64)
+    base = 10000.0 if kind != "i64" else tuple(100.0 * (a + 1) for a in range(len(sections)))
+    packed = torch.randn(B, N, Hq + Hk + 1, D, generator=g).to(dtype)           # strided views of one buffer
+    dev = packed.to(DEV).requires_grad_()
+    q, k = dev[:, :, :Hq], (dev[:, :, Hq:Hq + Hk] if Hk else None)
+    res = ops().rope_axes(q, k, pos.to(DEV), sections, base, interleaved, shared)
+    outs = list(res) if Hk else [res]
+    refin = packed.double().requires_grad_()
+    refs = [orc.rope_axes(t, pos, sections, base, interleaved, shared)
+            for t in ([refin[:, :, :Hq]] + ([refin[:, :, Hq:Hq + Hk]] if Hk else []))]
+    ups = [torch.randn(r.shape, generator=g).to(dtype) for r in refs]
+    grad, = torch.autograd.grad(outs, [dev], [u.to(DEV) for u in ups])
+    rgrad, = torch.autograd.grad(refs, [refin], [u.double() for u in ups])
+    P = sum(sections)
+    for n, o, r, x in zip("qk", outs, refs, (refin[:, :, :Hq], refin[:, :, Hq:Hq + Hk])):
+        within(n, o, r.detach(), rope_tol(x.detach(), P, interleaved))
+    up = torch.zeros_like(rgrad)
+    up[:, :, :Hq] = ups[0].double()
+    if Hk:
+        up[:, :, Hq:Hq + Hk] = ups[1].double()
+    within("grad", grad, rgrad, rope_tol(up, P, interleaved))
+    # the same without a graph, and in place in the packed buffer: bit for bit, the other slot untouched
+    with torch.no_grad():
+        again = ops().rope_axes(q, k, pos.to(DEV), sections, base, interleaved, shared)
+        buf = dev.detach().clone()
+        ver = buf._version
+        ops().rope_axes(buf[:, :, :Hq], buf[:, :, Hq:Hq + Hk] if Hk else None, pos.to(DEV), sections, base, interleaved, shared,
+                        inplace=True)
+    assert buf._version > ver
+    for a, o in zip(again if Hk else [again], outs):
+        assert torch.equal(a, o)
+    assert torch.equal(buf[:, :, :Hq], outs[0]) and torch.equal(buf[:, :, Hq + Hk:], dev[:, :, Hq + Hk:])
+    if Hk:
+        assert torch.equal(buf[:, :, Hq:Hq + Hk], outs[1])
+
+
+def test_rope_gradient_against_differences():
+    """A rotation is linear: <grad, d> is exactly f(x + d) - f(x) summed against the upstream gradient."""
+    g = gen(5)
+    x = torch.randn(2, 19, 3, 32, generator=g).to(DEV).requires_grad_()
+    pos = torch.randint(0, 1000, (19, 2), generator=g).to(DEV)
+    up, d = torch.randn(2, 19, 3, 32, generator=g).to(DEV), torch.randn(2, 19, 3, 32, generator=g).to(DEV)
+    f = lambda t: ops().rope_axes(t, None, pos, (7, 9))
+    grad, = torch.autograd.grad(f(x), x, up)
+    with torch.no_grad():
+        diff = ((f(x + d).double() - f(x).double()) * up.double()).sum()
+    # every term of the sum is good to 2^-20 of |x| + |d| + |x + d| < 10 times |up|
+    assert abs(diff - (grad.double() * d.double()).sum()) < 2.0 ** -20 * 10 * up.double().abs().sum()
+
+
+@pytest.mark.parametrize("shape", [(0, 3, 2, 16), (2, 0, 2, 16)])
+def test_rope_without_tokens(shape):
+    q = torch.zeros(shape, device=DEV).requires_grad_()
+    pos = torch.zeros(shape[1], 1, dtype=torch.int64, device=DEV)
+    y = ops().rope_axes(q, None, pos, (4,))
+    assert y.shape == q.shape
+    assert torch.autograd.grad(y.sum(), q)[0].shape == q.shape
+
+
+def test_rope_one_gradient_only_and_strided_gradients():
+    g = gen(6)
+    q, k = (torch.randn(2, 5, 2, 16, generator=g).to(DEV).requires_grad_() for _ in range(2))
+    pos = torch.randint(0, 9, (2, 5, 2), generator=g).to(DEV)
+    yq, yk = ops().rope_axes(q, k, pos, (3, 4))
+    up = torch.randn(2, 2, 16, 5, generator=g).to(DEV).permute(0, 3, 1, 2)        # no unit stride over the head dim
+    gk, = torch.autograd.grad(yk, k, up)
+    ref = ops().rope_axes(up.contiguous(), None, -pos, (3, 4))
+    within("dk", gk, ref.double().cpu(), rope_tol(up.double().cpu(), 7, False) * 2)
+
+
+# ---------------------------------------------------------------------------------------------- cross attention
+def attention_bounds(q, k, v, keep, do, dtype, o_step):
+    """Values and elementwise error bounds of (o, dq, dk, dv) in 64 bits.  Chains: D + 4 operations for a score, Nk + 8
+    for a sum over keys, R + 8 for one over rows; exp2 and log2 of the hardware within 2^-22 of their value, their
+    arguments rounded to 2^-24 of themselves (|argument| <= amax)."""
+    B, Nq, Hq, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    G, scale = Hq // Hk, D ** -0.5
+    r = 2.0 ** -8 if dtype == H else 0.0
+    out = {n: torch.zeros_like(t) for n, t in zip(("o", "dq", "dk", "dv"), (q, q, k, v))}
+    tol = {n: torch.zeros_like(t) for n, t in out.items()}
+    for b in range(B):
+        idx = keep[b].nonzero().flatten()
+        if idx.numel() == 0:
+            continue
+        for h in range(Hq):
+            qq, kk, vv, g = q[b, :, h], k[b, idx, h // G], v[b, idx, h // G], do[b, :, h]
+            s = scale * qq @ kk.T
+            sabs = scale * qq.abs() @ kk.abs().T
+            p = torch.softmax(s, -1)
+            amax = 1.4427 * s.abs().amax(-1, keepdim=True) + 16 + math.log2(len(idx))
+            es = (D + 4) * U * sabs.amax(-1, keepdim=True)
+            ep = 2 * es + 4 * U * amax + 2.0 ** -20
+            o = p @ vv
+            to = (p @ vv.abs()) * (ep + r + (Nk + 8) * U)
+            dp = g @ vv.T
+            edp = (D + 4) * U * (g.abs() @ vv.abs().T)
+            delta = (g * o).sum(-1, keepdim=True)
+            edelta = ((g.abs() * (to + o_step * (o.abs() + to))).sum(-1, keepdim=True)
+                      + (D + 4) * U * (g.abs() * o.abs()).sum(-1, keepdim=True))
+            ds = p * (dp - delta)
+            eds = p * ((ep + U) * (dp - delta).abs() + edp + edelta) * (1 + ep) + r * ds.abs()
+            eds = eds * (1 + r)
+            out["o"][b, :, h], tol["o"][b, :, h] = o, to
+            out["dq"][b, :, h] = scale * ds @ kk
+            tol["dq"][b, :, h] = scale * (eds @ kk.abs() + (Nk + 8) * U * (ds.abs() + eds) @ kk.abs())
+            out["dk"][b, idx, h // G] += scale * ds.T @ qq
+            tol["dk"][b, idx, h // G] += scale * (eds.T @ qq.abs() + (G * Nq + 8) * U * (ds.abs() + eds).T @ qq.abs())
+            out["dv"][b, idx, h // G] += p.T @ g
+            tol["dv"][b, idx, h // G] += (p * (ep + r)).T @ g.abs() * (1 + r) + (G * Nq + 8) * U * p.T @ g.abs() * (1 + r)
+    return out, tol
+
+
+XATTN = [  # B, Nq, Nk, Hq, Hk, D, mask
+    (1, 1, 1, 1, 1, 8, "none"), (2, 1, 197, 3, 3, 64, "none"), (3, 1, 1000, 8, 2, 128, "len"), (2, 5, 77, 4, 1, 40, "keys"),
+    (2, 33, 65, 2, 2, 32, "len"), (1, 130, 129, 2, 1, 96, "keys"), (2, 197, 333, 2, 2, 64, "none"),
+    (2, 64, 31, 3, 3, 16, "empty"), (1, 65, 64, 1, 1, 80, "len"), (2, 17, 50, 2, 1, 13, "keys"), (1, 3, 700, 2, 2, 1, "len"),
+    (2, 300, 1, 1, 1, 64, "none"), (1, 128, 128, 2, 2, 128, "none"), (1, 600, 70, 4, 2, 72, "empty"),
+    (1, 2, 4100, 1, 1, 64, "sparse"), (4, 70, 260, 1, 1, 127, "len"),
+]
+
+
+def xattn_inputs(case, dtype, seed=0):
+    B, Nq, Nk, Hq, Hk, D, mask = case
+    g = gen(seed + Nq * 7 + Nk)
+    q = torch.randn(B, Nq, Hq, D, generator=g).to(dtype)
+    kv = torch.randn(B, Nk, 2, Hk, D, generator=g).to(dtype)
+    do = torch.randn(B, Nq, Hq, D, generator=g).to(dtype)
+    lens = keep = None
+    if mask == "len":
+        lens = torch.randint(0, Nk + 1, (B,), generator=g).to(torch.int32 if Nq % 2 else torch.int64)
+        lens[0] = Nk
+    elif mask == "keys":
+        keep = torch.rand(B, Nk, generator=g) < 0.6
+    elif mask == "empty":
+        keep = torch.rand(B, Nk, generator=g) < 0.6
+        keep[0] = False
+    elif mask == "sparse":                                  # whole tiles without a key, one key in the last
+        keep = torch.zeros(B, Nk, dtype=torch.bool)
+        keep[:, 70:75] = keep[:, Nk - 1] = True
+    return q, kv, do, lens, keep
+
+
+@pytest.mark.parametrize("case", XATTN, ids=str)
+@pytest.mark.parametrize("dtype", [F, H], ids=["f32", "bf16"])
+def test_cross_attn(case, dtype):
+    B, Nq, Nk = case[:3]
+    q, kv, do, lens, keep = xattn_inputs(case, dtype)
+    allowed = orc.allowed_keys(B, Nk, lens, keep)
+    ref, tol = attention_bounds(q.double(), kv[:, :, 0].double(), kv[:, :, 1].double(), allowed, do.double(), dtype,
+                                half_step(q))
+    # what masked keys hold must not matter: infinities, NaN and the type's lowest value, by turns
+    junk = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).min])
+    off = ~allowed
+    kv[off] = junk.repeat(off.sum() // 4 + 1)[:off.sum()].to(dtype)[:, None, None, None].expand(-1, *kv.shape[2:])
+    qd, kvd = q.to(DEV).requires_grad_(), kv.to(DEV).requires_grad_()
+    m = dict(kv_len=None if lens is None else lens.to(DEV), key_mask=None if keep is None else keep.to(DEV))
+    o = ops().cross_attn(qd, kvd[:, :, 0], kvd[:, :, 1], **m)
+    within("o", o, ref["o"], tol["o"])
+    dq, dkv = torch.autograd.grad(o, (qd, kvd), do.to(DEV))
+    within("dq", dq, ref["dq"], tol["dq"])
+    within("dk", dkv[:, :, 0], ref["dk"], tol["dk"])
+    within("dv", dkv[:, :, 1], ref["dv"], tol["dv"])
+    assert not dkv[off.to(DEV)].any()                       # exactly zero
+    with torch.no_grad():                                   # the call that keeps nothing, and a repeat: bit for bit
+        assert torch.equal(ops().cross_attn(qd, kvd[:, :, 0], kvd[:, :, 1], **m), o)
+    again = torch.autograd.grad(ops().cross_attn(qd, kvd[:, :, 0], kvd[:, :, 1], **m), (qd, kvd), do.to(DEV))
+    assert torch.equal(again[0], dq) and torch.equal(again[1], dkv)
+
+
+@pytest.mark.parametrize("dtype", [F, H], ids=["f32", "bf16"])
+@pytest.mark.parametrize("Nq,D", [(3, 64), (90, 64), (90, 24)])
+def test_cross_attn_large_scores(dtype, Nq, D):
+    """Scores of several hundred whose running maximum keeps growing from tile to tile: the softmax is nearly one-hot."""
+    g = gen(11)
+    B, Nk, Hh = 1, 400, 2
+    q = torch.randn(B, Nq, Hh, D, generator=g).to(dtype)
+    k = (torch.randn(B, Nk, Hh, D, generator=g) * torch.linspace(1, 40, Nk)[None, :, None, None]).to(dtype)
+    v, do = torch.randn(B, Nk, Hh, D, generator=g).to(dtype), torch.randn(B, Nq, Hh, D, generator=g).to(dtype)
+    ref, tol = attention_bounds(q.double(), k.double(), v.double(), torch.ones(B, Nk, dtype=torch.bool), do.double(), dtype,
+                                half_step(q))
+    args = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    o = ops().cross_attn(*args)
+    for n, t in zip(("o", "dq", "dk", "dv"), (o,) + torch.autograd.grad(o, args, do.to(DEV))):
+        within(n, t, ref[n], tol[n])
+
+
+def test_cross_attn_lengths_outside_the_range_are_clamped():
+    g = gen(3)
+    q, k, v = (torch.randn(4, n, 2, 32, generator=g).to(DEV) for n in (3, 9, 9))
+    out = ops().cross_attn(q, k, v, kv_len=torch.tensor([-5, 0, 9, 2 ** 40], device=DEV))
+    full = ops().cross_attn(q, k, v)
+    assert not out[:2].any() and torch.equal(out[2:], full[2:])
+
+
+@pytest.mark.parametrize("dims", [(0, 3, 5), (2, 0, 5), (2, 3, 0)])
+def test_cross_attn_with_empty_axes(dims):
+    B, Nq, Nk = dims
+    q = torch.ones(B, Nq, 2, 16, device=DEV).requires_grad_()
+    k, v = (torch.ones(B, Nk, 1, 16, device=DEV).requires_grad_() for _ in range(2))
+    o = ops().cross_attn(q, k, v)
+    assert o.shape == q.shape and not o.any()
+    for t, gr in zip((q, k, v), torch.autograd.grad(o.sum(), (q, k, v))):
+        assert gr.shape == t.shape and not gr.any()
+
+
+def test_cross_attn_broadcast_states_and_head_slices():
+    """Encoder states shared by the batch (stride 0), queries sliced out of a wider projection, keys in [B, H, N, D]
+    order; the gradient of the shared states is the sum over the batch."""
+    g = gen(9)
+    wide = torch.randn(3, 20, 5, 48, generator=g).to(DEV).requires_grad_()
+    kv = torch.randn(2, 1, 2, 37, 32, generator=g).to(DEV).requires_grad_()
+    do = torch.randn(3, 20, 4, 32, generator=g).to(DEV)
+    q = wide[:, :, 1:, 8:40]
+    k, v = (t.transpose(1, 2).expand(3, 37, 2, 32) for t in kv)
+    o = ops().cross_attn(q, k, v)
+    gw, gkv = torch.autograd.grad(o, (wide, kv), do)
+    ref, tol = attention_bounds(*(t.detach().double().cpu() for t in (q, k, v)), torch.ones(3, 37, dtype=torch.bool),
+                                do.double().cpu(), F, half_step(o))
+    within("o", o, ref["o"], tol["o"])
+    within("dq", gw[:, :, 1:, 8:40], ref["dq"], tol["dq"])
+    assert not gw[:, :, 0].any() and not gw[..., :8].any() and not gw[..., 40:].any()
+    for i, n in enumerate(("dk", "dv")):
+        # the three samples' gradients are rounded one by one and added by torch
+        within(n, gkv[i, 0].transpose(0, 1), ref[n].sum(0), tol[n].sum(0) + 4 * U * ref[n].abs().sum(0))
+
+
+def test_cross_attn_unaligned_views():
+    """Pointers off a 16-byte border and odd strides take the element-wise loads."""
+    g = gen(10)
+    base = [torch.randn(2, n, 2, 33, generator=g).to(DEV, H) for n in (21, 45, 45, 21)]
+    q, k, v = (t[..., 1:].detach().requires_grad_() for t in base[:3])
+    o = ops().cross_attn(q, k, v)
+    got = (o,) + torch.autograd.grad(o, (q, k, v), base[3][..., 1:])
+    ref, tol = attention_bounds(*(t[..., 1:].double().cpu() for t in base[:3]), torch.ones(2, 45, dtype=torch.bool),
+                                base[3][..., 1:].double().cpu(), H, half_step(o))
+    for n, t in zip(("o", "dq", "dk", "dv"), got):
+        within(n, t, ref[n], tol[n])
+
+
+def test_cross_attn_states_beyond_32_bit_offsets():
+    """Keys whose element offsets pass 2^31: a long cache kept as [N, B, H, D], read at its far end."""
+    N, B, Hh, D = 140000, 2, 2, 64
+    wide = 4096                                             # 2 * 140000 * 8192 elements: 4.6 G bytes a tensor
+    k = torch.empty(N, B, wide * 2, dtype=H, device=DEV)
+    sl = k[:, :, -Hh * D:].unflatten(-1, (Hh, D)).transpose(0, 1)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    small = torch.randn(B, N, Hh, D, generator=g, device=DEV).to(H)
+    sl.copy_(small)
+    q = torch.randn(B, 3, Hh, D, generator=g, device=DEV).to(H)
+    keep = torch.zeros(B, N, dtype=torch.bool, device=DEV)
+    keep[:, N - 1000:] = True
+    assert torch.equal(ops().cross_attn(q, sl, sl, key_mask=keep), ops().cross_attn(q, small, small, key_mask=keep))
+
+
+# ---------------------------------------------------------------------------------------------- residual update
+NGR = [  # B, N, D, post, pre, gate, drop
+    (1, 1, 8, None, None, None, False), (2, 3, 768, "layer", "layer", "channel", False), (5, 7, 192, "layer", "layer", "sample", True),
+    (3, 50, 100, "rms", "layer", "channel", True), (2, 9, 1001, "layer", "rms", "sample", False), (4, 2, 1, "rms", "rms", None, False),
+    (2, 5, 4096, "rms", "rms", "sample", False), (1, 3, 8192, "layer", "layer", "channel", False), (2, 2, 8191, "rms", None, "channel", False),
+    (3, 40, 1028, None, "layer", "sample", True), (2, 33, 384, "layer", None, None, True), (700, 1, 64, "layer", "layer", "sample", True),
+    (1, 600, 36, "rms", "rms", "channel", False), (2, 3, 2052, "layer", "layer", "channel", True), (3, 4, 5000, None, "rms", None, False),
+]
+
+
+def norm_bound(v, ev, kind, w, eps):
+    """A norm's value and the bound on the computed one for an input off by ev: sums run over at most 24 additions deep,
+    so 64 U of the terms covers mean, deviations, variance and root."""
+    w = torch.ones(v.shape[-1], dtype=v.dtype) if w is None else w
+    mean = lambda t: t.mean(-1, keepdim=True)
+    c = v - mean(v) if kind == "layer" else v
+    r = 1 / (mean(c * c) + eps).sqrt()
+    vh = c * r
+    e = r * (ev + mean(ev)) + vh.abs() * r * ev.amax(-1, keepdim=True) + 64 * U * (r * (v.abs() + mean(v.abs())) * (1 + vh.abs()) + vh.abs())
+    return vh, e, r
+
+
+def ngr_reference(t, kw):
+    """Outputs and gradients by autograd of the definition in 64 bits, with elementwise bounds."""
+    loc = {n: v.double().clone().requires_grad_(n not in ("dy", "dh", "branch_scale")) if v is not None else None for n, v in t.items()}
+    y, h = orc.norm_gate_residual(**{n: v for n, v in loc.items() if n not in ("dy", "dh")}, **kw)
+    names = [n for n, v in loc.items() if v is not None and v.requires_grad]
+    outs, ups = [y], [loc["dy"]]
+    if h is not None:
+        outs, ups = [y, h], [loc["dy"], loc["dh"]]
+    grads = dict(zip(names, torch.autograd.grad(outs, [loc[n] for n in names], ups)))
+    d = {n: (None if v is None else v.detach()) for n, v in loc.items()}
+    eps, a, D = kw["eps"], abs(kw["res_scale"]), y.shape[-1]
+    rows = y.shape[0] * y.shape[1]
+    x, u = d["x"], d["u"]
+    one = torch.ones(D, dtype=torch.float64)
+    g = one if d["gate"] is None else d["gate"]
+    g = g if g.dim() == 1 else g[:, None]
+    s = torch.ones(x.shape[0], dtype=torch.float64) if d["branch_scale"] is None else d["branch_scale"]
+    s = s[:, None, None]
+    mean = lambda v: v.mean(-1, keepdim=True)
+    tol = {}
+    pw, pb = (one if d["post_weight"] is None else d["post_weight"]), (0 * one if d["post_bias"] is None else d["post_bias"])
+    if kw["post"]:
+        uh, euh, ru = norm_bound(u, torch.zeros_like(u), kw["post"], pw, eps)
+    else:
+        uh, euh, ru = u, torch.zeros_like(u), torch.ones_like(u[..., :1])
+    p = uh * pw + pb
+    sg = (s * g).abs()
+    tol["y"] = sg * pw.abs() * euh + 8 * U * (a * x.abs() + sg * ((uh * pw).abs() + pb.abs()))
+    et = torch.zeros_like(x)
+    tt = d["dy"]
+    if kw["pre"]:
+        qw = one if d["pre_weight"] is None else d["pre_weight"]
+        qb = 0 * one if d["pre_bias"] is None else d["pre_bias"]
+        yh, eyh, ry = norm_bound(y.detach(), tol["y"], kw["pre"], qw, eps)
+        tol["h"] = qw.abs() * eyh + 4 * U * ((yh * qw).abs() + qb.abs())
+        dh = d["dh"]
+        gh = dh * qw
+        c1 = mean(gh) if kw["pre"] == "layer" else 0
+        c2 = mean(gh * yh)
+        er = 64 * U + ry * tol["y"].amax(-1, keepdim=True)                      # relative error of ry
+        ec2 = mean(gh.abs() * eyh) + 64 * U * mean((gh * yh).abs())
+        core = gh - c1 - yh * c2
+        ecore = 4 * U * gh.abs() + 64 * U * mean(gh.abs()) + yh.abs() * ec2 + eyh * (c2.abs() + ec2) + 4 * U * (yh * c2).abs()
+        et = ry * (ecore * (1 + er) + core.abs() * er)
+        tt = tt + ry * core
+        n_sum = (rows + 64) * U
+        tol["pre_weight"] = (dh.abs() * eyh).sum((0, 1)) + n_sum * (dh * yh).abs().sum((0, 1))
+        tol["pre_bias"] = n_sum * dh.abs().sum((0, 1))
+    et = et + 4 * U * tt.abs()
+    tol["x"] = a * et + 4 * U * a * tt.abs()
+    st, est = (s * tt), s * et + 2 * U * (s * tt).abs()
+    n_sum = (rows + 64) * U
+    eA = est * uh.abs() + st.abs() * euh + est * euh
+    A, B = (st * uh).abs(), st.abs()
+    red = (lambda v: v.sum((0, 1))) if d["gate"] is None or d["gate"].dim() == 1 else (lambda v: v.sum(1))
+    tol["gate"] = pw.abs() * red(eA + n_sum * A) + pb.abs() * red(est + n_sum * B) + 4 * U * (pw.abs() * red(A) + pb.abs() * red(B))
+    tol["post_weight"] = (g.abs() * (eA + 2 * n_sum * A)).sum((0, 1))
+    tol["post_bias"] = (g.abs() * (est + 2 * n_sum * B)).sum((0, 1))
+    gu, egu = st * g * pw, est * (g * pw).abs() + 4 * U * (st * g * pw).abs()
+    if kw["post"]:
+        d1 = mean(gu) if kw["post"] == "layer" else 0
+        d2 = mean(gu * uh)
+        ed1 = mean(egu) + 64 * U * mean(gu.abs())
+        ed2 = mean(egu * uh.abs() + gu.abs() * euh + egu * euh) + 64 * U * mean((gu * uh).abs())
+        core = gu - d1 - uh * d2
+        ecore = egu + ed1 + uh.abs() * ed2 + euh * (d2.abs() + ed2) + 4 * U * (gu.abs() + mean(gu.abs()) + (uh * d2).abs())
+        tol["u"] = ru * (ecore + 66 * U * (core.abs() + ecore))
+    else:
+        tol["u"] = egu
+    return y.detach(), (None if h is None else h.detach()), grads, tol
+
+
+@pytest.mark.parametrize("case", NGR, ids=str)
+@pytest.mark.parametrize("types", [(H, H), (F, F), (F, H)], ids=["bf16", "f32", "mixed"])
+def test_norm_gate_residual(case, types):
+    B, N, D, post, pre, gate, drop = case
+    tx, tu = types
+    g = gen(B + N * 3 + D)
+    r = lambda *s, dt=F, sc=1.0, sh=0.0: (torch.randn(*s, generator=g) * sc + sh).to(dt)
+    t = dict(x=r(B, N, D, dt=tx, sc=1.5), u=r(B, N, D, dt=tu, sh=0.5),
+             gate=None if gate is None else (r(D, sc=0.5) if gate == "channel" else r(B, D, dt=tu, sc=0.5)), branch_scale=None)
+    if drop:
+        t["branch_scale"] = torch.where(torch.rand(B, generator=g) < 0.4, 0.0, 1.25)
+        t["branch_scale"][0] = 0.0
+    for side, kind in (("post", post), ("pre", pre)):
+        t[side + "_weight"] = r(D, sc=0.3, sh=1.0) if kind else None
+        t[side + "_bias"] = r(D, sc=0.3) if kind == "layer" else None
+    t["dy"], t["dh"] = r(B, N, D, dt=tx), (r(B, N, D, dt=tu) if pre else None)
+    kw = dict(post=post, pre=pre, res_scale=0.75, eps=1e-6)
+    y, h, grads, tol = ngr_reference(t, kw)
+    dev = {n: None if v is None else v.to(DEV) for n, v in t.items()}
+    if drop:
+        dev["u"][(t["branch_scale"] == 0).to(DEV)] = float("nan")               # an absent branch may hold anything
+    for n in grads:
+        dev[n].requires_grad_()
+    ins = {n: v for n, v in dev.items() if n not in ("dy", "dh")}
+    gy, gh = ops().norm_gate_residual(**ins, **kw)
+    within("y", gy, y, tol["y"])
+    outs, ups = [gy], [dev["dy"]]
+    if pre:
+        within("h", gh, h, tol["h"])
+        outs, ups = [gy, gh], [dev["dy"], dev["dh"]]
+    got = dict(zip(grads, torch.autograd.grad(outs, [dev[n] for n in grads], ups)))
+    for n in grads:
+        assert got[n].dtype == dev[n].dtype
+        within("d" + n, got[n], grads[n], tol[n])
+    with torch.no_grad():
+        ny, nh = ops().norm_gate_residual(**ins, **kw)
+    assert torch.equal(ny, gy) and (not pre or torch.equal(nh, gh))
+    again = torch.autograd.grad([v for v in ops().norm_gate_residual(**ins, **kw) if v is not None], [dev[n] for n in grads], ups)
+    for n, v in zip(grads, again):
+        assert torch.equal(v, got[n]), n                                        # sums in a fixed order
+
+
+def test_norm_gate_residual_views_and_partial_gradients():
+    """The tokens of a longer buffer without its class row, one gradient alone, no upstream gradient on one output."""
+    g = gen(21)
+    X = torch.randn(3, 11, 64, generator=g).to(DEV).requires_grad_()
+    Uu = torch.randn(3, 11, 80, generator=g).to(DEV).requires_grad_()
+    w = torch.randn(64, generator=g).to(DEV).requires_grad_()
+    dh = torch.randn(3, 10, 64, generator=g).to(DEV)
+    x, u = X[:, 1:], Uu[:, 1:, 16:]
+    y, h = ops().norm_gate_residual(x, u, gate=w, pre="layer")
+    y2, h2 = ops().norm_gate_residual(x.contiguous(), u.contiguous(), gate=w, pre="layer")
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+    full = torch.autograd.grad((y, h), (X, Uu, w), (torch.zeros_like(y), dh), retain_graph=True)
+    only_h = torch.autograd.grad(h, (X, Uu, w), dh, retain_graph=True)
+    for a, b in zip(full, only_h):
+        assert torch.equal(a, b)
+    only_w, = torch.autograd.grad(h, w, dh, retain_graph=True)
+    assert torch.equal(only_w, full[2])
+    only_y, = torch.autograd.grad(y, X, dh)
+    assert torch.equal(only_y[:, 1:], dh) and not only_y[:, 0].any()
+
+
+@pytest.mark.parametrize("shape", [(0, 3, 8), (2, 0, 8)])
+def test_norm_gate_residual_without_rows(shape):
+    x, u = (torch.zeros(shape, device=DEV).requires_grad_() for _ in range(2))
+    w = torch.ones(8, device=DEV).requires_grad_()
+    y, h = ops().norm_gate_residual(x, u, pre="rms", pre_weight=w)
+    gx, gw = torch.autograd.grad(h.sum() + y.sum(), (x, w))
+    assert y.shape == h.shape == gx.shape == x.shape and not gw.any()
+
+
+def test_norm_gate_residual_gradient_against_differences():
+    g = gen(31)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)
+    base = dict(x=r(2, 3, 48), u=r(2, 3, 48), gate=r(48), post_weight=r(48), post_bias=r(48), pre_weight=r(48), pre_bias=r(48))
+    up = (r(2, 3, 48), r(2, 3, 48))
+    f = lambda kw: sum((o.double() * w.double()).sum() for o, w in
+                       zip(ops().norm_gate_residual(post="layer", pre="layer", **kw), up))
+    leaf = {n: t.clone().requires_grad_() for n, t in base.items()}
+    grads = dict(zip(base, torch.autograd.grad(f(leaf), list(leaf.values()))))
+    e = 2.0 ** -7
+    with torch.no_grad():
+        for n in base:
+            d = r(*base[n].shape)
+            diff = (f({**base, n: base[n] + e * d}) - f({**base, n: base[n] - e * d})) / (2 * e)
+            want = (grads[n].double() * d.double()).sum()
+            # third derivatives enter with e^2 = 6e-5; 32-bit outputs with 2^-22 of 300 terms / e: under 2 % of the terms' size
+            assert abs(diff - want) < 0.02 * (grads[n].double() * d.double()).abs().sum(), n
+
+
+def test_cross_attn_gradient_against_differences():
+    g = gen(32)
+    r = lambda *s: torch.randn(*s, generator=g).to(DEV)
+    base = dict(q=r(2, 70, 2, 24), k=r(2, 45, 1, 24), v=r(2, 45, 1, 24))
+    up = r(2, 70, 2, 24)
+    lens = torch.tensor([45, 30], device=DEV)
+    f = lambda kw: (ops().cross_attn(kv_len=lens, **kw).double() * up.double()).sum()
+    leaf = {n: t.clone().requires_grad_() for n, t in base.items()}
+    grads = dict(zip(base, torch.autograd.grad(f(leaf), list(leaf.values()))))
+    e = 2.0 ** -6
+    with torch.no_grad():
+        for n in base:
+            d = r(*base[n].shape)
+            diff = (f({**base, n: base[n] + e * d}) - f({**base, n: base[n] - e * d})) / (2 * e)
+            want = (grads[n].double() * d.double()).sum()
+            # third derivatives enter with e^2 = 2.4e-4 of the terms, rounding with 2^-20 / e
+            assert abs(diff - want) < 0.02 * (grads[n].double() * d.double()).abs().sum(), n
+
+
+# ---------------------------------------------------------------------------------------------- together
+def decoder_block(lib, t, keep, pos_q, pos_k, cast):
+    """norm -> rotary queries and keys -> cross attention -> residual with gate and the next norm."""
+    if lib is orc:
+        rope = lambda x, p: orc.rope_axes(x, p, (4, 4))
+        attn = lambda q, k, v: orc.cross_attn(q, k, v, keep)
+    else:
+        rope = lambda x, p: lib.rope_axes(x, None, p, (4, 4))
+        attn = lambda q, k, v: lib.cross_attn(q, k, v, key_mask=keep)
+    B, N, D = t["x"].shape
+    _, h = lib.norm_gate_residual(t["x"], t["u"], pre="layer", pre_weight=t["w1"], pre_bias=t["b1"])
+    q = rope(h.unflatten(-1, (4, 16)), pos_q)
+    k = rope(t["k"], pos_k)
+    o = attn(q, k, t["v"]).reshape(B, N, D)
+    return lib.norm_gate_residual(cast(t["x"]), o, gate=t["gate"], post="rms", post_weight=t["w2"], pre="layer", pre_weight=t["w1"],
+                                  pre_bias=t["b1"])
+
+
+def block_inputs(dtype):
+    g = gen(77)
+    r = lambda *s, dt=F: torch.randn(*s, generator=g).to(dt)
+    t = dict(x=r(2, 37, 64, dt=dtype), u=r(2, 37, 64, dt=dtype), k=r(2, 50, 2, 16, dt=dtype), v=r(2, 50, 2, 16, dt=dtype),
+             w1=r(64), b1=r(64), w2=r(64), gate=r(64))
+    keep = torch.rand(2, 50, generator=g) < 0.7
+    return t, keep, torch.randint(0, 12, (37, 2), generator=g), torch.randint(0, 12, (50, 2), generator=g)
+
+
+@pytest.mark.parametrize("dtype,bar", [(F, 1e-4), (H, 2e-2)], ids=["f32", "bf16"])
+def test_decoder_block_together(dtype, bar):
+    """The operators in a row as a decoder block uses them, against the same row of definitions in 64 bits, at the
+    repository's bars for whole paths (largest deviation over the tensor's largest value): here bf16 intermediates are
+    rounded between the operators."""
+    t, keep, pq, pk = block_inputs(dtype)
+    ref = {n: v.double().requires_grad_() for n, v in t.items()}
+    dev = {n: v.to(DEV).requires_grad_() for n, v in t.items()}
+    ry, rh = decoder_block(orc, ref, keep, pq, pk, lambda x: x)
+    y, h = decoder_block(ops(), dev, keep.to(DEV), pq.to(DEV), pk.to(DEV), lambda x: x)
+    rg = torch.autograd.grad(ry.sum() + (rh * rh).sum(), list(ref.values()))
+    gg = torch.autograd.grad(y.float().sum() + (h.float() * h.float()).sum(), list(dev.values()))
+    for n, a, b in [("y", y, ry), ("h", h, rh)] + list(zip(t, gg, rg)):
+        err = (a.double().cpu() - b).abs().max() / b.abs().max()
+        assert err < bar, (n, err.item())
+
+
+def test_decoder_block_in_a_graph_and_on_another_stream():
+    """Forward and backward captured once and replayed with new inputs, eager work between the replays."""
+    t, keep, pq, pk = block_inputs(H)
+    keep, pq, pk = keep.to(DEV), pq.to(DEV), pk.to(DEV)
+    dev = {n: v.to(DEV).requires_grad_() for n, v in t.items()}
+
+    def step():
+        y, h = decoder_block(ops(), dev, keep, pq, pk, lambda x: x)
+        return (y.detach(), h.detach()) + torch.autograd.grad((y, h), list(dev.values()), (torch.ones_like(y), torch.ones_like(h)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = [v.clone() for v in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(first, step()):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        with torch.no_grad():
+            for n in ("x", "u", "k", "v"):
+                dev[n].copy_(torch.randn(dev[n].shape, generator=gen(100 + i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, step()):
+            assert torch.equal(a, b), i
+
+
+def test_two_graphs_and_streams_at_once_do_not_share_scratch():
+    """Split launches with workspaces of their own: two captured calls replayed side by side on two streams."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    sets = [[torch.randn(1, n, 2, 64, generator=g, device=DEV).to(H) for n in (2, 5000, 5000)] for _ in range(2)]
+    want = [ops().cross_attn(*s) for s in sets]
+    graphs, outs = [], []
+    for s in sets:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(ops().cross_attn(*s))
+        graphs.append(gr)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_per_sample_passes():
+    """Under per_sample_norms the operators without parameters pass gradients on as usual, the one with parameters
+    refuses; a clipped replay forms no input gradients."""
+    from visiontransformer_amd.ops import clipped_replay, per_sample_norms
+    x = torch.randn(2, 5, 2, 16, device=DEV).requires_grad_()
+    pos = torch.arange(5, device=DEV)[:, None]
+    y = ops().cross_attn(ops().rope_axes(x, None, pos, (8,)), x, x)
+    want, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    with per_sample_norms(2, DEV):
+        got, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    assert torch.equal(got, want)
+    with clipped_replay(torch.ones(2, device=DEV)):
+        got, = torch.autograd.grad(y.sum(), x)
+    assert got.shape == x.shape and not got.any()
+    w = torch.ones(16, device=DEV).requires_grad_()
+    u = torch.randn(2, 5, 16, device=DEV).requires_grad_()
+    z, _ = ops().norm_gate_residual(u, u, gate=w)
+    with per_sample_norms(2, DEV):
+        with pytest.raises(NotImplementedError, match="norm_gate_residual"):
+            torch.autograd.grad(z.sum(), w)

@@ -128,6 +128,14 @@ SIGNATURES = {
     "vitmi_ff_block_bwd_sums_strips": (I, [I, I, I, I]),
     "vitmi_attn_block_bwd_sums_offset": (L, [I, I, I, I, I, I]),
     "vitmi_attn_block_bwd_sums_strips": (I, [I, I, I, I, I, I]),
+    "vitmi_rope_axes": (I, [P, P]),
+    "vitmi_cross_attn_fwd_workspace_bytes": (L, [I, I, I, I, I, I, I]),
+    "vitmi_cross_attn_fwd": (I, [P, P, P]),
+    "vitmi_cross_attn_bwd_workspace_bytes": (L, [I, I, I, I, I, I, I]),
+    "vitmi_cross_attn_bwd": (I, [P, P, P]),
+    "vitmi_norm_gate_residual_fwd": (I, [P, P]),
+    "vitmi_norm_gate_residual_bwd_workspace_bytes": (L, [I, I, I, I]),
+    "vitmi_norm_gate_residual_bwd": (I, [P, P, P]),
 }
 
 

@@ -20,7 +20,8 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libvitmi_hip.so")
 ARCH = "gfx950"
-SOURCES = ["runtime.hip", "elementwise.hip", "gemm.hip", "gemm_fast.hip", "attention.hip", "rollout.hip", "blocks.hip", "persample.hip", "small.hip"]
+SOURCES = ["runtime.hip", "elementwise.hip", "gemm.hip", "gemm_fast.hip", "attention.hip", "rollout.hip", "blocks.hip", "persample.hip", "small.hip",
+           "rope.hip", "cross_attn.hip", "norm_gate.hip"]
 HEADERS = [os.path.join(CSRC, "common.h"), os.path.join(HERE, "..", "include", "vitmi.h")]
 # packed fp32 instructions stay off: some forms that the compiler picks for ordinary float code return wrong results now
 # and then on this target (the host pass does not know the feature and says so: harmless)

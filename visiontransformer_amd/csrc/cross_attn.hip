@@ -1,0 +1,975 @@
+// Attention of query rows over the states of another sequence, q [B, Nq, Hq, D] over k, v [B, Nk, Hk, D]: lengths of
+// their own, query heads that share a key head (group G = Hq / Hk), a key length per sample or a key mask.
+//     s = scale q.k over the allowed keys,  p = softmax(s),  o = p v;   a sample without an allowed key gives o = 0
+//     delta = sum_d dO o,  dp = dO.v,  ds = scale p (dp - delta),  dq = ds k,  dk = ds^T q,  dv = p^T dO (summed over the group)
+// One (sample, key head) is one problem of R = G * Nq query rows (row r: head r / Nq of the group, position r % Nq) and Nk
+// keys, so the heads of a group share the staged keys.
+//
+// All kernels work on 32 x 32 tiles of the matrix instructions with the index that a softmax or a sum runs along in a
+// lane's REGISTERS and the other on the lane: S^T = K Q^T holds one query per lane, so that the row statistics are
+// register work with a rare exchange between the two half waves, and the registers of P are the B operand of the next
+// product as they are.  For bf16 the key rows of the first product are fed in a permuted order (key_of) so that these
+// registers hold eight consecutive keys; the other operand (V^T, K^T, Q^T, dO^T) comes out of a row-major LDS image by
+// transposing reads.  The fp32 form runs the same code over the fp32 matrix instruction.
+//   forward      four waves of 32 rows share double-buffered key tiles; the running maximum is moved only when a row
+//                outgrows it by 2^8, so the rescale of the accumulators almost never runs.
+//   few rows     (up to 64 a problem: generation, pooling) the four waves share 32 rows and walk key tiles of their own
+//                without a barrier, bound by the bytes of K and V; their results are joined in LDS.
+//   dq           four waves of 32 rows over all key tiles (S, dP, dq);  dk / dv: four waves of 32 keys over all row tiles
+//                of all heads of the group (S, dP, dv, dk).  Seven products where five would do, and no atomics: every
+//                sum runs in a fixed order, results are bitwise reproducible.
+// Where the tiles of a launch leave compute units idle, the inner loop is split over workgroups that leave fp32 partial
+// results in the workspace, joined by a second launch.
+// Masked keys: their K and V rows are staged as zeros whatever they hold, their scores are -inf.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+constexpr float XA_LOG2E = 1.4426950408889634f;
+constexpr int XA_THREADS = 256;
+constexpr float XA_SLACK = 8.f;     // log2 of how far a row may outgrow its running maximum before it is moved
+
+struct XaArgs {
+    const void *q, *k, *v;
+    void* o;                              // dense [B, Nq, Hq, D]
+    long long qs[3], ks[3], vs[3];        // batch, row, head strides
+    const void* kv_len;                   // [B] int32 / int64 or NULL
+    const unsigned char* key_mask;        // [B, Nk] or NULL
+    long long mask_stride;
+    int len64;
+    float* lse;                           // [B, Hk, R], log2 domain; +inf: nothing to attend to
+    float *part_o, *part_ml;              // [splits][B, Nq, Hq, D], [splits][B, Hk, R][2]
+    int Nq, Nk, Hq, Hk, G, R, D, splits, tiles;
+    float c;                              // scale * log2(e)
+    float scale;
+    // backward
+    const void* dout;
+    long long dos[3];
+    float* delta;                         // [B, Hk, R]
+    void *dq, *dk, *dv;                   // dense, or NULL
+    float *part_dq, *part_dk, *part_dv;
+    long long n_q, n_k;                   // elements of q and of k
+};
+
+typedef float xf32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Mx;
+template <> struct Mx<bf16_t> {
+    typedef bf16x8 frag;
+    static constexpr int FE = 8, KD = 16;   // elements of a fragment per lane, contraction depth of a fragment
+    static constexpr int KT = 64;           // sequence rows of a staged tile
+};
+template <> struct Mx<float> {
+    typedef f32x4 frag;
+    static constexpr int FE = 4, KD = 8;
+    static constexpr int KT = 32;
+};
+
+__device__ __forceinline__ void mma(f32x16& acc, const bf16x8& a, const bf16x8& b) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& acc, const f32x4& a, const f32x4& b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
+}
+
+// sequence index (0..31) fed as row m of a 32-row A operand, and the index that accumulator register e of half wave h
+// then holds (the hardware's row of that register is 8 (e / 4) + 4 h + e % 4)
+template <typename T> __device__ __forceinline__ int key_of_row(int m);
+template <> __device__ __forceinline__ int key_of_row<bf16_t>(int m) {
+    const int g = m >> 3;
+    return 16 * (g >> 1) + 8 * ((m >> 2) & 1) + 4 * (g & 1) + (m & 3);
+}
+template <> __device__ __forceinline__ int key_of_row<float>(int m) { return m; }
+template <typename T> __device__ __forceinline__ int key_of(int e, int h);
+template <> __device__ __forceinline__ int key_of<bf16_t>(int e, int h) {
+    const int g = e >> 2;
+    return 16 * (g >> 1) + 8 * h + 4 * (g & 1) + (e & 3);
+}
+template <> __device__ __forceinline__ int key_of<float>(int e, int h) { return 8 * (e >> 2) + 4 * h + (e & 3); }
+
+// registers of a 32 x 32 accumulator as B operand: group n of KD consecutive sequence indices
+__device__ __forceinline__ bf16x8 acc_frag(const f32x16& p, int n, bf16_t) {
+    union {
+        bf16x2 h[4];
+        bf16x8 v;
+    } u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u.h[i] = __builtin_convertvector(f32x2{p[8 * n + 2 * i], p[8 * n + 2 * i + 1]}, bf16x2);
+    return u.v;
+}
+__device__ __forceinline__ f32x4 acc_frag(const f32x16& p, int n, float) {
+    return f32x4{p[4 * n], p[4 * n + 1], p[4 * n + 2], p[4 * n + 3]};
+}
+
+template <typename T> __device__ __forceinline__ typename Mx<T>::frag zero_frag() {
+    typename Mx<T>::frag z;
+#pragma unroll
+    for (int j = 0; j < Mx<T>::FE; ++j) z[j] = (T)0.f;
+    return z;
+}
+
+// row of an LDS image in elements: DP plus 16 bytes, which spreads both kinds of read over the banks
+template <typename T, int DP> constexpr int ld_of() { return DP + 16 / (int)sizeof(T); }
+
+template <typename T, int DP>
+__device__ __forceinline__ typename Mx<T>::frag row_frag(const T* img, int row, int c, int h) {
+    return *reinterpret_cast<const typename Mx<T>::frag*>(img + row * ld_of<T, DP>() + c * Mx<T>::KD + h * Mx<T>::FE);
+}
+// A operand [32 columns col0.. as rows][KD sequence rows seq0..]: lane l holds column col0 + l % 32 of sequence rows
+// seq0 + FE (l / 32) + 0..FE-1
+template <int DP>
+__device__ __forceinline__ bf16x8 col_frag(const bf16_t* img, int seq0, int col0, int lane) {
+    const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+    const bf16_t* a = img + (seq0 + 8 * (g >> 1) + q) * ld_of<bf16_t, DP>() + col0 + 16 * (g & 1) + 4 * p;
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    union {
+        s16x4 h[2];
+        bf16x8 v;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)a);
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a + 4 * ld_of<bf16_t, DP>()));
+    return u.v;
+}
+template <int DP>
+__device__ __forceinline__ f32x4 col_frag(const float* img, int seq0, int col0, int lane) {
+    const float* a = img + (seq0 + 4 * (lane >> 5)) * ld_of<float, DP>() + col0 + (lane & 31);
+    f32x4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = a[j * ld_of<float, DP>()];
+    return r;
+}
+
+// FE elements of a row in global memory from dim d on; dims beyond D read as zero
+template <typename T, bool VEC>
+__device__ __forceinline__ typename Mx<T>::frag global_piece(const T* row, int d, int D) {
+    typename Mx<T>::frag f = zero_frag<T>();
+    if (VEC) {
+        if (d < D) f = *reinterpret_cast<const typename Mx<T>::frag*>(row + d);
+    } else {
+#pragma unroll
+        for (int j = 0; j < Mx<T>::FE; ++j)
+            if (d + j < D) f[j] = row[d + j];
+    }
+    return f;
+}
+
+__device__ __forceinline__ int keys_of(const XaArgs& a, int b) {
+    if (!a.kv_len) return a.Nk;
+    const long long n = a.len64 ? ((const long long*)a.kv_len)[b] : (long long)((const int*)a.kv_len)[b];
+    return (int)(n < 0 ? 0 : (n > a.Nk ? a.Nk : n));
+}
+// one bit per key of [key0, key0 + KT): allowed
+template <int KT>
+__device__ __forceinline__ unsigned long long tile_mask(const XaArgs& a, int b, int key0, int n, int lane) {
+    if (key0 >= n) return 0;
+    const int left = n - key0 < KT ? n - key0 : KT;
+    unsigned long long m = left >= 64 ? ~0ull : (1ull << left) - 1;
+    if (a.key_mask) {
+        const bool on = lane < left && a.key_mask[b * a.mask_stride + key0 + lane] != 0;
+        m &= __ballot(on);
+    }
+    return m;
+}
+template <int KT> constexpr unsigned long long full_mask() { return KT >= 64 ? ~0ull : (1ull << KT) - 1; }
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// a tile of KT rows of two matrices on its way from global memory to LDS through registers, by TH threads
+template <typename T, int DP, bool VEC, int KT, int TH>
+struct Stage {
+    static constexpr int CPR = DP / Mx<T>::FE, IT = KT * CPR / TH;
+    static_assert(KT * CPR % TH == 0, "a tile is a whole number of pieces per thread");
+    typename Mx<T>::frag x[IT], y[IT];
+    // rows row0 + r of two matrices with row strides lx, ly; rows from n on are not read
+    __device__ __forceinline__ void fetch(const T* px, long long lx, const T* py, long long ly, int row0, int n, int D, int t) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = t + i * TH, r = row0 + c / CPR, d = (c % CPR) * Mx<T>::FE;
+            x[i] = y[i] = zero_frag<T>();
+            if (r < n) {
+                x[i] = global_piece<T, VEC>(px + r * lx, d, D);
+                y[i] = global_piece<T, VEC>(py + r * ly, d, D);
+            }
+        }
+    }
+    // query rows: row r of the flattened group is position r % Nq of head r / Nq
+    __device__ __forceinline__ void fetch_rows(const T* px, const long long* sx, const T* py, const long long* sy, int row0, int R, int Nq,
+                                               int D, int t) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = t + i * TH, r = row0 + c / CPR, d = (c % CPR) * Mx<T>::FE;
+            x[i] = y[i] = zero_frag<T>();
+            if (r < R) {
+                const int g = r / Nq, n = r - g * Nq;
+                x[i] = global_piece<T, VEC>(px + n * sx[1] + g * sx[2], d, D);
+                y[i] = global_piece<T, VEC>(py + n * sy[1] + g * sy[2], d, D);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* ix, T* iy, unsigned long long mask, int t) {
+        if (mask != full_mask<KT>()) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+                if (!((mask >> ((t + i * TH) / CPR)) & 1)) x[i] = y[i] = zero_frag<T>();
+        }
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int c = t + i * TH, o = (c / CPR) * ld_of<T, DP>() + (c % CPR) * Mx<T>::FE;
+            *reinterpret_cast<typename Mx<T>::frag*>(ix + o) = x[i];
+            *reinterpret_cast<typename Mx<T>::frag*>(iy + o) = y[i];
+        }
+    }
+};
+
+// Workgroups are dealt to the 8 XCDs round-robin: this gives each XCD a contiguous range of tiles, whose keys it then
+// fetches into its own L2 once
+__device__ __forceinline__ int xa_block() {
+    const int n = gridDim.x, x = blockIdx.x & 7, slot = blockIdx.x >> 3, q = n >> 3, rem = n & 7;
+    return x * q + (x < rem ? x : rem) + slot;
+}
+
+// scores of one 32-key block against the lane's query
+template <typename T, int DP>
+__device__ __forceinline__ void scores(f32x16& s, const T* img, int key0, const typename Mx<T>::frag (&f)[DP / Mx<T>::KD], int lane) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+    const int row = key0 + key_of_row<T>(lane & 31);
+#pragma unroll
+    for (int c = 0; c < DP / Mx<T>::KD; ++c) mma(s, row_frag<T, DP>(img, row, c, lane >> 5), f[c]);
+}
+
+template <typename T>
+__device__ __forceinline__ void mask_scores(f32x16& s, unsigned m, int h) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if (!((m >> key_of<T>(e, h)) & 1)) s[e] = -INFINITY;
+}
+
+// one staged tile against the lane's query: running softmax and o^T += V^T P^T
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typename Mx<T>::frag (&qf)[DP / Mx<T>::KD],
+                                       unsigned long long mask, float c, f32x16 (&o)[DP / 32], float& m, float& l, int lane) {
+    constexpr int KB = KT / 32;
+    f32x16 s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) scores<T, DP>(s[kb], kimg, 32 * kb, qf, lane);
+    if (mask != full_mask<KT>()) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) mask_scores<T>(s[kb], (unsigned)(mask >> (32 * kb)), lane >> 5);
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+    mx *= c;
+    if (__any(mx > m + XA_SLACK)) {
+        const float mn = fmaxf(m, fmaxf(mx, other_half(mx)));
+        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= f;
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], c, -m));
+            l += s[kb][e];
+        }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int n = 0; n < 32 / Mx<T>::KD; ++n) {
+            const typename Mx<T>::frag pf = acc_frag(s[kb], n, T());
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<DP>(vimg, 32 * kb + n * Mx<T>::KD, 32 * d, lane), pf);
+        }
+}
+
+// four consecutive dims (8 g + 4 h ..) of an accumulator block to a dense row
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* row, int d, int D, float v0, float v1, float v2, float v3) {
+    if (VEC) {
+        if (d < D) {
+            T p[4] = {from_f32<T>(v0), from_f32<T>(v1), from_f32<T>(v2), from_f32<T>(v3)};
+            struct alignas(4 * sizeof(T)) Q {
+                T v[4];
+            };
+            *reinterpret_cast<Q*>(row + d) = *reinterpret_cast<Q*>(p);
+        }
+    } else {
+        const float v[4] = {v0, v1, v2, v3};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (d + j < D) row[d + j] = from_f32<T>(v[j]);
+    }
+}
+template <typename T, bool VEC, int DP>
+__device__ __forceinline__ void store_acc(T* row, const f32x16 (&o)[DP / 32], float f, int h, int D) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            store4<T, VEC>(row, 32 * db + 8 * g + 4 * h, D, o[db][4 * g] * f, o[db][4 * g + 1] * f, o[db][4 * g + 2] * f,
+                           o[db][4 * g + 3] * f);
+}
+
+// element offset of query row r of problem (b, hk) in a dense [B, Nq, Hq, D]
+__device__ __forceinline__ long long dense_row(const XaArgs& a, int b, int hk, int r) {
+    const int g = r / a.Nq, n = r - g * a.Nq;
+    return (((long long)b * a.Nq + n) * a.Hq + hk * a.G + g) * a.D;
+}
+
+// result rows of a forward kernel: normalised output and lse, or (splits) unnormalised partials
+template <typename T, int DP, bool VEC>
+__device__ __forceinline__ void finish_rows(const XaArgs& a, int b, int hk, int r, int split, const f32x16 (&o)[DP / 32], float m, float l,
+                                            int h) {
+    if (r >= a.R) return;
+    const long long row = dense_row(a, b, hk, r), st = ((long long)b * a.Hk + hk) * a.R + r;
+    if (a.splits == 1) {
+        store_acc<T, VEC, DP>((T*)a.o + row, o, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), h, a.D);
+        if (a.lse && h == 0) a.lse[st] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    } else {
+        store_acc<float, VEC, DP>(a.part_o + split * a.n_q + row, o, 1.f, h, a.D);
+        if (h == 0) {
+            float2* ml = reinterpret_cast<float2*>(a.part_ml) + (long long)split * (a.n_q / a.D) + st;
+            *ml = make_float2(m, l);
+        }
+    }
+}
+
+// this workgroup's share [t0, t1) of `tiles` tiles
+__device__ __forceinline__ void split_range(int tiles, int splits, int split, int& t0, int& t1) {
+    t0 = (int)((long long)tiles * split / splits);
+    t1 = (int)((long long)tiles * (split + 1) / splits);
+}
+
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(XA_THREADS) void xattn_fwd_kernel(XaArgs a) {
+    constexpr int KT = Mx<T>::KT, IMG = KT * ld_of<T, DP>();
+    extern __shared__ __align__(16) char xa_lds[];
+    T* const lds = reinterpret_cast<T*>(xa_lds);        // K, V, K, V
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    int idx = xa_block();
+    const int rt = idx % a.tiles;
+    idx /= a.tiles;
+    const int split = idx % a.splits;
+    idx /= a.splits;
+    const int hk = idx % a.Hk, b = idx / a.Hk;
+    const int r = rt * 128 + wave * 32 + (lane & 31);
+    typename Mx<T>::frag qf[DP / Mx<T>::KD];
+    {
+        const int g = r / a.Nq, n = r - g * a.Nq;
+        const T* qp = (const T*)a.q + b * a.qs[0] + n * a.qs[1] + (hk * a.G + g) * a.qs[2];
+#pragma unroll
+        for (int c = 0; c < DP / Mx<T>::KD; ++c)
+            qf[c] = r < a.R ? global_piece<T, VEC>(qp, c * Mx<T>::KD + h * Mx<T>::FE, a.D) : zero_frag<T>();
+    }
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const int n = keys_of(a, b);
+    const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    int t0, t1;
+    split_range((n + KT - 1) / KT, a.splits, split, t0, t1);
+    Stage<T, DP, VEC, KT, XA_THREADS> st;
+    unsigned long long mask = 0;
+    if (t0 < t1) {
+        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, n, a.D, t);
+        mask = tile_mask<KT>(a, b, t0 * KT, n, lane);
+    }
+    for (int kt = t0; kt < t1; ++kt) {
+        T* img = lds + (kt & 1) * 2 * IMG;
+        const unsigned long long mk = mask;
+        st.store(img, img + IMG, mk, t);
+        __syncthreads();
+        if (kt + 1 < t1) {
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, n, a.D, t);
+            mask = tile_mask<KT>(a, b, (kt + 1) * KT, n, lane);
+        }
+        if (mk) attend<T, DP, KT>(img, img + IMG, qf, mk, a.c, o, m, l, lane);
+    }
+    l += other_half(l);
+    finish_rows<T, DP, VEC>(a, b, hk, r, split, o, m, l, h);
+}
+
+// one wave's LDS image is written and read by that wave alone: its LDS operations run in order, only the compiler is held
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// up to 64 rows a problem: every wave walks 32-key tiles of its own for the same 32 rows
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
+    constexpr int KT = 32, IMG = KT * ld_of<T, DP>();
+    extern __shared__ __align__(16) char xa_lds[];
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    T* const img = reinterpret_cast<T*>(xa_lds) + wave * 2 * IMG;
+    int idx = xa_block();
+    const int rt = idx % a.tiles;
+    idx /= a.tiles;
+    const int split = idx % a.splits;
+    idx /= a.splits;
+    const int hk = idx % a.Hk, b = idx / a.Hk;
+    const int r = rt * 32 + (lane & 31);
+    const int n = keys_of(a, b);
+    const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    int t0, t1;
+    split_range((n + KT - 1) / KT, a.splits, split, t0, t1);
+    Stage<T, DP, VEC, KT, 64> st;
+    unsigned long long mask = 0;
+    if (t0 + wave < t1) {
+        st.fetch(kp, a.ks[1], vp, a.vs[1], (t0 + wave) * KT, n, a.D, lane);
+        mask = tile_mask<KT>(a, b, (t0 + wave) * KT, n, lane);
+    }
+    typename Mx<T>::frag qf[DP / Mx<T>::KD];
+    {
+        const int g = r / a.Nq, nn = r - g * a.Nq;
+        const T* qp = (const T*)a.q + b * a.qs[0] + nn * a.qs[1] + (hk * a.G + g) * a.qs[2];
+#pragma unroll
+        for (int c = 0; c < DP / Mx<T>::KD; ++c)
+            qf[c] = r < a.R ? global_piece<T, VEC>(qp, c * Mx<T>::KD + h * Mx<T>::FE, a.D) : zero_frag<T>();
+    }
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (int kt = t0 + wave; kt < t1; kt += 4) {
+        const unsigned long long mk = mask;
+        st.store(img, img + IMG, mk, lane);
+        wave_fence();
+        if (kt + 4 < t1) {
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, n, a.D, lane);
+            mask = tile_mask<KT>(a, b, (kt + 4) * KT, n, lane);
+        }
+        if (mk) attend<T, DP, KT>(img, img + IMG, qf, mk, a.c, o, m, l, lane);
+        wave_fence();
+    }
+    l += other_half(l);
+    // join the four waves in wave order: running maxima first, then the rescaled sums and outputs
+    float* const xo = reinterpret_cast<float*>(xa_lds);                    // [4][DP][32] after the barrier
+    float* const xm = xo + 4 * DP * 32;                                   // [4][32][2]
+    __syncthreads();
+    if (h == 0) {
+        xm[(wave * 32 + (lane & 31)) * 2] = m;
+        xm[(wave * 32 + (lane & 31)) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) xo[(wave * DP + 32 * d + 8 * (e >> 2) + 4 * h + (e & 3)) * 32 + (lane & 31)] = o[d][e];
+    __syncthreads();
+    float mm = -INFINITY, w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mm = fmaxf(mm, xm[(i * 32 + (lane & 31)) * 2]);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float mi = xm[(i * 32 + (lane & 31)) * 2], li = xm[(i * 32 + (lane & 31)) * 2 + 1];
+        w[i] = mi == -INFINITY ? (li == 0.f ? 0.f : li) : __builtin_amdgcn_exp2f(mi - mm);
+        l += mi == -INFINITY ? li : li * w[i];
+    }
+    m = mm;
+    if (r >= a.R) return;
+    const float f = a.splits == 1 ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+    const long long row = dense_row(a, b, hk, r), sti = ((long long)b * a.Hk + hk) * a.R + r;
+    // the waves share the dims of the output: 8 consecutive ones a thread and step
+    for (int d = 8 * (2 * wave + h); d < DP; d += 64) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float oi = xo[(i * DP + d + j) * 32 + (lane & 31)];
+                v[j] = w[i] == 0.f ? v[j] : fmaf(oi, w[i], v[j]);
+            }
+            v[j] *= f;
+        }
+        if (a.splits == 1) {
+            store4<T, VEC>((T*)a.o + row, d, a.D, v[0], v[1], v[2], v[3]);
+            store4<T, VEC>((T*)a.o + row, d + 4, a.D, v[4], v[5], v[6], v[7]);
+        } else {
+            store4<float, VEC>(a.part_o + split * a.n_q + row, d, a.D, v[0], v[1], v[2], v[3]);
+            store4<float, VEC>(a.part_o + split * a.n_q + row, d + 4, a.D, v[4], v[5], v[6], v[7]);
+        }
+    }
+    if (wave == 0 && h == 0) {
+        if (a.splits == 1) {
+            if (a.lse) a.lse[sti] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+        } else {
+            reinterpret_cast<float2*>(a.part_ml)[(long long)split * (a.n_q / a.D) + sti] = make_float2(m, l);
+        }
+    }
+}
+
+// joins the key splits of a forward launch, one wave a row
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long rows) {
+    const int lane = threadIdx.x & 63;
+    const long long st = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (st >= rows) return;
+    const int r = (int)(st % a.R);
+    const long long bh = st / a.R;
+    const int hk = (int)(bh % a.Hk), b = (int)(bh / a.Hk);
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + st;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * rows].x);
+    const long long row = dense_row(a, b, hk, r);
+    float o0 = 0.f, o1 = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 p = ml[s * rows];
+        if (p.y == 0.f) continue;                    // a share without an allowed key
+        const float w = p.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p.x - m);
+        l = fmaf(p.y, w, l);
+        const float* po = a.part_o + s * a.n_q + row;
+        if (lane < a.D) o0 = fmaf(po[lane], w, o0);
+        if (lane + 64 < a.D) o1 = fmaf(po[lane + 64], w, o1);
+    }
+    const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* op = (T*)a.o + row;
+    if (lane < a.D) op[lane] = from_f32<T>(o0 * f);
+    if (lane + 64 < a.D) op[lane + 64] = from_f32<T>(o1 * f);
+    if (a.lse && lane == 0) a.lse[st] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(XA_THREADS) void xattn_dq_kernel(XaArgs a) {
+    constexpr int KT = Mx<T>::KT, IMG = KT * ld_of<T, DP>(), NF = DP / Mx<T>::KD;
+    extern __shared__ __align__(16) char xa_lds[];
+    T* const lds = reinterpret_cast<T*>(xa_lds);
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    int idx = xa_block();
+    const int rt = idx % a.tiles;
+    idx /= a.tiles;
+    const int split = idx % a.splits;
+    idx /= a.splits;
+    const int hk = idx % a.Hk, b = idx / a.Hk;
+    const int r = rt * 128 + wave * 32 + (lane & 31);
+    const bool in = r < a.R;
+    const long long row = in ? dense_row(a, b, hk, r) : 0, sti = ((long long)b * a.Hk + hk) * a.R + r;
+    typename Mx<T>::frag qf[NF], gf[NF];
+    float lse = INFINITY, delta = 0.f;
+    {
+        const int g = r / a.Nq, n = r - g * a.Nq;
+        const T* qp = (const T*)a.q + b * a.qs[0] + n * a.qs[1] + (hk * a.G + g) * a.qs[2];
+        const T* gp = (const T*)a.dout + b * a.dos[0] + n * a.dos[1] + (hk * a.G + g) * a.dos[2];
+        const T* op = (const T*)a.o + row;
+#pragma unroll
+        for (int c = 0; c < NF; ++c) {
+            const int d = c * Mx<T>::KD + h * Mx<T>::FE;
+            qf[c] = in ? global_piece<T, VEC>(qp, d, a.D) : zero_frag<T>();
+            gf[c] = in ? global_piece<T, VEC>(gp, d, a.D) : zero_frag<T>();
+            const typename Mx<T>::frag of = in ? global_piece<T, VEC>(op, d, a.D) : zero_frag<T>();
+#pragma unroll
+            for (int j = 0; j < Mx<T>::FE; ++j) delta = fmaf(to_f32(gf[c][j]), to_f32(of[j]), delta);
+        }
+        if (in) lse = a.lse[sti];
+    }
+    delta += other_half(delta);
+    if (in && h == 0 && split == 0) a.delta[sti] = delta;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    const int n = keys_of(a, b);
+    const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    int t0, t1;
+    split_range(a.dq ? (n + KT - 1) / KT : 0, a.splits, split, t0, t1);      // without dq only delta is wanted
+    Stage<T, DP, VEC, KT, XA_THREADS> st;
+    unsigned long long mask = 0;
+    if (t0 < t1) {
+        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, n, a.D, t);
+        mask = tile_mask<KT>(a, b, t0 * KT, n, lane);
+    }
+    for (int kt = t0; kt < t1; ++kt) {
+        T* img = lds + (kt & 1) * 2 * IMG;
+        const unsigned long long mk = mask;
+        st.store(img, img + IMG, mk, t);
+        __syncthreads();
+        if (kt + 1 < t1) {
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, n, a.D, t);
+            mask = tile_mask<KT>(a, b, (kt + 1) * KT, n, lane);
+        }
+        if (mk) {
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb) {
+                f32x16 s, dp;
+                scores<T, DP>(s, img, 32 * kb, qf, lane);
+                scores<T, DP>(dp, img + IMG, 32 * kb, gf, lane);
+                if (mk != full_mask<KT>()) mask_scores<T>(s, (unsigned)(mk >> (32 * kb)), h);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse)) * (dp[e] - delta);
+#pragma unroll
+                for (int g = 0; g < 32 / Mx<T>::KD; ++g) {
+                    const typename Mx<T>::frag f = acc_frag(s, g, T());
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) mma(acc[d], col_frag<DP>(img, 32 * kb + g * Mx<T>::KD, 32 * d, lane), f);
+                }
+            }
+        }
+    }
+    if (!in || !a.dq) return;
+    if (a.splits == 1)
+        store_acc<T, VEC, DP>((T*)a.dq + row, acc, a.scale, h, a.D);
+    else
+        store_acc<float, VEC, DP>(a.part_dq + split * a.n_q + row, acc, 1.f, h, a.D);
+}
+
+// dk and dv: four waves of 32 keys over the row tiles of the whole group
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(XA_THREADS) void xattn_dkv_kernel(XaArgs a) {
+    constexpr int QT = Mx<T>::KT, IMG = QT * ld_of<T, DP>(), NF = DP / Mx<T>::KD;
+    extern __shared__ __align__(16) char xa_lds[];
+    T* const lds = reinterpret_cast<T*>(xa_lds);                           // Q, dO, Q, dO
+    float* const rows = reinterpret_cast<float*>(xa_lds + 4 * IMG * sizeof(T));   // [2][lse, delta][QT]
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    int idx = xa_block();
+    const int kt = idx % a.tiles;
+    idx /= a.tiles;
+    const int split = idx % a.splits;
+    idx /= a.splits;
+    const int hk = idx % a.Hk, b = idx / a.Hk;
+    const int key = kt * 128 + wave * 32 + (lane & 31);
+    const int n = keys_of(a, b);
+    const bool on = key < n && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0);
+    typename Mx<T>::frag kf[NF], vf[NF];
+    {
+        const T* kp = (const T*)a.k + b * a.ks[0] + key * a.ks[1] + hk * a.ks[2];
+        const T* vp = (const T*)a.v + b * a.vs[0] + key * a.vs[1] + hk * a.vs[2];
+#pragma unroll
+        for (int c = 0; c < NF; ++c) {
+            const int d = c * Mx<T>::KD + h * Mx<T>::FE;
+            kf[c] = on ? global_piece<T, VEC>(kp, d, a.D) : zero_frag<T>();
+            vf[c] = on ? global_piece<T, VEC>(vp, d, a.D) : zero_frag<T>();
+        }
+    }
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+    int t0 = 0, t1 = 0;
+    if (__syncthreads_or(on)) split_range((a.R + QT - 1) / QT, a.splits, split, t0, t1);
+    const T* qp = (const T*)a.q + b * a.qs[0] + (long long)hk * a.G * a.qs[2];
+    const T* gp = (const T*)a.dout + b * a.dos[0] + (long long)hk * a.G * a.dos[2];
+    const long long sti = ((long long)b * a.Hk + hk) * a.R;
+    Stage<T, DP, VEC, QT, XA_THREADS> st;
+    float stat = 0.f;                                     // threads 0..QT-1: lse, QT..2QT-1: delta
+    auto fetch = [&](int tile) {
+        st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, a.D, t);
+        if (t < 2 * QT) {
+            const int r = tile * QT + (t < QT ? t : t - QT);
+            stat = t < QT ? INFINITY : 0.f;
+            if (r < a.R) stat = t < QT ? a.lse[sti + r] : a.delta[sti + r];
+        }
+    };
+    if (t0 < t1) fetch(t0);
+    for (int qt = t0; qt < t1; ++qt) {
+        T* img = lds + (qt & 1) * 2 * IMG;
+        float* rs = rows + (qt & 1) * 2 * QT;
+        st.store(img, img + IMG, full_mask<QT>(), t);
+        if (t < 2 * QT) rs[t] = stat;
+        __syncthreads();
+        if (qt + 1 < t1) fetch(qt + 1);
+#pragma unroll
+        for (int qb = 0; qb < QT / 32; ++qb) {
+            f32x16 s, dp;
+            scores<T, DP>(s, img, 32 * qb, kf, lane);
+            scores<T, DP>(dp, img + IMG, 32 * qb, vf, lane);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int q = 32 * qb + key_of<T>(e, h);
+                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -rs[q]));
+                dp[e] = s[e] * (dp[e] - rs[QT + q]);
+            }
+#pragma unroll
+            for (int g = 0; g < 32 / Mx<T>::KD; ++g) {
+                const typename Mx<T>::frag pf = acc_frag(s, g, T()), df = acc_frag(dp, g, T());
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    mma(dv[d], col_frag<DP>(img + IMG, 32 * qb + g * Mx<T>::KD, 32 * d, lane), pf);
+                    mma(dk[d], col_frag<DP>(img, 32 * qb + g * Mx<T>::KD, 32 * d, lane), df);
+                }
+            }
+        }
+    }
+    if (key >= a.Nk) return;
+    if (!on) {                                            // a masked key's lane worked on zeros: its gradients are zero
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+    }
+    const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
+    if (a.splits == 1) {
+        store_acc<T, VEC, DP>((T*)a.dk + row, dk, a.scale, h, a.D);
+        store_acc<T, VEC, DP>((T*)a.dv + row, dv, 1.f, h, a.D);
+    } else {
+        store_acc<float, VEC, DP>(a.part_dk + split * a.n_k + row, dk, 1.f, h, a.D);
+        store_acc<float, VEC, DP>(a.part_dv + split * a.n_k + row, dv, 1.f, h, a.D);
+    }
+}
+
+// out[i] = scale * sum over the splits, in split order; blockIdx.y picks one of two tensors of equal size
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* p0, T* o0, float f0, const float* p1, T* o1, float f1, long long n,
+                                                        int splits) {
+    const float* p = blockIdx.y ? p1 : p0;
+    T* o = blockIdx.y ? o1 : o0;
+    const float f = blockIdx.y ? f1 : f0;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += p[k * n + i];
+        o[i] = from_f32<T>(s * f);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+constexpr int XA_MAX_D = 128;
+
+int xa_check(const char* who, const vitmi_xattn_args* g) {
+    VITMI_CHECK_ARG(g, "%s: null arguments", who);
+    VITMI_CHECK_ARG(g->dt == VITMI_F32 || g->dt == VITMI_BF16, "%s: bad dtype %d", who, g->dt);
+    VITMI_CHECK_ARG(g->B >= 0 && g->Nq >= 0 && g->Nk >= 0 && g->Hq > 0 && g->Hk > 0 && g->D > 0,
+                    "%s: bad shape B=%d Nq=%d Nk=%d Hq=%d Hk=%d D=%d", who, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D);
+    VITMI_CHECK_ARG(g->Hq % g->Hk == 0, "%s: %d query heads do not share %d key heads evenly", who, g->Hq, g->Hk);
+    VITMI_CHECK_ARG(g->scale > 0.f && g->scale < INFINITY, "%s: the scale must be positive and finite", who);
+    VITMI_CHECK_ARG(!(g->kv_len && g->key_mask), "%s: key lengths and a key mask exclude each other", who);
+    if (g->D > XA_MAX_D) {
+        vitmi_set_error("%s: heads of %d exceed the supported width %d", who, g->D, XA_MAX_D);
+        return VITMI_ERR_UNSUPPORTED;
+    }
+    const long long lim = 1ll << 31;
+    VITMI_CHECK_ARG((long long)(g->Hq / g->Hk) * g->Nq < lim - 256 && (long long)g->Nk < lim - 256, "%s: lengths beyond one call", who);
+    return VITMI_OK;
+}
+
+bool xa_vec(const vitmi_xattn_args* g) {
+    const int fe = g->dt == VITMI_F32 ? 4 : 8;
+    if (g->D % fe) return false;
+    for (const void* p : {g->q, g->k, g->v, (const void*)g->o, g->dout, (const void*)g->dq, (const void*)g->dk, (const void*)g->dv})
+        if (reinterpret_cast<uintptr_t>(p) & 15) return false;
+    for (int i = 0; i < 3; ++i)
+        if (g->qs[i] % fe || g->ks[i] % fe || g->vs[i] % fe || (g->dout && g->dos[i] % fe)) return false;
+    return true;
+}
+
+int xa_width(int D, bool vec) { return !vec ? 128 : D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+struct XaPlan {
+    bool few;
+    int fwd_tiles, fwd_splits, dq_tiles, dq_splits, dkv_tiles, dkv_splits;
+};
+
+int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Splits of an inner loop of `steps` tiles over workgroups: none while the launch fills the chip twice over, else enough for
+// that, each with `least` tiles or more
+int xa_splits(long long blocks, int steps, int least) {
+    if (blocks >= 512 || steps < 2 * least) return 1;
+    const long long want = (512 + blocks - 1) / blocks;
+    return (int)std::max<long long>(1, std::min<long long>({want, steps / least, 64}));
+}
+
+XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk) {
+    XaPlan p;
+    const int R = Hq / Hk * Nq, KT = dt == VITMI_F32 ? 32 : 64;
+    const long long bh = (long long)B * Hk;
+    p.few = R <= 64;
+    p.fwd_tiles = cdiv(R, p.few ? 32 : 128);
+    p.fwd_splits = p.few ? xa_splits(bh * p.fwd_tiles, cdiv(Nk, 32), 8) : xa_splits(bh * p.fwd_tiles, cdiv(Nk, KT), 4);
+    p.dq_tiles = cdiv(R, 128);
+    p.dq_splits = xa_splits(bh * p.dq_tiles, cdiv(Nk, KT), 4);
+    p.dkv_tiles = cdiv(Nk, 128);
+    p.dkv_splits = xa_splits(bh * p.dkv_tiles, cdiv(R, KT), 4);
+    return p;
+}
+
+long long up256(long long x) { return (x + 255) & ~255ll; }
+
+void xa_fill(const vitmi_xattn_args* g, XaArgs* a) {
+    *a = XaArgs{};
+    a->q = g->q; a->k = g->k; a->v = g->v; a->o = g->o;
+    for (int i = 0; i < 3; ++i) {
+        a->qs[i] = g->qs[i];
+        a->ks[i] = g->ks[i];
+        a->vs[i] = g->vs[i];
+        a->dos[i] = g->dos[i];
+    }
+    a->kv_len = g->kv_len;
+    a->len64 = g->kv_len_i64;
+    a->key_mask = (const unsigned char*)g->key_mask;
+    a->mask_stride = g->mask_stride;
+    a->lse = g->lse;
+    a->Nq = g->Nq; a->Nk = g->Nk; a->Hq = g->Hq; a->Hk = g->Hk; a->D = g->D;
+    a->G = g->Hq / g->Hk;
+    a->R = a->G * g->Nq;
+    a->scale = g->scale;
+    a->c = g->scale * XA_LOG2E;
+    a->dout = g->dout;
+    a->dq = g->dq; a->dk = g->dk; a->dv = g->dv;
+    a->n_q = (long long)g->B * g->Nq * g->Hq * g->D;
+    a->n_k = (long long)g->B * g->Nk * g->Hk * g->D;
+}
+
+enum { XK_FWD, XK_FEW, XK_DQ, XK_DKV };
+
+template <typename T, int DP, bool VEC>
+int xa_launch(int kind, const XaArgs& a, long long blocks, hipStream_t s) {
+    constexpr size_t tile4 = 4ull * Mx<T>::KT * ld_of<T, DP>() * sizeof(T);
+    constexpr size_t few = std::max<size_t>(8ull * 32 * ld_of<T, DP>() * sizeof(T), (4ull * DP * 32 + 256) * sizeof(float));
+    constexpr size_t dkv = tile4 + 4ull * Mx<T>::KT * sizeof(float);
+    const size_t lds = kind == XK_FEW ? few : kind == XK_DKV ? dkv : tile4;
+    const void* fn = kind == XK_FWD   ? (const void*)&xattn_fwd_kernel<T, DP, VEC>
+                     : kind == XK_FEW ? (const void*)&xattn_few_kernel<T, DP, VEC>
+                     : kind == XK_DQ  ? (const void*)&xattn_dq_kernel<T, DP, VEC>
+                                      : (const void*)&xattn_dkv_kernel<T, DP, VEC>;
+    if (lds > 64 * 1024) {
+        hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return vitmi_hip_fail(e, "vitmi_cross_attn: LDS size");
+    }
+    VITMI_CHECK_ARG(blocks < (1ll << 32) / XA_THREADS, "vitmi_cross_attn: %lld tiles are beyond one launch", blocks);
+    const dim3 grid((unsigned)blocks), block(XA_THREADS);
+    if (kind == XK_FWD) hipLaunchKernelGGL((xattn_fwd_kernel<T, DP, VEC>), grid, block, lds, s, a);
+    else if (kind == XK_FEW) hipLaunchKernelGGL((xattn_few_kernel<T, DP, VEC>), grid, block, lds, s, a);
+    else if (kind == XK_DQ) hipLaunchKernelGGL((xattn_dq_kernel<T, DP, VEC>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((xattn_dkv_kernel<T, DP, VEC>), grid, block, lds, s, a);
+    VITMI_LAUNCH_CHECK("vitmi_cross_attn");
+    return VITMI_OK;
+}
+
+template <typename T>
+int xa_dispatch(int kind, const XaArgs& a, bool vec, long long blocks, hipStream_t s) {
+    if (!vec) return xa_launch<T, 128, false>(kind, a, blocks, s);
+    switch (xa_width(a.D, true)) {
+        case 32: return xa_launch<T, 32, true>(kind, a, blocks, s);
+        case 64: return xa_launch<T, 64, true>(kind, a, blocks, s);
+        case 96: return xa_launch<T, 96, true>(kind, a, blocks, s);
+        default: return xa_launch<T, 128, true>(kind, a, blocks, s);
+    }
+}
+
+int xa_run(int kind, int dt, const XaArgs& a, bool vec, long long blocks, hipStream_t s) {
+    return dt == VITMI_F32 ? xa_dispatch<float>(kind, a, vec, blocks, s) : xa_dispatch<bf16_t>(kind, a, vec, blocks, s);
+}
+
+int xa_sum(int dt, const float* p0, void* o0, float f0, const float* p1, void* o1, float f1, long long n, int splits, hipStream_t s) {
+    const dim3 grid((unsigned)std::min<long long>(4096, (n + 255) / 256), o1 ? 2 : 1);
+    if (dt == VITMI_F32)
+        hipLaunchKernelGGL((xattn_sum_kernel<float>), grid, dim3(256), 0, s, p0, (float*)o0, f0, p1, (float*)o1, f1, n, splits);
+    else
+        hipLaunchKernelGGL((xattn_sum_kernel<bf16_t>), grid, dim3(256), 0, s, p0, (bf16_t*)o0, f0, p1, (bf16_t*)o1, f1, n, splits);
+    VITMI_LAUNCH_CHECK("vitmi_cross_attn(sum)");
+    return VITMI_OK;
+}
+
+}  // namespace
+
+extern "C" long long vitmi_cross_attn_fwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
+    if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
+    if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
+    const int s = xa_plan(dt, B, Nq, Nk, Hq, Hk).fwd_splits;
+    if (s == 1) return 0;
+    const long long rows = (long long)B * Nq * Hq;
+    return up256(s * rows * D * 4) + up256(s * rows * 8);
+}
+
+extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, void* stream) {
+    const char* who = "vitmi_cross_attn_fwd";
+    if (int rc = xa_check(who, g)) return rc;
+    if (g->B == 0 || g->Nq == 0) return VITMI_OK;
+    VITMI_CHECK_ARG(g->q && g->o && (g->Nk == 0 || (g->k && g->v)), "%s: null pointer", who);
+    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk);
+    VITMI_CHECK_ARG(p.fwd_splits == 1 || workspace, "%s: this shape needs a workspace", who);
+    XaArgs a;
+    xa_fill(g, &a);
+    const long long rows = (long long)g->B * g->Nq * g->Hq;
+    a.tiles = p.fwd_tiles;
+    a.splits = p.fwd_splits;
+    a.part_o = (float*)workspace;
+    a.part_ml = (float*)((char*)workspace + up256((long long)a.splits * rows * g->D * 4));
+    hipStream_t s = as_stream(stream);
+    ProfScope prof(VITMI_FAM_ATTN_FWD, s, 4.0 * rows * g->Nk * g->D);
+    const long long blocks = (long long)g->B * g->Hk * a.tiles * a.splits;
+    if (int rc = xa_run(p.few ? XK_FEW : XK_FWD, g->dt, a, xa_vec(g), blocks, s)) return rc;
+    if (a.splits > 1) {
+        const dim3 grid((unsigned)((rows + 3) / 4));
+        if (g->dt == VITMI_F32)
+            hipLaunchKernelGGL((xattn_join_kernel<float>), grid, dim3(256), 0, s, a, rows);
+        else
+            hipLaunchKernelGGL((xattn_join_kernel<bf16_t>), grid, dim3(256), 0, s, a, rows);
+        VITMI_LAUNCH_CHECK(who);
+    }
+    return VITMI_OK;
+}
+
+extern "C" long long vitmi_cross_attn_bwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
+    if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
+    if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
+    const XaPlan p = xa_plan(dt, B, Nq, Nk, Hq, Hk);
+    const long long rows = (long long)B * Nq * Hq, keys = (long long)B * Nk * Hk;
+    return up256(rows * 4) + (p.dq_splits > 1 ? up256(p.dq_splits * rows * D * 4) : 0) +
+           (p.dkv_splits > 1 ? 2 * up256(p.dkv_splits * keys * D * 4) : 0);
+}
+
+extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, void* stream) {
+    const char* who = "vitmi_cross_attn_bwd";
+    if (int rc = xa_check(who, g)) return rc;
+    VITMI_CHECK_ARG(g->B > 0 && g->Nq > 0 && g->Nk > 0, "%s: nothing to differentiate", who);
+    VITMI_CHECK_ARG(g->q && g->k && g->v && g->o && g->dout && g->lse && workspace, "%s: null pointer", who);
+    VITMI_CHECK_ARG((g->dk == nullptr) == (g->dv == nullptr), "%s: dk and dv come together", who);
+    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk);
+    XaArgs a;
+    xa_fill(g, &a);
+    const long long rows = (long long)g->B * g->Nq * g->Hq;
+    char* w = (char*)workspace;
+    a.delta = (float*)w;
+    w += up256(rows * 4);
+    if (p.dq_splits > 1) {
+        a.part_dq = (float*)w;
+        w += up256(p.dq_splits * a.n_q * 4);
+    }
+    if (p.dkv_splits > 1) {
+        a.part_dk = (float*)w;
+        a.part_dv = (float*)(w + up256(p.dkv_splits * a.n_k * 4));
+    }
+    const bool vec = xa_vec(g);
+    hipStream_t s = as_stream(stream);
+    ProfScope prof(VITMI_FAM_ATTN_BWD, s, 10.0 * rows * g->Nk * g->D);
+    a.tiles = p.dq_tiles;
+    a.splits = p.dq_splits;
+    if (int rc = xa_run(XK_DQ, g->dt, a, vec, (long long)g->B * g->Hk * a.tiles * a.splits, s)) return rc;
+    if (g->dq && a.splits > 1)
+        if (int rc = xa_sum(g->dt, a.part_dq, g->dq, g->scale, nullptr, nullptr, 0.f, a.n_q, a.splits, s)) return rc;
+    if (g->dk) {
+        a.tiles = p.dkv_tiles;
+        a.splits = p.dkv_splits;
+        if (int rc = xa_run(XK_DKV, g->dt, a, vec, (long long)g->B * g->Hk * a.tiles * a.splits, s)) return rc;
+        if (a.splits > 1)
+            if (int rc = xa_sum(g->dt, a.part_dk, g->dk, g->scale, a.part_dv, g->dv, 1.f, a.n_k, a.splits, s)) return rc;
+    }
+    return VITMI_OK;
+}

@@ -1,0 +1,696 @@
+// The residual update between two sub-blocks with the norms on both sides of it, one pass forwards and one backwards:
+//     p = post(u),   y = a x + s_b g * p,   h = pre(y)
+// u the branch's output, post / pre a LayerNorm, an RMS norm or nothing, g a gate per channel or per sample, s_b the
+// sample's branch scale (stochastic depth; a sample at 0 keeps y = a x and u is not read), a the residual scale.
+// With uh = (u - mu) r the normalised branch the affine part folds into the gate: s g p = s (uh * gw + gb),
+// gw = g * w_post, gb = g * b_post, so a row needs gw, gb and the parameters of pre, no more.
+//
+// Backward, per row:  t = dy + pre'(dh),  dx = a t,  du = post'(s t gw), and four column sums
+//     A = sum s t uh,  B = sum s t,  C = sum dh yh,  E = sum dh
+// from which every parameter gradient follows: dg = w_post A + b_post B, dw_post = g A, db_post = g B, dw_pre = C,
+// db_pre = E.  uh and yh are formed again from x and u in 32 bits (the stored y is rounded), the four row statistics
+// are kept by the forward pass.
+//
+// Bound by HBM (forward x, u -> y, h; backward dy, dh, x, u -> dx, du).  A row lives in the registers of one wave up to
+// 1024 elements, of 4 or 8 waves beyond, and is read once; parameters and column sums stay in registers while
+// a wave walks its rows.  Column sums are added over the workgroup's rows, written once per workgroup and reduced in a
+// fixed order by a second launch: no atomics, results are bitwise reproducible.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+enum { NG_NONE = 0, NG_LAYER = 1, NG_RMS = 2 };
+
+struct NgArgs {
+    const void *x, *u;
+    long long xs[2], us[2];            // batch and token strides of x and u
+    void *y, *h;                       // dense [rows, D]
+    const void* gate;
+    int gate_f32;                      // gate stored as fp32 (else bf16)
+    long long gate_stride;             // elements between samples; 0: one gate per channel
+    const float *branch_scale, *post_w, *post_b, *pre_w, *pre_b;
+    float* stats;                      // [4][rows]: mu_u, r_u, mu_y, r_y (NULL: not kept)
+    // backward
+    const void *dy, *dh;               // dense, may be NULL
+    void *dx, *du;                     // dense, may be NULL
+    float* partial;                    // [blocks][4][D]
+    long long rows;
+    int N, D, post, pre, chunks;       // chunks: row ranges per sample (gate per sample) or in all (gate per channel)
+    float res_scale, eps;
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) NVec {
+    T v[V];
+};
+
+// pair sums over the 64 lanes of a wave
+__device__ __forceinline__ void wave_sum2(float& a, float& b) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        a += __shfl_xor(a, o, 64);
+        b += __shfl_xor(b, o, 64);
+    }
+}
+
+// pair sums over the WPR waves that share a row; `red` alternates between two halves so that one barrier a call is enough
+template <int WPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& flip) {
+    wave_sum2(a, b);
+    if (WPR > 1) {
+        float* r = red + flip * 2 * WPR;
+        flip ^= 1;
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+            r[2 * w] = a;
+            r[2 * w + 1] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+            a += r[2 * i];
+            b += r[2 * i + 1];
+        }
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void load_f32v(const float* p, float (&o)[V]) {
+    const NVec<float, V> t = *reinterpret_cast<const NVec<float, V>*>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = t.v[j];
+}
+
+// what a thread's columns need of the parameters: gw = gate * post_w, gb = gate * post_b
+template <int V, int ITERS, int WPR>
+__device__ __forceinline__ void load_gate(const NgArgs& a, int b, float (&gw)[ITERS][V], float (&gb)[ITERS][V]) {
+    const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        const int c = (it * 64 * WPR + t) * V;
+        float g[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            g[j] = 1.f;
+            gb[it][j] = 0.f;
+        }
+        if (c < a.D) {
+            if (a.gate) {
+                const long long o = (long long)b * a.gate_stride + c;
+                if (a.gate_f32) {
+                    load_f32v<V>((const float*)a.gate + o, g);
+                } else {
+                    const NVec<bf16_t, V> tv = *reinterpret_cast<const NVec<bf16_t, V>*>((const bf16_t*)a.gate + o);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) g[j] = to_f32(tv.v[j]);
+                }
+            }
+            if (a.post_b) {
+                load_f32v<V>(a.post_b + c, gb[it]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) gb[it][j] *= g[j];
+            }
+            if (a.post_w) {
+                float w[V];
+                load_f32v<V>(a.post_w + c, w);
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[j] *= w[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) gw[it][j] = g[j];
+    }
+}
+
+template <int V, int ITERS, int WPR>
+__device__ __forceinline__ void load_param(const float* p, int D, float fill, float (&o)[ITERS][V]) {
+    const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        const int c = (it * 64 * WPR + t) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[it][j] = fill;
+        if (p && c < D) load_f32v<V>(p + c, o[it]);
+    }
+}
+
+template <typename T, int V, int ITERS, int WPR>
+__device__ __forceinline__ void fetch_row(const T* p, int D, NVec<T, V> (&o)[ITERS]) {
+    const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        const int c = (it * 64 * WPR + t) * V;
+        if (p && c < D) {
+            o[it] = *reinterpret_cast<const NVec<T, V>*>(p + c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[it].v[j] = from_f32<T>(0.f);
+        }
+    }
+}
+
+// mean and 1/sqrt(var + eps) of a row held in registers: deviations are taken from the mean in a second sweep over the
+// registers, so a large common offset costs no digits
+template <int V, int ITERS, int WPR>
+__device__ __forceinline__ void row_stats(const NgArgs& a, const float (&v)[ITERS][V], int kind, float& mu, float& r, float* red,
+                                          int& flip) {
+    const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+    mu = 0.f;
+    if (kind == NG_LAYER) {
+        float s = 0.f, z = 0.f;
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s += v[it][j];
+        row_sum2<WPR>(s, z, red, flip);
+        mu = s / (float)a.D;
+    }
+    float q = 0.f, z = 0.f;
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it) {
+        if ((it * 64 * WPR + t) * V < a.D) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = v[it][j] - mu;
+                q += d * d;
+            }
+        }
+    }
+    row_sum2<WPR>(q, z, red, flip);
+    r = rsqrtf(q / (float)a.D + a.eps);
+}
+
+template <typename TX, typename TU, int V, int ITERS, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void ngr_fwd_kernel(NgArgs a) {
+    constexpr int RPB = WPR == 1 ? 4 : 1;          // rows a workgroup works on at a time
+    __shared__ float red[4 * WPR];
+    int flip = 0;
+    const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+    const int wave = WPR == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0;
+    float gw[ITERS][V], gb[ITERS][V], pw[ITERS][V], pb[ITERS][V];
+    load_param<V, ITERS, WPR>(a.pre_w, a.D, 1.f, pw);
+    load_param<V, ITERS, WPR>(a.pre_b, a.D, 0.f, pb);
+    int gate_of = -1;
+    const long long stride = (long long)gridDim.x * RPB;
+    long long row = (long long)blockIdx.x * RPB + wave;
+    if (row >= a.rows) return;
+    NVec<TX, V> nx[ITERS];
+    NVec<TU, V> nu[ITERS];
+    float ns = 1.f;
+    int nb = 0;
+    auto fetch = [&](long long r) {
+        const long long b = r / a.N, n = r - b * a.N;
+        nb = (int)b;
+        ns = a.branch_scale ? a.branch_scale[b] : 1.f;
+        fetch_row<TX, V, ITERS, WPR>((const TX*)a.x + b * a.xs[0] + n * a.xs[1], a.D, nx);
+        fetch_row<TU, V, ITERS, WPR>(ns != 0.f ? (const TU*)a.u + b * a.us[0] + n * a.us[1] : (const TU*)nullptr, a.D, nu);
+    };
+    fetch(row);
+    for (; row < a.rows; row += stride) {
+        float xv[ITERS][V], uv[ITERS][V];
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                xv[it][j] = to_f32(nx[it].v[j]);
+                uv[it][j] = to_f32(nu[it].v[j]);
+            }
+        const float s = ns;
+        const int b = nb;
+        if (row + stride < a.rows) fetch(row + stride);
+        if (gate_of < 0 || (a.gate_stride && b != gate_of)) {
+            load_gate<V, ITERS, WPR>(a, b, gw, gb);
+            gate_of = b;
+        }
+        float mu = 0.f, ru = 1.f, my = 0.f, ry = 1.f;
+        if (s == 0.f)
+            ru = 0.f;
+        else if (a.post != NG_NONE)
+            row_stats<V, ITERS, WPR>(a, uv, a.post, mu, ru, red, flip);
+        TX* yr = (TX*)a.y + row * (long long)a.D;
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it) {
+            const int c = (it * 64 * WPR + t) * V;
+            NVec<TX, V> o;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float p = fmaf((uv[it][j] - mu) * ru, gw[it][j], gb[it][j]);
+                xv[it][j] = s == 0.f ? a.res_scale * xv[it][j] : fmaf(s, p, a.res_scale * xv[it][j]);
+                if (c >= a.D) xv[it][j] = 0.f;
+                o.v[j] = from_f32<TX>(xv[it][j]);
+            }
+            if (c < a.D) *reinterpret_cast<NVec<TX, V>*>(yr + c) = o;
+        }
+        if (a.pre != NG_NONE) {
+            row_stats<V, ITERS, WPR>(a, xv, a.pre, my, ry, red, flip);
+            TU* hr = (TU*)a.h + row * (long long)a.D;
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it) {
+                const int c = (it * 64 * WPR + t) * V;
+                if (c < a.D) {
+                    NVec<TU, V> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o.v[j] = from_f32<TU>(fmaf((xv[it][j] - my) * ry, pw[it][j], pb[it][j]));
+                    *reinterpret_cast<NVec<TU, V>*>(hr + c) = o;
+                }
+            }
+        }
+        if (a.stats && t == 0) {
+            a.stats[row] = mu;
+            a.stats[a.rows + row] = ru;
+            a.stats[2 * a.rows + row] = my;
+            a.stats[3 * a.rows + row] = ry;
+        }
+    }
+}
+
+// one workgroup: rows [r0, r1) of one range; with a gate per sample a range lies within one sample
+template <typename TX, typename TU, int V, int ITERS, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void ngr_bwd_kernel(NgArgs a) {
+    constexpr int RPB = WPR == 1 ? 4 : 1;
+    __shared__ float red[4 * WPR];
+    __shared__ float cols[WPR == 1 ? 3 * 64 * V : 1];
+    int flip = 0;
+    const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
+    const int wave = WPR == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0;
+    float gw[ITERS][V], gb[ITERS][V], pw[ITERS][V];
+    float sA[ITERS][V], sB[ITERS][V], sC[ITERS][V], sE[ITERS][V];
+    load_param<V, ITERS, WPR>(a.pre_w, a.D, 1.f, pw);
+#pragma unroll
+    for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sA[it][j] = sB[it][j] = sC[it][j] = sE[it][j] = 0.f;
+    const long long per = a.gate_stride ? a.N : a.rows;
+    const int seg = blockIdx.x / a.chunks, chunk = blockIdx.x - seg * a.chunks;
+    const long long r0 = seg * per + chunk * per / a.chunks, r1 = seg * per + (chunk + 1) * per / a.chunks;
+    load_gate<V, ITERS, WPR>(a, seg, gw, gb);
+    const float inv_d = 1.f / (float)a.D;
+    for (long long row = r0 + wave; row < r1; row += RPB) {
+        const long long b = row / a.N, n = row - b * a.N;
+        const float s = a.branch_scale ? a.branch_scale[b] : 1.f;
+        const bool live = s != 0.f;
+        NVec<TX, V> nx[ITERS], ndy[ITERS];
+        NVec<TU, V> nu[ITERS], ndh[ITERS];
+        const bool pre = a.pre != NG_NONE && a.dh;
+        fetch_row<TX, V, ITERS, WPR>(a.dy ? (const TX*)a.dy + row * a.D : (const TX*)nullptr, a.D, ndy);
+        fetch_row<TU, V, ITERS, WPR>(live ? (const TU*)a.u + b * a.us[0] + n * a.us[1] : (const TU*)nullptr, a.D, nu);
+        fetch_row<TU, V, ITERS, WPR>(pre ? (const TU*)a.dh + row * a.D : (const TU*)nullptr, a.D, ndh);
+        fetch_row<TX, V, ITERS, WPR>(pre ? (const TX*)a.x + b * a.xs[0] + n * a.xs[1] : (const TX*)nullptr, a.D, nx);
+        const float mu = a.stats[row], ru = a.stats[a.rows + row];
+        const float my = a.stats[2 * a.rows + row], ry = a.stats[3 * a.rows + row];
+        float tv[ITERS][V], uh[ITERS][V];
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                tv[it][j] = to_f32(ndy[it].v[j]);
+                uh[it][j] = (to_f32(nu[it].v[j]) - mu) * ru;
+            }
+        if (pre) {
+            float yh[ITERS][V];
+            float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it) {
+                const bool in = (it * 64 * WPR + t) * V < a.D;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float dh = to_f32(ndh[it].v[j]);
+                    const float ax = a.res_scale * to_f32(nx[it].v[j]);
+                    const float yv = live ? fmaf(s, fmaf(uh[it][j], gw[it][j], gb[it][j]), ax) : ax;
+                    yh[it][j] = in ? (yv - my) * ry : 0.f;
+                    sC[it][j] = fmaf(dh, yh[it][j], sC[it][j]);
+                    sE[it][j] += dh;
+                    const float g = dh * pw[it][j];
+                    c1 += g;
+                    c2 = fmaf(g, yh[it][j], c2);
+                }
+            }
+            row_sum2<WPR>(c1, c2, red, flip);
+            c1 = a.pre == NG_LAYER ? c1 * inv_d : 0.f;
+            c2 *= inv_d;
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    tv[it][j] = fmaf(ry, fmaf(to_f32(ndh[it].v[j]), pw[it][j], -c1) - yh[it][j] * c2, tv[it][j]);
+        }
+        if (a.dx) {
+            TX* dr = (TX*)a.dx + row * a.D;
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it) {
+                const int c = (it * 64 * WPR + t) * V;
+                if (c < a.D) {
+                    NVec<TX, V> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o.v[j] = from_f32<TX>(a.res_scale * tv[it][j]);
+                    *reinterpret_cast<NVec<TX, V>*>(dr + c) = o;
+                }
+            }
+        }
+        float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it) {
+            const bool in = (it * 64 * WPR + t) * V < a.D;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float st = live && in ? s * tv[it][j] : 0.f;
+                sA[it][j] = fmaf(st, uh[it][j], sA[it][j]);
+                sB[it][j] += st;
+                tv[it][j] = st * gw[it][j];
+                d1 += tv[it][j];
+                d2 = fmaf(tv[it][j], uh[it][j], d2);
+            }
+        }
+        if (a.du) {
+            if (a.post != NG_NONE) {
+                row_sum2<WPR>(d1, d2, red, flip);
+                d1 = a.post == NG_LAYER ? d1 * inv_d : 0.f;
+                d2 *= inv_d;
+#pragma unroll
+                for (int it = 0; it < ITERS; ++it)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) tv[it][j] = ru * ((tv[it][j] - d1) - uh[it][j] * d2);
+            }
+            TU* dr = (TU*)a.du + row * a.D;
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it) {
+                const int c = (it * 64 * WPR + t) * V;
+                if (c < a.D) {
+                    NVec<TU, V> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o.v[j] = from_f32<TU>(tv[it][j]);
+                    *reinterpret_cast<NVec<TU, V>*>(dr + c) = o;
+                }
+            }
+        }
+    }
+    if (!a.partial) return;
+    float* out = a.partial + (long long)blockIdx.x * 4 * a.D;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it) {
+            const int c = (it * 64 * WPR + t) * V;
+            float v[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = q == 0 ? sA[it][j] : q == 1 ? sB[it][j] : q == 2 ? sC[it][j] : sE[it][j];
+            if (WPR == 1) {                        // the four waves' sums meet in LDS, in wave order
+                __syncthreads();
+                if (wave > 0)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) cols[((wave - 1) * V + j) * 64 + t] = v[j];
+                __syncthreads();
+                if (wave == 0)
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+#pragma unroll
+                        for (int w = 0; w < 3; ++w) v[j] += cols[(w * V + j) * 64 + t];
+            }
+            if (wave == 0 && c < a.D) {
+                NVec<float, V> o;
+#pragma unroll
+                for (int j = 0; j < V; ++j) o.v[j] = v[j];
+                *reinterpret_cast<NVec<float, V>*>(out + (long long)q * a.D + c) = o;
+            }
+        }
+    }
+}
+
+struct NgFinal {
+    const float* partial;          // [segs][chunks][4][D]
+    const void* gate;
+    int gate_f32;
+    long long gate_stride;
+    const float *post_w, *post_b;
+    void* dgate;                   // [segs][D], of the gate's type
+    float *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+    int segs, chunks, D;
+};
+
+__device__ __forceinline__ float gate_at(const NgFinal& f, int seg, int c) {
+    if (!f.gate) return 1.f;
+    const long long o = (long long)seg * f.gate_stride + c;
+    return f.gate_f32 ? ((const float*)f.gate)[o] : to_f32(((const bf16_t*)f.gate)[o]);
+}
+
+// 64 columns x 16 row groups a workgroup, partials added in a fixed order; segments one after the other
+__global__ __launch_bounds__(1024) void ngr_final_kernel(NgFinal f) {
+    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    const int c = blockIdx.x * 64 + lane;
+    __shared__ float red[16][4][64];
+    float tw = 0.f, tb = 0.f, tc = 0.f, te = 0.f;
+    if (f.gate_stride == 0) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (c < f.D)
+            for (int k = grp; k < f.chunks; k += 16)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) s[q] += f.partial[((long long)k * 4 + q) * f.D + c];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) red[grp][q][lane] = s[q];
+        __syncthreads();
+        if (grp == 0 && c < f.D) {
+            for (int g = 0; g < 16; ++g) {
+                tw += red[g][0][lane];
+                tb += red[g][1][lane];
+                tc += red[g][2][lane];
+                te += red[g][3][lane];
+            }
+            const float g = gate_at(f, 0, c);
+            if (f.dgate) {
+                const float d = (f.post_w ? f.post_w[c] : 1.f) * tw + (f.post_b ? f.post_b[c] * tb : 0.f);
+                if (f.gate_f32) ((float*)f.dgate)[c] = d;
+                else ((bf16_t*)f.dgate)[c] = (bf16_t)d;
+            }
+            tw *= g;
+            tb *= g;
+        }
+    } else {
+        // a gate per sample: a row group takes samples grp, grp + 16, .., each over its chunks
+        if (c < f.D)
+            for (int seg = grp; seg < f.segs; seg += 16) {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < f.chunks; ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) s[q] += f.partial[(((long long)seg * f.chunks + k) * 4 + q) * f.D + c];
+                const float g = gate_at(f, seg, c);
+                if (f.dgate) {
+                    const float d = (f.post_w ? f.post_w[c] : 1.f) * s[0] + (f.post_b ? f.post_b[c] * s[1] : 0.f);
+                    if (f.gate_f32) ((float*)f.dgate)[(long long)seg * f.D + c] = d;
+                    else ((bf16_t*)f.dgate)[(long long)seg * f.D + c] = (bf16_t)d;
+                }
+                tw = fmaf(g, s[0], tw);
+                tb = fmaf(g, s[1], tb);
+                tc += s[2];
+                te += s[3];
+            }
+        red[grp][0][lane] = tw;
+        red[grp][1][lane] = tb;
+        red[grp][2][lane] = tc;
+        red[grp][3][lane] = te;
+        __syncthreads();
+        if (grp == 0) {
+            tw = tb = tc = te = 0.f;
+            for (int g = 0; g < 16; ++g) {
+                tw += red[g][0][lane];
+                tb += red[g][1][lane];
+                tc += red[g][2][lane];
+                te += red[g][3][lane];
+            }
+        }
+    }
+    if (grp == 0 && c < f.D) {
+        if (f.dpost_w) f.dpost_w[c] = tw;
+        if (f.dpost_b) f.dpost_b[c] = tb;
+        if (f.dpre_w) f.dpre_w[c] = tc;
+        if (f.dpre_b) f.dpre_b[c] = te;
+    }
+}
+
+struct NgPlan {
+    int V, iters, wpr;
+};
+
+// A row goes to the fewest waves that hold it in sixteen values per lane
+bool ng_plan(int D, bool vec, NgPlan* p) {
+    p->V = vec ? 4 : 1;
+    const int cap = vec ? 4 : 16;                    // vectors per lane
+    for (int w : {1, 4, 8}) {
+        const int iters = ceil_div(D, 64 * w * p->V);
+        if (iters <= cap) {
+            p->wpr = w;
+            p->iters = iters;
+            return true;
+        }
+    }
+    return false;
+}
+
+// partial-sum rows of the backward pass: two workgroups a compute unit, spread over the samples where the gate is per sample
+int ng_chunks(bool per_sample, int B, int N, int wpr) {
+    const long long rows = (long long)B * N;
+    const int rpb = wpr == 1 ? 4 : 1;
+    const int target = wpr <= 4 ? 512 : 256;
+    if (!per_sample) return (int)std::max<long long>(1, std::min<long long>(target, (rows + rpb - 1) / rpb));
+    return std::max(1, std::min(target / std::max(1, B), ceil_div(N, rpb)));
+}
+
+template <typename TX, typename TU, int V, int ITERS, int WPR>
+void ng_launch(const NgArgs& a, bool fwd, unsigned blocks, hipStream_t s) {
+    constexpr int THREADS = WPR == 1 ? 256 : 64 * WPR;
+    if (fwd)
+        hipLaunchKernelGGL((ngr_fwd_kernel<TX, TU, V, ITERS, WPR>), dim3(blocks), dim3(THREADS), 0, s, a);
+    else
+        hipLaunchKernelGGL((ngr_bwd_kernel<TX, TU, V, ITERS, WPR>), dim3(blocks), dim3(THREADS), 0, s, a);
+}
+
+template <typename TX, typename TU, int V, int WPR>
+void ng_iters(const NgArgs& a, int iters, bool fwd, unsigned blocks, hipStream_t s) {
+    if (V == 4) {
+        if (iters <= 1) ng_launch<TX, TU, 4, 1, WPR>(a, fwd, blocks, s);
+        else if (iters == 2) ng_launch<TX, TU, 4, 2, WPR>(a, fwd, blocks, s);
+        else if (iters == 3) ng_launch<TX, TU, 4, 3, WPR>(a, fwd, blocks, s);
+        else ng_launch<TX, TU, 4, 4, WPR>(a, fwd, blocks, s);
+    } else {
+        if (iters <= 4) ng_launch<TX, TU, 1, 4, WPR>(a, fwd, blocks, s);
+        else ng_launch<TX, TU, 1, 16, WPR>(a, fwd, blocks, s);
+    }
+}
+
+template <typename TX, typename TU>
+void ng_dispatch(const NgArgs& a, const NgPlan& p, bool fwd, unsigned blocks, hipStream_t s) {
+#define NG_W(V)                                                                    \
+    do {                                                                           \
+        if (p.wpr == 1) ng_iters<TX, TU, V, 1>(a, p.iters, fwd, blocks, s);        \
+        else if (p.wpr == 4) ng_iters<TX, TU, V, 4>(a, p.iters, fwd, blocks, s);   \
+        else ng_iters<TX, TU, V, 8>(a, p.iters, fwd, blocks, s);                   \
+    } while (0)
+    if (p.V == 4) NG_W(4);
+    else NG_W(1);
+#undef NG_W
+}
+
+bool ng_types_ok(int dx, int du) {
+    return (dx == VITMI_F32 && (du == VITMI_F32 || du == VITMI_BF16)) || (dx == VITMI_BF16 && du == VITMI_BF16);
+}
+
+int ng_check(const char* who, const vitmi_ngr_args* g) {
+    VITMI_CHECK_ARG(g, "%s: null arguments", who);
+    VITMI_CHECK_ARG(ng_types_ok(g->dt_x, g->dt_u), "%s: residual type %d with branch type %d (fp32 or bf16, the residual at least as wide)",
+                    who, g->dt_x, g->dt_u);
+    VITMI_CHECK_ARG(g->B >= 0 && g->N >= 0 && g->D > 0, "%s: bad shape B=%d N=%d D=%d", who, g->B, g->N, g->D);
+    VITMI_CHECK_ARG(g->post >= 0 && g->post <= 2 && g->pre >= 0 && g->pre <= 2, "%s: bad norm kind %d / %d", who, g->post, g->pre);
+    VITMI_CHECK_ARG(!g->gate || g->gate_dt == VITMI_F32 || g->gate_dt == VITMI_BF16, "%s: bad gate type %d", who, g->gate_dt);
+    if (g->D > 8192) {
+        vitmi_set_error("%s: D=%d exceeds the supported row length 8192", who, g->D);
+        return VITMI_ERR_UNSUPPORTED;
+    }
+    return VITMI_OK;
+}
+
+bool ng_vec(const vitmi_ngr_args* g) {
+    if (g->D % 4) return false;
+    const uintptr_t ex = g->dt_x == VITMI_F32 ? 16 : 8, eu = g->dt_u == VITMI_F32 ? 16 : 8, eg = g->gate_dt == VITMI_F32 ? 16 : 8;
+    auto al = [](const void* p, uintptr_t m) { return (reinterpret_cast<uintptr_t>(p) & (m - 1)) == 0; };
+    for (int i = 0; i < 2; ++i)
+        if (g->xs[i] % 4 || g->us[i] % 4) return false;
+    if (g->gate && (g->gate_stride % 4 || !al(g->gate, eg))) return false;
+    return al(g->x, ex) && al(g->u, eu) && al(g->y, ex) && al(g->h, eu) && al(g->post_w, 16) && al(g->post_b, 16) &&
+           al(g->pre_w, 16) && al(g->pre_b, 16) && al(g->dy, ex) && al(g->dh, eu) && al(g->dx, ex) && al(g->du, eu);
+}
+
+void ng_fill(const vitmi_ngr_args* g, NgArgs* a) {
+    *a = NgArgs{};
+    a->x = g->x; a->u = g->u; a->y = g->y; a->h = g->h;
+    for (int i = 0; i < 2; ++i) {
+        a->xs[i] = g->xs[i];
+        a->us[i] = g->us[i];
+    }
+    a->gate = g->gate;
+    a->gate_f32 = g->gate_dt == VITMI_F32;
+    a->gate_stride = g->gate ? g->gate_stride : 0;
+    a->branch_scale = g->branch_scale;
+    a->post_w = g->post == NG_NONE ? nullptr : g->post_w;
+    a->post_b = g->post == NG_NONE ? nullptr : g->post_b;
+    a->pre_w = g->pre == NG_NONE ? nullptr : g->pre_w;
+    a->pre_b = g->pre == NG_NONE ? nullptr : g->pre_b;
+    a->stats = g->stats;
+    a->dy = g->dy; a->dh = g->dh; a->dx = g->dx; a->du = g->du;
+    a->rows = (long long)g->B * g->N;
+    a->N = g->N; a->D = g->D; a->post = g->post; a->pre = g->pre;
+    a->res_scale = g->res_scale;
+    a->eps = g->eps;
+}
+
+}  // namespace
+
+extern "C" int vitmi_norm_gate_residual_fwd(const vitmi_ngr_args* g, void* stream) {
+    const char* who = "vitmi_norm_gate_residual_fwd";
+    if (int rc = ng_check(who, g)) return rc;
+    if (g->B == 0 || g->N == 0) return VITMI_OK;
+    VITMI_CHECK_ARG(g->x && g->u && g->y && (g->pre == NG_NONE || g->h), "%s: null pointer", who);
+    NgPlan p;
+    if (!ng_plan(g->D, ng_vec(g), &p)) {
+        vitmi_set_error("%s: no plan for D=%d", who, g->D);
+        return VITMI_ERR_UNSUPPORTED;
+    }
+    NgArgs a;
+    ng_fill(g, &a);
+    hipStream_t s = as_stream(stream);
+    const int ex = g->dt_x == VITMI_F32 ? 4 : 2, eu = g->dt_u == VITMI_F32 ? 4 : 2;
+    ProfScope prof(VITMI_FAM_LAYERNORM, s, (double)a.rows * g->D * (2 * ex + eu * (g->pre ? 2 : 1)));
+    const int rpb = p.wpr == 1 ? 4 : 1;
+    // sixteen waves a compute unit walk the rows, each with its next row's loads outstanding
+    const long long cap = p.wpr == 8 ? 512 : 1024;
+    const unsigned blocks = (unsigned)std::min<long long>((a.rows + rpb - 1) / rpb, cap);
+    if (g->dt_x == VITMI_BF16) ng_dispatch<bf16_t, bf16_t>(a, p, true, blocks, s);
+    else if (g->dt_u == VITMI_BF16) ng_dispatch<float, bf16_t>(a, p, true, blocks, s);
+    else ng_dispatch<float, float>(a, p, true, blocks, s);
+    VITMI_LAUNCH_CHECK(who);
+    return VITMI_OK;
+}
+
+extern "C" long long vitmi_norm_gate_residual_bwd_workspace_bytes(int B, int N, int D, int gate_per_sample) {
+    if (B <= 0 || N <= 0 || D <= 0) return 0;
+    // the plan depends on alignment: room for the most row ranges any plan makes
+    const long long a = ng_chunks(gate_per_sample != 0, B, N, 1), b = ng_chunks(gate_per_sample != 0, B, N, 4);
+    return std::max(a, b) * (gate_per_sample ? B : 1) * 4ll * D * (long long)sizeof(float);
+}
+
+extern "C" int vitmi_norm_gate_residual_bwd(const vitmi_ngr_args* g, void* workspace, void* stream) {
+    const char* who = "vitmi_norm_gate_residual_bwd";
+    if (int rc = ng_check(who, g)) return rc;
+    const bool per_sample = g->gate && g->gate_stride != 0;
+    const bool sums = g->dgate || g->dpost_w || g->dpost_b || g->dpre_w || g->dpre_b;
+    VITMI_CHECK_ARG(g->B > 0 && g->N > 0, "%s: no rows", who);
+    VITMI_CHECK_ARG(g->x && g->u && g->stats && (g->dy || g->dh) && (workspace || !sums), "%s: null pointer", who);
+    VITMI_CHECK_ARG(!g->dgate || g->gate, "%s: gradient of an absent gate", who);
+    NgPlan p;
+    if (!ng_plan(g->D, ng_vec(g), &p)) {
+        vitmi_set_error("%s: no plan for D=%d", who, g->D);
+        return VITMI_ERR_UNSUPPORTED;
+    }
+    VITMI_CHECK_ARG(!per_sample || g->B < (1 << 22), "%s: gates of %d samples are beyond one launch", who, g->B);
+    NgArgs a;
+    ng_fill(g, &a);
+    a.chunks = ng_chunks(per_sample, g->B, g->N, p.wpr);
+    a.partial = sums ? (float*)workspace : nullptr;
+    const int segs = per_sample ? g->B : 1;
+    hipStream_t s = as_stream(stream);
+    const int ex = g->dt_x == VITMI_F32 ? 4 : 2, eu = g->dt_u == VITMI_F32 ? 4 : 2;
+    ProfScope prof(VITMI_FAM_LAYERNORM, s, (double)a.rows * g->D * (3 * ex + 3 * eu));
+    const unsigned blocks = (unsigned)(segs * a.chunks);
+    if (g->dt_x == VITMI_BF16) ng_dispatch<bf16_t, bf16_t>(a, p, false, blocks, s);
+    else if (g->dt_u == VITMI_BF16) ng_dispatch<float, bf16_t>(a, p, false, blocks, s);
+    else ng_dispatch<float, float>(a, p, false, blocks, s);
+    VITMI_LAUNCH_CHECK(who);
+    if (sums) {
+        NgFinal f = {a.partial, a.gate, a.gate_f32, a.gate_stride, a.post_w, a.post_b, g->dgate, g->dpost_w, g->dpost_b,
+                     g->dpre_w, g->dpre_b, segs, a.chunks, g->D};
+        hipLaunchKernelGGL(ngr_final_kernel, dim3(ceil_div(g->D, 64)), dim3(1024), 0, s, f);
+        VITMI_LAUNCH_CHECK(who);
+    }
+    return VITMI_OK;
+}

@@ -1,0 +1,273 @@
+// Rotary positions with several axes (time, height, width) on query / key rows [B, N, H, DH].
+//
+// Pair p of a head belongs to axis a and turns by theta = pos_a * base_a^(-j / s_a), j its index within the axis (or
+// p / P over one ladder shared by the axes):
+//     y1 = x1 cos(theta) - x2 sin(theta),   y2 = x2 cos(theta) + x1 sin(theta),
+// the pair being dims (p, P + p) or (2p, 2p + 1); dims from 2P on pass through.  The backward pass is the same with -theta.
+//
+// Bound by HBM: every element is read once and written once, three operations each.  A workgroup takes a tile of
+// tokens of one sample and ALL heads of both tensors, so that the angles of a token (the only expensive arithmetic) are
+// formed once per tile and shared by the heads through LDS; its first row loads are on their way meanwhile.
+// The angle is formed in turns in 64 bits and reduced to an eighth of a turn there -- a far position times a frequency
+// keeps no fraction of a turn in 32 bits -- and only the reduced angle goes to the 32-bit sine and cosine.
+#include <algorithm>
+
+#include "common.h"
+
+namespace {
+
+constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_MAX_PAIRS = 256;
+
+struct RopeTensor {
+    const void* x;
+    void* y;
+    long long xs[3], ys[3];   // batch, token, head strides
+};
+struct RopeArgs {
+    RopeTensor t[2];
+    const void* pos;
+    long long ps[3];          // batch, token, axis strides
+    double log2_base[4];
+    int first_pair[5];        // first pair of each axis; [axes] = P
+    int axes, pos_type, P, DH, N, tile, tiles;
+    int units_tok, units_0;   // units per token, of which the first tensor's
+    int units_head, units_rot;
+    int copy_rest;            // the pass-through dims are copied (not in place)
+    int shared, inverse;
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) RVec {
+    T v[V];
+};
+
+template <typename T, int V>
+struct RopeUnit {
+    RVec<T, V> a, b;
+    long long out;            // element offset of the unit's first vector in y
+    int tok, pair;            // pair < 0: a pass-through unit (vector a only)
+    int which;                // 0 / 1: tensor; -1: no unit
+};
+
+__device__ __forceinline__ double rope_pos(const RopeArgs& a, long long off) {
+    if (a.pos_type == VITMI_POS_I64) return (double)((const long long*)a.pos)[off];
+    if (a.pos_type == VITMI_POS_I32) return (double)((const int*)a.pos)[off];
+    return (double)((const float*)a.pos)[off];
+}
+
+// cos and sin of 2 pi * turns, turns in 64 bits; the 32-bit functions see at most an eighth of a turn
+__device__ __forceinline__ float2 rope_cos_sin(double turns) {
+    const double t = turns - rint(turns), q = rint(4.0 * t);
+    const float r = (float)(2.0 * (t - 0.25 * q));    // half turns in [-1/4, 1/4]
+    float s, c;
+    sincospif(r, &s, &c);
+    const int k = (int)q & 3;
+    const float c1 = (k & 1) ? -s : c, s1 = (k & 1) ? c : s;
+    return (k & 2) ? make_float2(-c1, -s1) : make_float2(c1, s1);
+}
+
+template <typename T, int V, bool INTER>
+__device__ __forceinline__ void rope_fetch(const RopeArgs& a, RopeUnit<T, V>& r, int u, int total, int b, int n0) {
+    r.which = -1;
+    if (u >= total) return;
+    const int tok = u / a.units_tok;
+    int rem = u - tok * a.units_tok;
+    const int w = rem >= a.units_0;
+    if (w) rem -= a.units_0;
+    const int head = rem / a.units_head, c = rem - head * a.units_head;
+    const RopeTensor& t = w ? a.t[1] : a.t[0];
+    const bool rot = c < a.units_rot;
+    const int d = rot ? c * V * (INTER ? 2 : 1) : 2 * a.P + (c - a.units_rot) * V;
+    const T* x = (const T*)t.x + b * t.xs[0] + (n0 + tok) * t.xs[1] + head * t.xs[2] + d;
+    r.out = b * t.ys[0] + (n0 + tok) * t.ys[1] + head * t.ys[2] + d;
+    r.which = w;
+    r.tok = tok;
+    r.pair = rot ? c * V : -1;
+    r.a = *reinterpret_cast<const RVec<T, V>*>(x);
+    if (rot) r.b = *reinterpret_cast<const RVec<T, V>*>(x + (INTER ? V : a.P));
+}
+
+template <typename T, int V, bool INTER>
+__device__ __forceinline__ void rope_finish(const RopeArgs& a, RopeUnit<T, V>& r, const float2* cs) {
+    if (r.which < 0) return;
+    T* y = (T*)(r.which ? a.t[1].y : a.t[0].y) + r.out;
+    if (r.pair < 0) {
+        *reinterpret_cast<RVec<T, V>*>(y) = r.a;
+        return;
+    }
+    const float2* w = cs + r.tok * a.P + r.pair;
+    if (INTER) {
+        float e[2 * V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            e[j] = to_f32(r.a.v[j]);
+            e[V + j] = to_f32(r.b.v[j]);
+        }
+        T o[2 * V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float2 t = w[j];
+            o[2 * j] = from_f32<T>(e[2 * j] * t.x - e[2 * j + 1] * t.y);
+            o[2 * j + 1] = from_f32<T>(e[2 * j + 1] * t.x + e[2 * j] * t.y);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            r.a.v[j] = o[j];
+            r.b.v[j] = o[V + j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float2 t = w[j];
+            const float p = to_f32(r.a.v[j]), q = to_f32(r.b.v[j]);
+            r.a.v[j] = from_f32<T>(p * t.x - q * t.y);
+            r.b.v[j] = from_f32<T>(q * t.x + p * t.y);
+        }
+    }
+    *reinterpret_cast<RVec<T, V>*>(y) = r.a;
+    *reinterpret_cast<RVec<T, V>*>(y + (INTER ? V : a.P)) = r.b;
+}
+
+template <typename T, int V, bool INTER>
+__global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeArgs a) {
+    extern __shared__ double rope_lds[];
+    double* freq = rope_lds;                                   // [P] turns per position step
+    float2* cs = reinterpret_cast<float2*>(rope_lds + a.P);     // [tile][P]
+    const int b = blockIdx.x / a.tiles, n0 = (blockIdx.x - b * a.tiles) * a.tile;
+    const int toks = min(a.tile, a.N - n0);
+    const int total = toks * a.units_tok;
+    constexpr int K = 2;
+    RopeUnit<T, V> r[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) rope_fetch<T, V, INTER>(a, r[i], (int)threadIdx.x + i * ROPE_THREADS, total, b, n0);
+
+    if ((int)threadIdx.x < a.P) {
+        const int p = threadIdx.x;
+        int ax = 0;
+        while (p >= a.first_pair[ax + 1]) ++ax;
+        const double e = a.shared ? (double)p / a.P
+                                  : (double)(p - a.first_pair[ax]) / (a.first_pair[ax + 1] - a.first_pair[ax]);
+        freq[p] = exp2(-e * a.log2_base[ax]) * 0.15915494309189533577;   // 1 / (2 pi)
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < toks * a.P; i += ROPE_THREADS) {
+        const int tok = i / a.P, p = i - tok * a.P;
+        int ax = 0;
+        while (p >= a.first_pair[ax + 1]) ++ax;
+        float2 w = rope_cos_sin(rope_pos(a, b * a.ps[0] + (n0 + tok) * a.ps[1] + ax * a.ps[2]) * freq[p]);
+        if (a.inverse) w.y = -w.y;
+        cs[i] = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < K; ++i) rope_finish<T, V, INTER>(a, r[i], cs);
+    for (int u = (int)threadIdx.x + K * ROPE_THREADS; u < total; u += K * ROPE_THREADS) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) rope_fetch<T, V, INTER>(a, r[i], u + i * ROPE_THREADS, total, b, n0);
+#pragma unroll
+        for (int i = 0; i < K; ++i) rope_finish<T, V, INTER>(a, r[i], cs);
+    }
+}
+
+template <typename T, int V>
+void launch_rope(const RopeArgs& k, bool inter, unsigned blocks, size_t lds, hipStream_t s) {
+    if (inter)
+        hipLaunchKernelGGL((rope_kernel<T, V, true>), dim3(blocks), dim3(ROPE_THREADS), lds, s, k);
+    else
+        hipLaunchKernelGGL((rope_kernel<T, V, false>), dim3(blocks), dim3(ROPE_THREADS), lds, s, k);
+}
+
+}  // namespace
+
+extern "C" int vitmi_rope_axes(const vitmi_rope_args* a, void* stream) {
+    VITMI_CHECK_ARG(a, "vitmi_rope_axes: null arguments");
+    VITMI_CHECK_ARG(a->dt == VITMI_F32 || a->dt == VITMI_BF16, "vitmi_rope_axes: bad dtype %d", a->dt);
+    VITMI_CHECK_ARG(a->axes >= 1 && a->axes <= 4, "vitmi_rope_axes: %d axes, 1 to 4 are supported", a->axes);
+    VITMI_CHECK_ARG(a->pos_type == VITMI_POS_I32 || a->pos_type == VITMI_POS_I64 || a->pos_type == VITMI_POS_F32,
+                    "vitmi_rope_axes: bad position type %d", a->pos_type);
+    VITMI_CHECK_ARG(a->B >= 0 && a->N >= 0 && a->DH > 0 && a->t[0].heads > 0, "vitmi_rope_axes: bad shape B=%d N=%d DH=%d H=%d",
+                    a->B, a->N, a->DH, a->t[0].heads);
+    RopeArgs k = {};
+    int P = 0;
+    for (int i = 0; i < a->axes; ++i) {
+        VITMI_CHECK_ARG(a->sections[i] > 0 && a->sections[i] <= ROPE_MAX_PAIRS, "vitmi_rope_axes: section %d holds %d pairs", i,
+                        a->sections[i]);
+        VITMI_CHECK_ARG(a->log2_base[i] > 0, "vitmi_rope_axes: the base of axis %d must be above 1", i);
+        k.first_pair[i] = P;
+        k.log2_base[i] = a->log2_base[i];
+        P += a->sections[i];
+    }
+    for (int i = a->axes; i < 5; ++i) k.first_pair[i] = P;
+    VITMI_CHECK_ARG(P <= ROPE_MAX_PAIRS && 2 * P <= a->DH, "vitmi_rope_axes: %d pairs do not fit a head of %d (at most %d)", P,
+                    a->DH, ROPE_MAX_PAIRS);
+    if (a->B == 0 || a->N == 0) return VITMI_OK;
+    VITMI_CHECK_ARG(a->pos && a->t[0].x && a->t[0].y, "vitmi_rope_axes: null pointer");
+    VITMI_CHECK_ARG(!a->t[1].x || (a->t[1].y && a->t[1].heads > 0), "vitmi_rope_axes: second tensor without output or heads");
+
+    const int esz = a->dt == VITMI_F32 ? 4 : 2;
+    const int nt = a->t[1].x ? 2 : 1;
+    // widest vector of V elements (16 bytes and below) that pairs, rest, strides and pointers are all multiples of
+    int V = a->dt == VITMI_F32 ? 4 : 8;
+    auto fits = [&](int v) {
+        if (P % v || (a->DH - 2 * P) % v) return false;
+        for (int i = 0; i < nt; ++i) {
+            const vitmi_rope_tensor& t = a->t[i];
+            if ((reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.y)) % (v * esz)) return false;
+            for (int d = 0; d < 3; ++d)
+                if (t.xs[d] % v || t.ys[d] % v) return false;
+        }
+        return true;
+    };
+    if (V == 8 && !fits(8)) V = 4;
+    if (V == 4 && !fits(4)) V = 1;
+    long long heads = 0;
+    bool in_place = true;
+    for (int i = 0; i < nt; ++i) {
+        const vitmi_rope_tensor& t = a->t[i];
+        k.t[i].x = t.x;
+        k.t[i].y = t.y;
+        for (int d = 0; d < 3; ++d) {
+            k.t[i].xs[d] = t.xs[d];
+            k.t[i].ys[d] = t.ys[d];
+            in_place = in_place && t.xs[d] == t.ys[d];
+        }
+        in_place = in_place && t.x == t.y;
+        heads += t.heads;
+    }
+    k.pos = a->pos;
+    for (int d = 0; d < 3; ++d) k.ps[d] = a->pos_stride[d];
+    k.axes = a->axes;
+    k.pos_type = a->pos_type;
+    k.P = P;
+    k.DH = a->DH;
+    k.N = a->N;
+    k.shared = a->shared_ladder;
+    k.inverse = a->inverse;
+    k.units_rot = P / V;
+    k.units_head = k.units_rot + (in_place ? 0 : (a->DH - 2 * P) / V);
+    const long long ut = heads * k.units_head;
+    VITMI_CHECK_ARG(ut * 8 < (1ll << 31), "vitmi_rope_axes: %lld heads of %d are beyond one call", heads, a->DH);
+    k.units_tok = (int)ut;
+    k.units_0 = a->t[0].heads * k.units_head;
+    // tokens per workgroup: eight share one round of angles, fewer while that leaves compute units without work
+    int tile = 8;
+    while (tile > 1 && (long long)a->B * ceil_div(a->N, tile) < 1024) tile >>= 1;
+    k.tile = tile;
+    k.tiles = ceil_div(a->N, tile);
+    const long long blocks = (long long)a->B * k.tiles;
+    VITMI_CHECK_ARG(blocks < (1ll << 32) / ROPE_THREADS, "vitmi_rope_axes: %lld tiles are beyond one launch", blocks);
+    hipStream_t s = as_stream(stream);
+    ProfScope prof(VITMI_FAM_OTHER, s, 2.0 * a->B * a->N * heads * a->DH * esz);
+    const size_t lds = (size_t)P * 8 * (1 + tile);
+    if (a->dt == VITMI_F32) {
+        if (V == 4) launch_rope<float, 4>(k, a->interleaved, (unsigned)blocks, lds, s);
+        else launch_rope<float, 1>(k, a->interleaved, (unsigned)blocks, lds, s);
+    } else {
+        if (V == 8) launch_rope<bf16_t, 8>(k, a->interleaved, (unsigned)blocks, lds, s);
+        else if (V == 4) launch_rope<bf16_t, 4>(k, a->interleaved, (unsigned)blocks, lds, s);
+        else launch_rope<bf16_t, 1>(k, a->interleaved, (unsigned)blocks, lds, s);
+    }
+    VITMI_LAUNCH_CHECK("vitmi_rope_axes");
+    return VITMI_OK;
+}

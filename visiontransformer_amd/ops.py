@@ -4,6 +4,7 @@ Every function here moves raw device pointers, shapes and the current HIP stream
 boundary; tensors are allocated by PyTorch's caching allocator.  There is no CPU or eager
 fallback: CPU tensors raise.
 """
+import math
 import os
 import weakref
 
@@ -1591,3 +1592,428 @@ class MeanPoolFn(torch.autograd.Function):
         dx = torch.empty((B, ctx.n, D), dtype=dout.dtype, device=dout.device)
         check(lib.vitmi_meanpool_bwd(_p(dout), _p(dx), _dt(dout), B, ctx.n, D, _stream()), "vitmi_meanpool_bwd")
         return dx
+
+
+# ---------------------------------------------------------------------------------------------
+# decoder-block operators: rotary positions with several axes, cross attention, the residual update with its norms
+# ---------------------------------------------------------------------------------------------
+class _RopeTensor(_ct.Structure):
+    _fields_ = [("x", _ct.c_void_p), ("y", _ct.c_void_p), ("xs", _ct.c_longlong * 3), ("ys", _ct.c_longlong * 3),
+                ("heads", _ct.c_int), ("pad", _ct.c_int)]
+
+
+class _RopeArgs(_ct.Structure):
+    _fields_ = [("t", _RopeTensor * 2), ("pos", _ct.c_void_p), ("pos_stride", _ct.c_longlong * 3),
+                ("log2_base", _ct.c_double * 4), ("sections", _ct.c_int * 4), ("axes", _ct.c_int), ("pos_type", _ct.c_int),
+                ("dt", _ct.c_int), ("B", _ct.c_int), ("N", _ct.c_int), ("DH", _ct.c_int), ("interleaved", _ct.c_int),
+                ("shared_ladder", _ct.c_int), ("inverse", _ct.c_int), ("pad", _ct.c_int)]
+
+
+class _XattnArgs(_ct.Structure):
+    _fields_ = [("q", _ct.c_void_p), ("k", _ct.c_void_p), ("v", _ct.c_void_p), ("o", _ct.c_void_p),
+                ("qs", _ct.c_longlong * 3), ("ks", _ct.c_longlong * 3), ("vs", _ct.c_longlong * 3),
+                ("kv_len", _ct.c_void_p), ("key_mask", _ct.c_void_p), ("mask_stride", _ct.c_longlong),
+                ("lse", _ct.c_void_p), ("dout", _ct.c_void_p), ("dos", _ct.c_longlong * 3), ("dq", _ct.c_void_p),
+                ("dk", _ct.c_void_p), ("dv", _ct.c_void_p), ("kv_len_i64", _ct.c_int), ("dt", _ct.c_int),
+                ("B", _ct.c_int), ("Nq", _ct.c_int), ("Nk", _ct.c_int), ("Hq", _ct.c_int), ("Hk", _ct.c_int),
+                ("D", _ct.c_int), ("scale", _ct.c_float), ("pad", _ct.c_int)]
+
+
+class _NgrArgs(_ct.Structure):
+    _fields_ = [("x", _ct.c_void_p), ("u", _ct.c_void_p), ("xs", _ct.c_longlong * 2), ("us", _ct.c_longlong * 2),
+                ("y", _ct.c_void_p), ("h", _ct.c_void_p), ("gate", _ct.c_void_p), ("gate_stride", _ct.c_longlong),
+                ("branch_scale", _ct.c_void_p), ("post_w", _ct.c_void_p), ("post_b", _ct.c_void_p),
+                ("pre_w", _ct.c_void_p), ("pre_b", _ct.c_void_p), ("stats", _ct.c_void_p), ("dy", _ct.c_void_p),
+                ("dh", _ct.c_void_p), ("dx", _ct.c_void_p), ("du", _ct.c_void_p), ("dgate", _ct.c_void_p),
+                ("dpost_w", _ct.c_void_p), ("dpost_b", _ct.c_void_p), ("dpre_w", _ct.c_void_p), ("dpre_b", _ct.c_void_p),
+                ("gate_dt", _ct.c_int), ("dt_x", _ct.c_int), ("dt_u", _ct.c_int), ("B", _ct.c_int), ("N", _ct.c_int),
+                ("D", _ct.c_int), ("post", _ct.c_int), ("pre", _ct.c_int), ("res_scale", _ct.c_float), ("eps", _ct.c_float)]
+
+
+class _on_device:
+    """Makes t's device the current one for a launch when it is not already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, t):
+        cur = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+        self.guard = None if t.device.index == cur else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _same_device(first, *rest):
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors of a call live on one device, got {first.device} and {t.device}")
+
+
+def _builds_graph(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _heads4(name, t):
+    """[B, N, H, D] with unit stride over D (a copy only where the layout has another)."""
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be [batch, tokens, heads, head dim], got {tuple(t.shape)}")
+    return t if t.stride(3) == 1 or t.shape[3] == 1 or t.numel() == 0 else t.contiguous()
+
+
+def _s3(t):
+    s = t.stride()
+    return s[:3]
+
+
+_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _rope_launch(xs, outs, pos, sections, log2_base, interleaved, shared, inverse):
+    a = _RopeArgs()
+    B, N, _, DH = xs[0].shape
+    for i, (x, y) in enumerate(zip(xs, outs)):
+        t = a.t[i]
+        t.x, t.y, t.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
+        t.xs[:] = _s3(x)
+        t.ys[:] = _s3(y)
+    ps = pos.stride()
+    a.pos = pos.data_ptr()
+    a.pos_stride[:] = ps if pos.dim() == 3 else (0,) + ps
+    n = len(sections)
+    a.log2_base[:n] = log2_base
+    a.sections[:n] = sections
+    a.axes, a.pos_type, a.dt, a.B, a.N, a.DH = n, _POS_TYPES[pos.dtype], _dt(xs[0]), B, N, DH
+    a.interleaved, a.shared_ladder, a.inverse = interleaved, shared, inverse
+    with _on_device(xs[0]):
+        check(lib.vitmi_rope_axes(_ct.addressof(a), _stream()), "vitmi_rope_axes")
+    return outs
+
+
+class RopeAxesFn(torch.autograd.Function):
+    """The node behind rope_axes; the backward pass is the same launch with the angles turned round."""
+
+    @staticmethod
+    def forward(ctx, q, k, pos, sections, log2_base, interleaved, shared):
+        xs = [t for t in (q, k) if t is not None]
+        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+        _rope_launch(xs, outs, pos, sections, log2_base, interleaved, shared, False)
+        ctx.save_for_backward(pos)
+        ctx.meta = (sections, log2_base, interleaved, shared, k is not None)
+        ctx.set_materialize_grads(False)
+        return tuple(outs) if k is not None else outs[0]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        if _PS2 is not None:                # a replay forms no input gradients
+            return tuple(None if g is None else _no_grad_like(g.shape, g.dtype, g.device) for g in grads) + \
+                (None,) * (7 - len(grads))
+        pos, = ctx.saved_tensors
+        sections, log2_base, interleaved, shared, two = ctx.meta
+        res = [None, None]
+        want = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
+        if want:
+            gs = [_heads4("gradient", grads[i]) for i in want]
+            outs = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in gs]
+            _rope_launch(gs, outs, pos, sections, log2_base, interleaved, shared, True)
+            for i, o in zip(want, outs):
+                res[i] = o
+        return res[0], res[1], None, None, None, None, None
+
+
+def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladder=False, inplace=False):
+    """Rotary positions with several axes (time, height, width) on queries [B, N, Hq, D] and, unless None, keys
+    [B, N, Hk, D] of the same tokens, in one launch; differentiable.  Returns the rotated (q, k), or q alone.
+
+    pos [N, A] or [B, N, A] (int32, int64 or float32) holds a token's position on each axis; position 0 on every axis
+    leaves a token as it is (class token).  sections: how many of the head's pairs turn with each axis; pair j of an axis
+    with s pairs turns by pos * base^(-j / s) (base a number or one per axis), or, with shared_ladder, pair p of all P by
+    pos * base^(-p / P).  A pair is dims (p, P + p), or (2p, 2p + 1) with interleaved; dims from 2P on pass through.
+    q and k may be strided views (the slots of a packed projection); the results are dense.  inplace rotates q and k
+    where they lie, outside of autograd only."""
+    q = _heads4("q", q) if not inplace else q
+    if k is not None:
+        k = _heads4("k", k) if not inplace else k
+        if k.dtype != q.dtype or (k.shape[0], k.shape[1], k.shape[3]) != (q.shape[0], q.shape[1], q.shape[3]):
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in everything but heads")
+    _dt(q)
+    B, N, _, D = q.shape
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 1:
+        raise ValueError(f"sections {sections}: one to four axes of at least one pair each")
+    if 2 * sum(sections) > D or sum(sections) > 256:
+        raise ValueError(f"sections {sections} turn {2 * sum(sections)} dims, the head has {D} (at most 256 pairs)")
+    if pos.dtype not in _POS_TYPES:
+        raise TypeError(f"positions are int32, int64 or float32, not {pos.dtype}")
+    if tuple(pos.shape) not in ((N, len(sections)), (B, N, len(sections))):
+        raise ValueError(f"pos {tuple(pos.shape)} must be [{N}, {len(sections)}] or [{B}, {N}, {len(sections)}]")
+    bases = tuple(float(b) for b in base) if isinstance(base, (tuple, list)) else (float(base),) * len(sections)
+    if len(bases) != len(sections) or not all(1.0 < b < float("inf") for b in bases):
+        raise ValueError(f"base {base}: one number above 1, or one per axis")
+    if shared_ladder and len(set(bases)) > 1:
+        raise ValueError("a shared ladder has one base")
+    log2_base = tuple(math.log2(b) for b in bases)
+    _same_device(q, k, pos)
+    xs = [t for t in (q, k) if t is not None]
+    if inplace:
+        if _builds_graph(q, k):
+            raise RuntimeError("rope_axes(inplace=True) is for tensors outside of autograd")
+        for t in xs:
+            if t.dim() != 4 or (t.stride(3) != 1 and D > 1):
+                raise ValueError("inplace needs [batch, tokens, heads, head dim] with unit stride over the head dim")
+            if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                raise ValueError("inplace on a broadcast tensor would turn the same memory several times")
+        if k is not None and q.data_ptr() == k.data_ptr() and q.numel():
+            raise ValueError("inplace needs q and k apart")
+        _need_gpu(q, k, pos)
+        _rope_launch(xs, xs, pos, sections, log2_base, interleaved, shared_ladder, False)
+        for t in xs:
+            torch.autograd.graph.increment_version(t)
+        return (q, k) if k is not None else q
+    _need_gpu(q, k, pos)
+    if _builds_graph(q, k):
+        return RopeAxesFn.apply(q, k, pos, sections, log2_base, interleaved, shared_ladder)
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+    _rope_launch(xs, outs, pos, sections, log2_base, interleaved, shared_ladder, False)
+    return tuple(outs) if k is not None else outs[0]
+
+
+def _xattn_args(q, k, v, o, kv_len, key_mask, scale, lse):
+    a = _XattnArgs()
+    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
+    a.qs[:] = _s3(q)
+    a.ks[:] = _s3(k)
+    a.vs[:] = _s3(v)
+    if kv_len is not None:
+        a.kv_len, a.kv_len_i64 = kv_len.data_ptr(), kv_len.dtype == torch.int64
+    if key_mask is not None:
+        a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    a.dt = _dt(q)
+    a.B, a.Nq, a.Hq, a.D = q.shape
+    a.Nk, a.Hk = k.shape[1], k.shape[2]
+    a.scale = scale
+    return a
+
+
+def _xattn_fwd(q, k, v, kv_len, key_mask, scale, keep_lse):
+    B, Nq, Hq, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    o = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq * Nq), dtype=torch.float32, device=q.device) if keep_lse else None
+    a = _xattn_args(q, k, v, o, kv_len, key_mask, scale, lse)
+    with _on_device(q):
+        n = lib.vitmi_cross_attn_fwd_workspace_bytes(a.dt, B, Nq, Nk, Hq, Hk, D)
+        ws = _ws(n, q.device) if n else None
+        check(lib.vitmi_cross_attn_fwd(_ct.addressof(a), _p(ws), _stream()), "vitmi_cross_attn_fwd")
+    return o, lse
+
+
+class CrossAttnFn(torch.autograd.Function):
+    """The node behind cross_attn: keeps q, k, v, the output and a log-sum-exp per row; probabilities are formed again."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, kv_len, key_mask, scale):
+        o, lse = _xattn_fwd(q, k, v, kv_len, key_mask, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, kv_len, key_mask)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse, kv_len, key_mask = ctx.saved_tensors
+        if _PS2 is not None:                # a replay forms no input gradients
+            return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None, None, None)
+        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_kv else None
+        if q.numel() == 0 or k.numel() == 0:
+            for t in (dq, dk, dv):
+                if t is not None:
+                    t.zero_()
+            return dq, dk, dv, None, None, None
+        do = _heads4("gradient", do)
+        a = _xattn_args(q, k, v, o, kv_len, key_mask, ctx.scale, lse)
+        a.dout = do.data_ptr()
+        a.dos[:] = _s3(do)
+        a.dq, a.dk, a.dv = _p(dq), _p(dk), _p(dv)
+        with _on_device(q):
+            ws = _ws(lib.vitmi_cross_attn_bwd_workspace_bytes(a.dt, a.B, a.Nq, a.Nk, a.Hq, a.Hk, a.D), q.device)
+            check(lib.vitmi_cross_attn_bwd(_ct.addressof(a), _p(ws), _stream()), "vitmi_cross_attn_bwd")
+        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
+
+
+def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
+    """softmax(scale q k^T) v of queries [B, Nq, Hq, D] over the states [B, Nk, Hk, D] of another sequence, [B, Nq, Hq, D];
+    differentiable in q, k and v.  Hq is a multiple of Hk (query heads share key heads in order); D up to 128; scale
+    defaults to D^-0.5.  q, k and v may be strided or broadcast views.
+
+    Which keys count: kv_len [B] (int32 / int64), the first kv_len[b] of sample b (values outside 0 .. Nk are taken as
+    the nearer end), or key_mask [B, Nk] bool, True = attend, or all.  The rows of other keys may hold anything, their
+    gradients are zero.  A sample without a key to attend to gives zeros, and zero gradients."""
+    q, k, v = _heads4("q", q), _heads4("k", k), _heads4("v", v)
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    _dt(q)
+    B, Nq, Hq, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [{B}, Nk, Hk, {D}] for q {tuple(q.shape)}")
+    if Hk == 0 or Hq == 0 or D == 0 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads cannot share {Hk} key heads of {D}")
+    if D > 128:
+        raise ValueError(f"heads of {D} exceed the supported width 128")
+    if kv_len is not None:
+        if key_mask is not None:
+            raise ValueError("give key lengths or a key mask, not both")
+        if kv_len.dtype not in (torch.int32, torch.int64) or tuple(kv_len.shape) != (B,):
+            raise ValueError(f"kv_len must be int32 or int64 [{B}], got {kv_len.dtype} {tuple(kv_len.shape)}")
+        kv_len = kv_len.contiguous()
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, Nk):
+            raise ValueError(f"key_mask must be bool [{B}, {Nk}], got {key_mask.dtype} {tuple(key_mask.shape)}")
+        if Nk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale {scale} must be positive and finite")
+    _same_device(q, k, v, kv_len, key_mask)
+    _need_gpu(q, k, v, kv_len, key_mask)
+    if _builds_graph(q, k, v):
+        return CrossAttnFn.apply(q, k, v, kv_len, key_mask, scale)
+    return _xattn_fwd(q, k, v, kv_len, key_mask, scale, False)[0]
+
+
+_NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+
+
+def _ngr_args(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, stats):
+    res_scale, post, pre, eps = meta
+    a = _NgrArgs()
+    B, N, D = x.shape
+    a.x, a.u = x.data_ptr(), u.data_ptr()
+    a.xs[:] = x.stride()[:2]
+    a.us[:] = u.stride()[:2]
+    if gate is not None:
+        a.gate, a.gate_dt = gate.data_ptr(), _dt(gate)
+        a.gate_stride = gate.stride(0) if gate.dim() == 2 else 0
+    a.branch_scale, a.post_w, a.post_b, a.pre_w, a.pre_b = (_p(branch_scale), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b))
+    a.stats = _p(stats)
+    a.dt_x, a.dt_u, a.B, a.N, a.D, a.post, a.pre = _dt(x), _dt(u), B, N, D, _NORM_KINDS[post], _NORM_KINDS[pre]
+    a.res_scale, a.eps = res_scale, eps
+    return a
+
+
+def _ngr_fwd(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, keep):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = torch.empty(x.shape, dtype=u.dtype, device=x.device) if meta[2] is not None else None
+    stats = torch.empty((4, x.shape[0] * x.shape[1]), dtype=torch.float32, device=x.device) if keep else None
+    a = _ngr_args(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, stats)
+    a.y, a.h = y.data_ptr(), _p(h)
+    with _on_device(x):
+        check(lib.vitmi_norm_gate_residual_fwd(_ct.addressof(a), _stream()), "vitmi_norm_gate_residual_fwd")
+    return y, h, stats
+
+
+class NormGateResidualFn(torch.autograd.Function):
+    """The node behind norm_gate_residual: keeps its inputs and four fp32 statistics a row."""
+
+    @staticmethod
+    def forward(ctx, x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta):
+        y, h, stats = _ngr_fwd(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, True)
+        ctx.save_for_backward(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, stats)
+        ctx.meta = meta
+        ctx.set_materialize_grads(False)
+        return (y, h) if h is not None else y
+
+    @staticmethod
+    def backward(ctx, dy, dh=None):
+        x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if (_PS is not None or _PS2 is not None) and any(need[i] for i in (2, 4, 5, 6, 7)):
+            raise NotImplementedError("per-sample norms of norm_gate_residual's gate and norm parameters")
+        if _PS2 is not None:                # a replay forms no input gradients
+            return (_no_grad_like(x.shape, x.dtype, x.device), _no_grad_like(u.shape, u.dtype, u.device)) + (None,) * 7
+        if dy is None and dh is None:
+            return (None,) * 9
+
+        def new(i, t, dtype=None):
+            return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device) if need[i] else None
+        dx, du, dgate = new(0, x), new(1, u), new(2, gate)
+        dw = [new(i, t) for i, t in ((4, post_w), (5, post_b), (6, pre_w), (7, pre_b))]
+        grads = [dx, du, dgate, None, *dw, None]
+        if x.numel() == 0:
+            for t in grads:
+                if t is not None:
+                    t.zero_()
+            return tuple(grads)
+        a = _ngr_args(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, ctx.meta, stats)
+        dy = dy.contiguous() if dy is not None else None
+        dh = dh.contiguous() if dh is not None else None
+        a.dy, a.dh, a.dx, a.du, a.dgate = _p(dy), _p(dh), _p(dx), _p(du), _p(dgate)
+        a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_p(t) for t in dw)
+        with _on_device(x):
+            ws = None
+            if dgate is not None or any(t is not None for t in dw):
+                ws = _ws(lib.vitmi_norm_gate_residual_bwd_workspace_bytes(a.B, a.N, a.D, gate is not None and gate.dim() == 2),
+                         x.device)
+            check(lib.vitmi_norm_gate_residual_bwd(_ct.addressof(a), _p(ws), _stream()), "vitmi_norm_gate_residual_bwd")
+        return tuple(grads)
+
+
+def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=None, post_weight=None, post_bias=None,
+                       pre=None, pre_weight=None, pre_bias=None, eps=1e-6):
+    """The step between two sub-blocks in one pass:  y = res_scale * x + branch_scale[b] * gate * post(u),  h = pre(y).
+    Returns (y, h); h is None without pre.  Differentiable in x, u, gate and the norms' parameters.
+
+    x, u [B, N, D] (views with unit stride over D are read in place): the residual stream and the branch's output, both
+    bf16 or both fp32, or an fp32 stream with bf16 branches; y has x's dtype, h has u's.  gate: layer scale [D], or a gate
+    per sample [B, D] (fp32 or bf16).  branch_scale [B] fp32, not differentiated: stochastic depth; a sample at 0 is
+    y = res_scale * x, whatever u holds.  post, pre: "layer" (LayerNorm), "rms" or None, with optional fp32 weight and
+    (LayerNorm or RMS) bias [D].  D up to 8192."""
+    if x.dim() != 3 or x.shape != u.shape:
+        raise ValueError(f"x and u must be [batch, tokens, dim] alike, got {tuple(x.shape)} and {tuple(u.shape)}")
+    B, N, D = x.shape
+    if _dt(x) == BF16 and _dt(u) == F32:
+        raise TypeError("a bf16 residual stream takes bf16 branches")
+    if not 1 <= D <= 8192:
+        raise ValueError(f"rows of {D} are outside 1 .. 8192")
+    for name, kind, w, b in (("post", post, post_weight, post_bias), ("pre", pre, pre_weight, pre_bias)):
+        if kind not in _NORM_KINDS:
+            raise ValueError(f'{name}={kind!r}: "layer", "rms" or None')
+        for what, t in (("weight", w), ("bias", b)):
+            if t is None:
+                continue
+            if kind is None:
+                raise ValueError(f"{name}_{what} without {name}")
+            if tuple(t.shape) != (D,) or t.dtype != torch.float32:
+                raise ValueError(f"{name}_{what} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
+    if gate is not None:
+        _dt(gate)
+        if tuple(gate.shape) not in ((D,), (B, D)):
+            raise ValueError(f"gate {tuple(gate.shape)} must be [{D}] or [{B}, {D}]")
+        if gate.stride(-1) != 1 or (gate.dim() == 2 and gate.stride(0) < D):
+            gate = gate.contiguous()
+    if branch_scale is not None:
+        if branch_scale.dtype != torch.float32 or tuple(branch_scale.shape) != (B,):
+            raise ValueError(f"branch_scale must be float32 [{B}], got {branch_scale.dtype} {tuple(branch_scale.shape)}")
+        if branch_scale.requires_grad:
+            raise ValueError("branch_scale is not differentiated")
+        branch_scale = branch_scale.contiguous()
+    x, u = (t if t.stride(2) == 1 or D == 1 else t.contiguous() for t in (x, u))
+    post_weight, post_bias, pre_weight, pre_bias = (t if t is None or t.is_contiguous() else t.contiguous()
+                                                    for t in (post_weight, post_bias, pre_weight, pre_bias))
+    meta = (float(res_scale), post, pre, float(eps))
+    _same_device(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias)
+    _need_gpu(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias)
+    if _builds_graph(x, u, gate, post_weight, post_bias, pre_weight, pre_bias):
+        res = NormGateResidualFn.apply(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias, meta)
+        return res if pre is not None else (res, None)
+    y, h, _ = _ngr_fwd(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias, meta, False)
+    return y, h
