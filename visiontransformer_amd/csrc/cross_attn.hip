@@ -255,7 +255,14 @@ __device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typen
     constexpr int KB = KT / 32;
     f32x16 s[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) scores<T, DP>(s[kb], kimg, 32 * kb, qf, lane);
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+    for (int cc = 0; cc < DP / Mx<T>::KD; ++cc)       // the blocks' accumulation chains take turns
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+            mma(s[kb], row_frag<T, DP>(kimg, 32 * kb + key_of_row<T>(lane & 31), cc, lane >> 5), qf[cc]);
     if (mask != full_mask<KT>()) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) mask_scores<T>(s[kb], (unsigned)(mask >> (32 * kb)), lane >> 5);
@@ -352,7 +359,7 @@ __device__ __forceinline__ void split_range(int tiles, int splits, int split, in
 }
 
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(XA_THREADS) void xattn_fwd_kernel(XaArgs a) {
+__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_kernel(XaArgs a) {
     constexpr int KT = Mx<T>::KT, IMG = KT * ld_of<T, DP>();
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);        // K, V, K, V
@@ -520,7 +527,8 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     }
 }
 
-// joins the key splits of a forward launch, one wave a row
+// joins the key splits (at most 64) of a forward launch, one wave a row: lane s holds split s's maximum and sum, the partial rows
+// are then added in split order, eight loads in flight
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long rows) {
     const int lane = threadIdx.x & 63;
@@ -529,30 +537,43 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long row
     const int r = (int)(st % a.R);
     const long long bh = st / a.R;
     const int hk = (int)(bh % a.Hk), b = (int)(bh / a.Hk);
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + st;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, ml[s * rows].x);
+    float2 p = make_float2(-INFINITY, 0.f);
+    if (lane < a.splits) p = reinterpret_cast<const float2*>(a.part_ml)[lane * rows + st];
+    const float m = wave_max(p.x);
+    // a share without an allowed key counts for nothing, whatever its partial row holds
+    const float w = p.y == 0.f ? 0.f : (p.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p.x - m));
+    const float l = wave_sum(p.y == 0.f ? 0.f : p.y * w);
     const long long row = dense_row(a, b, hk, r);
+    const bool in0 = lane < a.D, in1 = lane + 64 < a.D;
     float o0 = 0.f, o1 = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 p = ml[s * rows];
-        if (p.y == 0.f) continue;                    // a share without an allowed key
-        const float w = p.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p.x - m);
-        l = fmaf(p.y, w, l);
-        const float* po = a.part_o + s * a.n_q + row;
-        if (lane < a.D) o0 = fmaf(po[lane], w, o0);
-        if (lane + 64 < a.D) o1 = fmaf(po[lane + 64], w, o1);
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {
+        float x0[8], x1[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float* po = a.part_o + (s0 + i) * a.n_q + row + lane;
+            const bool on = s0 + i < a.splits;
+            x0[i] = on && in0 ? po[0] : 0.f;
+            x1[i] = on && in1 ? po[64] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float wi = __shfl(w, (s0 + i) & 63, 64);
+            if (s0 + i < a.splits && wi != 0.f) {
+                o0 = fmaf(x0[i], wi, o0);
+                o1 = fmaf(x1[i], wi, o1);
+            }
+        }
     }
     const float f = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     T* op = (T*)a.o + row;
-    if (lane < a.D) op[lane] = from_f32<T>(o0 * f);
-    if (lane + 64 < a.D) op[lane + 64] = from_f32<T>(o1 * f);
+    if (in0) op[lane] = from_f32<T>(o0 * f);
+    if (in1) op[lane + 64] = from_f32<T>(o1 * f);
     if (a.lse && lane == 0) a.lse[st] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(XA_THREADS) void xattn_dq_kernel(XaArgs a) {
+__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_kernel(XaArgs a) {
     constexpr int KT = Mx<T>::KT, IMG = KT * ld_of<T, DP>(), NF = DP / Mx<T>::KD;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);
@@ -639,7 +660,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_dq_kernel(XaArgs a) {
 
 // dk and dv: four waves of 32 keys over the row tiles of the whole group
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(XA_THREADS) void xattn_dkv_kernel(XaArgs a) {
+__global__ __launch_bounds__(XA_THREADS, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xattn_dkv_kernel(XaArgs a) {
     constexpr int QT = Mx<T>::KT, IMG = QT * ld_of<T, DP>(), NF = DP / Mx<T>::KD;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);                           // Q, dO, Q, dO

@@ -46,19 +46,26 @@ struct alignas(sizeof(T) * V) NVec {
     T v[V];
 };
 
-// pair sums over the 64 lanes of a wave
-__device__ __forceinline__ void wave_sum2(float& a, float& b) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        a += __shfl_xor(a, o, 64);
-        b += __shfl_xor(b, o, 64);
-    }
+// sum over the 64 lanes of a wave, the same value in every lane: shifts within the rows of 16, two broadcasts between
+// rows, all on the vector unit (a shuffle would go through LDS six times)
+__device__ __forceinline__ float lanes_sum(float v) {
+#define NG_STEP(ctrl, rows) \
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, true))
+    NG_STEP(0x111, 0xf);   // row_shr 1, 2, 4, 8
+    NG_STEP(0x112, 0xf);
+    NG_STEP(0x114, 0xf);
+    NG_STEP(0x118, 0xf);
+    NG_STEP(0x142, 0xa);   // row_bcast 15, 31
+    NG_STEP(0x143, 0xc);
+#undef NG_STEP
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // pair sums over the WPR waves that share a row; `red` alternates between two halves so that one barrier a call is enough
 template <int WPR>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& flip) {
-    wave_sum2(a, b);
+    a = lanes_sum(a);
+    b = lanes_sum(b);
     if (WPR > 1) {
         float* r = red + flip * 2 * WPR;
         flip ^= 1;
@@ -75,6 +82,16 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& fl
             b += r[2 * i + 1];
         }
     }
+}
+
+template <int WPR>
+__device__ __forceinline__ float row_sum(float a, float* red, int& flip) {
+    if (WPR > 1) {
+        float z = 0.f;
+        row_sum2<WPR>(a, z, red, flip);
+        return a;
+    }
+    return lanes_sum(a);
 }
 
 template <int V>
@@ -160,15 +177,14 @@ __device__ __forceinline__ void row_stats(const NgArgs& a, const float (&v)[ITER
     const int t = WPR > 1 ? (int)threadIdx.x : (int)(threadIdx.x & 63);
     mu = 0.f;
     if (kind == NG_LAYER) {
-        float s = 0.f, z = 0.f;
+        float s = 0.f;
 #pragma unroll
         for (int it = 0; it < ITERS; ++it)
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v[it][j];
-        row_sum2<WPR>(s, z, red, flip);
-        mu = s / (float)a.D;
+        mu = row_sum<WPR>(s, red, flip) / (float)a.D;
     }
-    float q = 0.f, z = 0.f;
+    float q = 0.f;
 #pragma unroll
     for (int it = 0; it < ITERS; ++it) {
         if ((it * 64 * WPR + t) * V < a.D) {
@@ -179,8 +195,7 @@ __device__ __forceinline__ void row_stats(const NgArgs& a, const float (&v)[ITER
             }
         }
     }
-    row_sum2<WPR>(q, z, red, flip);
-    r = rsqrtf(q / (float)a.D + a.eps);
+    r = rsqrtf(row_sum<WPR>(q, red, flip) / (float)a.D + a.eps);
 }
 
 template <typename TX, typename TU, int V, int ITERS, int WPR>
@@ -288,46 +303,58 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void ngr_bwd_kernel(NgAr
     const long long r0 = seg * per + chunk * per / a.chunks, r1 = seg * per + (chunk + 1) * per / a.chunks;
     load_gate<V, ITERS, WPR>(a, seg, gw, gb);
     const float inv_d = 1.f / (float)a.D;
-    for (long long row = r0 + wave; row < r1; row += RPB) {
+    const bool pre = a.pre != NG_NONE && a.dh;
+    // the next row's loads are in flight behind a row's arithmetic where their registers (dy, x, dh, u as stored) leave room
+    constexpr bool AHEAD = ITERS * V * (sizeof(TX) + sizeof(TU)) / 2 <= 40;
+    NVec<TX, V> nx[ITERS], ndy[ITERS];
+    NVec<TU, V> nu[ITERS], ndh[ITERS];
+    float ns = 1.f, nmu = 0.f, nru = 0.f, nmy = 0.f, nry = 0.f;
+    auto fetch = [&](long long row) {
         const long long b = row / a.N, n = row - b * a.N;
-        const float s = a.branch_scale ? a.branch_scale[b] : 1.f;
-        const bool live = s != 0.f;
-        NVec<TX, V> nx[ITERS], ndy[ITERS];
-        NVec<TU, V> nu[ITERS], ndh[ITERS];
-        const bool pre = a.pre != NG_NONE && a.dh;
+        ns = a.branch_scale ? a.branch_scale[b] : 1.f;
         fetch_row<TX, V, ITERS, WPR>(a.dy ? (const TX*)a.dy + row * a.D : (const TX*)nullptr, a.D, ndy);
-        fetch_row<TU, V, ITERS, WPR>(live ? (const TU*)a.u + b * a.us[0] + n * a.us[1] : (const TU*)nullptr, a.D, nu);
         fetch_row<TU, V, ITERS, WPR>(pre ? (const TU*)a.dh + row * a.D : (const TU*)nullptr, a.D, ndh);
         fetch_row<TX, V, ITERS, WPR>(pre ? (const TX*)a.x + b * a.xs[0] + n * a.xs[1] : (const TX*)nullptr, a.D, nx);
-        const float mu = a.stats[row], ru = a.stats[a.rows + row];
-        const float my = a.stats[2 * a.rows + row], ry = a.stats[3 * a.rows + row];
-        float tv[ITERS][V], uh[ITERS][V];
+        nmu = a.stats[row];
+        nru = a.stats[a.rows + row];
+        nmy = a.stats[2 * a.rows + row];
+        nry = a.stats[3 * a.rows + row];
+        fetch_row<TU, V, ITERS, WPR>(ns != 0.f ? (const TU*)a.u + b * a.us[0] + n * a.us[1] : (const TU*)nullptr, a.D, nu);
+    };
+    if (AHEAD && r0 + wave < r1) fetch(r0 + wave);
+    for (long long row = r0 + wave; row < r1; row += RPB) {
+        if (!AHEAD) fetch(row);
+        const float s = ns, mu = nmu, ru = nru, my = nmy, ry = nry;
+        const bool live = s != 0.f;
+        float tv[ITERS][V], uh[ITERS][V], yh[ITERS][V];
+        NVec<TU, V> dhv[ITERS];
 #pragma unroll
-        for (int it = 0; it < ITERS; ++it)
+        for (int it = 0; it < ITERS; ++it) {
+            const bool in = (it * 64 * WPR + t) * V < a.D;
+            dhv[it] = ndh[it];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 tv[it][j] = to_f32(ndy[it].v[j]);
                 uh[it][j] = (to_f32(nu[it].v[j]) - mu) * ru;
+                const float ax = a.res_scale * to_f32(nx[it].v[j]);
+                const float yv = live ? fmaf(s, fmaf(uh[it][j], gw[it][j], gb[it][j]), ax) : ax;
+                yh[it][j] = in ? (yv - my) * ry : 0.f;
             }
+        }
+        if (AHEAD && row + RPB < r1) fetch(row + RPB);
         if (pre) {
-            float yh[ITERS][V];
             float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-            for (int it = 0; it < ITERS; ++it) {
-                const bool in = (it * 64 * WPR + t) * V < a.D;
+            for (int it = 0; it < ITERS; ++it)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float dh = to_f32(ndh[it].v[j]);
-                    const float ax = a.res_scale * to_f32(nx[it].v[j]);
-                    const float yv = live ? fmaf(s, fmaf(uh[it][j], gw[it][j], gb[it][j]), ax) : ax;
-                    yh[it][j] = in ? (yv - my) * ry : 0.f;
+                    const float dh = to_f32(dhv[it].v[j]);
                     sC[it][j] = fmaf(dh, yh[it][j], sC[it][j]);
                     sE[it][j] += dh;
                     const float g = dh * pw[it][j];
                     c1 += g;
                     c2 = fmaf(g, yh[it][j], c2);
                 }
-            }
             row_sum2<WPR>(c1, c2, red, flip);
             c1 = a.pre == NG_LAYER ? c1 * inv_d : 0.f;
             c2 *= inv_d;
@@ -335,7 +362,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void ngr_bwd_kernel(NgAr
             for (int it = 0; it < ITERS; ++it)
 #pragma unroll
                 for (int j = 0; j < V; ++j)
-                    tv[it][j] = fmaf(ry, fmaf(to_f32(ndh[it].v[j]), pw[it][j], -c1) - yh[it][j] * c2, tv[it][j]);
+                    tv[it][j] = fmaf(ry, fmaf(to_f32(dhv[it].v[j]), pw[it][j], -c1) - yh[it][j] * c2, tv[it][j]);
         }
         if (a.dx) {
             TX* dr = (TX*)a.dx + row * a.D;
@@ -436,76 +463,78 @@ __device__ __forceinline__ float gate_at(const NgFinal& f, int seg, int c) {
     return f.gate_f32 ? ((const float*)f.gate)[o] : to_f32(((const bf16_t*)f.gate)[o]);
 }
 
-// 64 columns x 16 row groups a workgroup, partials added in a fixed order; segments one after the other
-__global__ __launch_bounds__(1024) void ngr_final_kernel(NgFinal f) {
-    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;
-    __shared__ float red[16][4][64];
-    float tw = 0.f, tb = 0.f, tc = 0.f, te = 0.f;
-    if (f.gate_stride == 0) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        if (c < f.D)
-            for (int k = grp; k < f.chunks; k += 16)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) s[q] += f.partial[((long long)k * 4 + q) * f.D + c];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) red[grp][q][lane] = s[q];
-        __syncthreads();
-        if (grp == 0 && c < f.D) {
-            for (int g = 0; g < 16; ++g) {
-                tw += red[g][0][lane];
-                tb += red[g][1][lane];
-                tc += red[g][2][lane];
-                te += red[g][3][lane];
+// NF_COLS columns x NF_GROUPS row groups a workgroup; blockIdx.y = 0 reduces the pair (A, B), 1 the pair (C, E).  Partials
+// are added in a fixed order.  Few columns a workgroup, because a row of 768 would otherwise occupy 12 of them.
+constexpr int NF_COLS = 16, NF_GROUPS = 64;
+
+__device__ __forceinline__ void final_pair(float& p, float& q, float (*red)[2][NF_COLS], int col, int grp) {
+    red[grp][0][col] = p;
+    red[grp][1][col] = q;
+    __syncthreads();
+    p = q = 0.f;
+    if (grp == 0)
+        for (int g = 0; g < NF_GROUPS; ++g) {
+            p += red[g][0][col];
+            q += red[g][1][col];
+        }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(NF_COLS* NF_GROUPS) void ngr_final_kernel(NgFinal f) {
+    const int col = threadIdx.x % NF_COLS, grp = threadIdx.x / NF_COLS;
+    const int c = blockIdx.x * NF_COLS + col;
+    const bool in = c < f.D, branch = blockIdx.y == 0;
+    __shared__ float red[NF_GROUPS][2][NF_COLS];
+    const float* part = f.partial + (branch ? 0 : 2ll * f.D) + c;
+    auto add = [&](long long k, float& p, float& q) {
+        p += part[k * 4 * f.D];
+        q += part[k * 4 * f.D + f.D];
+    };
+    auto gate_grad = [&](int seg, float p, float q) {
+        if (!f.dgate) return;
+        const float d = (f.post_w ? f.post_w[c] : 1.f) * p + (f.post_b ? f.post_b[c] * q : 0.f);
+        const long long o = (long long)seg * f.D + c;
+        if (f.gate_f32) ((float*)f.dgate)[o] = d;
+        else ((bf16_t*)f.dgate)[o] = (bf16_t)d;
+    };
+    float tp = 0.f, tq = 0.f;
+    if (!branch || f.chunks >= NF_GROUPS) {
+        // a sum over everything, or one segment after the other with the groups on its chunks
+        const int segs = branch ? f.segs : 1;
+        const long long n = branch ? f.chunks : (long long)f.segs * f.chunks;
+        for (int seg = 0; seg < segs; ++seg) {
+            float p = 0.f, q = 0.f;
+            if (in)
+                for (long long k = grp; k < n; k += NF_GROUPS) add(seg * n + k, p, q);
+            final_pair(p, q, red, col, grp);
+            if (grp == 0 && in) {
+                if (branch) {
+                    gate_grad(seg, p, q);
+                    const float g = gate_at(f, seg, c);
+                    p *= g;
+                    q *= g;
+                }
+                tp += p;
+                tq += q;
             }
-            const float g = gate_at(f, 0, c);
-            if (f.dgate) {
-                const float d = (f.post_w ? f.post_w[c] : 1.f) * tw + (f.post_b ? f.post_b[c] * tb : 0.f);
-                if (f.gate_f32) ((float*)f.dgate)[c] = d;
-                else ((bf16_t*)f.dgate)[c] = (bf16_t)d;
-            }
-            tw *= g;
-            tb *= g;
         }
     } else {
-        // a gate per sample: a row group takes samples grp, grp + 16, .., each over its chunks
-        if (c < f.D)
-            for (int seg = grp; seg < f.segs; seg += 16) {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int k = 0; k < f.chunks; ++k)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) s[q] += f.partial[(((long long)seg * f.chunks + k) * 4 + q) * f.D + c];
+        // many segments of few chunks: a group takes whole segments
+        if (in)
+            for (int seg = grp; seg < f.segs; seg += NF_GROUPS) {
+                float p = 0.f, q = 0.f;
+                for (int k = 0; k < f.chunks; ++k) add((long long)seg * f.chunks + k, p, q);
+                gate_grad(seg, p, q);
                 const float g = gate_at(f, seg, c);
-                if (f.dgate) {
-                    const float d = (f.post_w ? f.post_w[c] : 1.f) * s[0] + (f.post_b ? f.post_b[c] * s[1] : 0.f);
-                    if (f.gate_f32) ((float*)f.dgate)[(long long)seg * f.D + c] = d;
-                    else ((bf16_t*)f.dgate)[(long long)seg * f.D + c] = (bf16_t)d;
-                }
-                tw = fmaf(g, s[0], tw);
-                tb = fmaf(g, s[1], tb);
-                tc += s[2];
-                te += s[3];
+                tp = fmaf(g, p, tp);
+                tq = fmaf(g, q, tq);
             }
-        red[grp][0][lane] = tw;
-        red[grp][1][lane] = tb;
-        red[grp][2][lane] = tc;
-        red[grp][3][lane] = te;
-        __syncthreads();
-        if (grp == 0) {
-            tw = tb = tc = te = 0.f;
-            for (int g = 0; g < 16; ++g) {
-                tw += red[g][0][lane];
-                tb += red[g][1][lane];
-                tc += red[g][2][lane];
-                te += red[g][3][lane];
-            }
-        }
+        final_pair(tp, tq, red, col, grp);
     }
-    if (grp == 0 && c < f.D) {
-        if (f.dpost_w) f.dpost_w[c] = tw;
-        if (f.dpost_b) f.dpost_b[c] = tb;
-        if (f.dpre_w) f.dpre_w[c] = tc;
-        if (f.dpre_b) f.dpre_b[c] = te;
+    if (grp == 0 && in) {
+        float *o0 = branch ? f.dpost_w : f.dpre_w, *o1 = branch ? f.dpost_b : f.dpre_b;
+        if (o0) o0[c] = tp;
+        if (o1) o1[c] = tq;
     }
 }
 
@@ -528,7 +557,7 @@ bool ng_plan(int D, bool vec, NgPlan* p) {
     return false;
 }
 
-// partial-sum rows of the backward pass: two workgroups a compute unit, spread over the samples where the gate is per sample
+// partial-sum rows of the backward pass: two workgroups of four waves a compute unit (one of eight), spread over the samples where the gate is per sample
 int ng_chunks(bool per_sample, int B, int N, int wpr) {
     const long long rows = (long long)B * N;
     const int rpb = wpr == 1 ? 4 : 1;
@@ -689,7 +718,7 @@ extern "C" int vitmi_norm_gate_residual_bwd(const vitmi_ngr_args* g, void* works
     if (sums) {
         NgFinal f = {a.partial, a.gate, a.gate_f32, a.gate_stride, a.post_w, a.post_b, g->dgate, g->dpost_w, g->dpost_b,
                      g->dpre_w, g->dpre_b, segs, a.chunks, g->D};
-        hipLaunchKernelGGL(ngr_final_kernel, dim3(ceil_div(g->D, 64)), dim3(1024), 0, s, f);
+        hipLaunchKernelGGL(ngr_final_kernel, dim3(ceil_div(g->D, NF_COLS), 2), dim3(NF_COLS * NF_GROUPS), 0, s, f);
         VITMI_LAUNCH_CHECK(who);
     }
     return VITMI_OK;

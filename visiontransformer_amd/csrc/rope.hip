@@ -30,7 +30,9 @@ struct RopeArgs {
     long long ps[3];          // batch, token, axis strides
     double log2_base[4];
     int first_pair[5];        // first pair of each axis; [axes] = P
-    int axes, pos_type, P, DH, N, tile, tiles;
+    int axes, pos_type, P, DH, B, N, tile, tiles;
+    int group;                // samples a workgroup takes with one set of angles (positions shared by the batch)
+    unsigned div_tok, div_head;
     int units_tok, units_0;   // units per token, of which the first tensor's
     int units_head, units_rot;
     int copy_rest;            // the pass-through dims are copied (not in place)
@@ -42,13 +44,20 @@ struct alignas(sizeof(T) * V) RVec {
     T v[V];
 };
 
-template <typename T, int V>
+// how a unit of V pairs lies in memory: two vectors of V elements P apart; one vector of 2V (interleaved); two single
+// elements side by side (interleaved where no two-element vector fits: odd widths or strides)
+enum { ROPE_HALVES = 0, ROPE_INTER = 1, ROPE_INTER_SCALAR = 2 };
+
+template <typename T, int V, int MODE>
 struct RopeUnit {
-    RVec<T, V> a, b;
+    RVec<T, MODE == ROPE_INTER ? 2 * V : V> a, b;
     long long out;            // element offset of the unit's first vector in y
     int tok, pair;            // pair < 0: a pass-through unit (vector a only)
     int which;                // 0 / 1: tensor; -1: no unit
 };
+
+// n / d for n, d < 2^16 with m = ceil(2^32 / d): a division would cost more than the rest of a unit's addressing
+__device__ __forceinline__ int div16(int n, unsigned m) { return m ? (int)__umulhi((unsigned)n, m) : n; }
 
 __device__ __forceinline__ double rope_pos(const RopeArgs& a, long long off) {
     if (a.pos_type == VITMI_POS_I64) return (double)((const long long*)a.pos)[off];
@@ -67,80 +76,62 @@ __device__ __forceinline__ float2 rope_cos_sin(double turns) {
     return (k & 2) ? make_float2(-c1, -s1) : make_float2(c1, s1);
 }
 
-template <typename T, int V, bool INTER>
-__device__ __forceinline__ void rope_fetch(const RopeArgs& a, RopeUnit<T, V>& r, int u, int total, int b, int n0) {
+template <typename T, int V, int MODE>
+__device__ __forceinline__ void rope_fetch(const RopeArgs& a, RopeUnit<T, V, MODE>& r, int u, int total, int b, int n0) {
     r.which = -1;
     if (u >= total) return;
-    const int tok = u / a.units_tok;
+    const int tok = div16(u, a.div_tok);
     int rem = u - tok * a.units_tok;
     const int w = rem >= a.units_0;
     if (w) rem -= a.units_0;
-    const int head = rem / a.units_head, c = rem - head * a.units_head;
+    const int head = div16(rem, a.div_head), c = rem - head * a.units_head;
     const RopeTensor& t = w ? a.t[1] : a.t[0];
+    constexpr int W = MODE == ROPE_INTER ? 2 * V : V;
     const bool rot = c < a.units_rot;
-    const int d = rot ? c * V * (INTER ? 2 : 1) : 2 * a.P + (c - a.units_rot) * V;
+    const int d = rot ? c * (MODE == ROPE_HALVES ? V : 2 * V) : 2 * a.P + (c - a.units_rot) * W;
     const T* x = (const T*)t.x + b * t.xs[0] + (n0 + tok) * t.xs[1] + head * t.xs[2] + d;
     r.out = b * t.ys[0] + (n0 + tok) * t.ys[1] + head * t.ys[2] + d;
     r.which = w;
     r.tok = tok;
     r.pair = rot ? c * V : -1;
-    r.a = *reinterpret_cast<const RVec<T, V>*>(x);
-    if (rot) r.b = *reinterpret_cast<const RVec<T, V>*>(x + (INTER ? V : a.P));
+    r.a = *reinterpret_cast<const RVec<T, W>*>(x);
+    if (MODE != ROPE_INTER && rot) r.b = *reinterpret_cast<const RVec<T, W>*>(x + (MODE == ROPE_HALVES ? a.P : 1));
 }
 
-template <typename T, int V, bool INTER>
-__device__ __forceinline__ void rope_finish(const RopeArgs& a, RopeUnit<T, V>& r, const float2* cs) {
+template <typename T, int V, int MODE>
+__device__ __forceinline__ void rope_finish(const RopeArgs& a, RopeUnit<T, V, MODE>& r, const float2* cs) {
     if (r.which < 0) return;
+    constexpr int W = MODE == ROPE_INTER ? 2 * V : V;
     T* y = (T*)(r.which ? a.t[1].y : a.t[0].y) + r.out;
-    if (r.pair < 0) {
-        *reinterpret_cast<RVec<T, V>*>(y) = r.a;
-        return;
-    }
-    const float2* w = cs + r.tok * a.P + r.pair;
-    if (INTER) {
-        float e[2 * V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            e[j] = to_f32(r.a.v[j]);
-            e[V + j] = to_f32(r.b.v[j]);
-        }
-        T o[2 * V];
+    if (r.pair >= 0) {
+        const float2* w = cs + r.tok * a.P + r.pair;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float2 t = w[j];
-            o[2 * j] = from_f32<T>(e[2 * j] * t.x - e[2 * j + 1] * t.y);
-            o[2 * j + 1] = from_f32<T>(e[2 * j + 1] * t.x + e[2 * j] * t.y);
+            T& e1 = MODE == ROPE_INTER ? r.a.v[2 * j] : r.a.v[j];
+            T& e2 = MODE == ROPE_INTER ? r.a.v[2 * j + 1] : r.b.v[j];
+            const float p = to_f32(e1), q = to_f32(e2);
+            e1 = from_f32<T>(p * t.x - q * t.y);
+            e2 = from_f32<T>(q * t.x + p * t.y);
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            r.a.v[j] = o[j];
-            r.b.v[j] = o[V + j];
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float2 t = w[j];
-            const float p = to_f32(r.a.v[j]), q = to_f32(r.b.v[j]);
-            r.a.v[j] = from_f32<T>(p * t.x - q * t.y);
-            r.b.v[j] = from_f32<T>(q * t.x + p * t.y);
-        }
+        if (MODE != ROPE_INTER) *reinterpret_cast<RVec<T, W>*>(y + (MODE == ROPE_HALVES ? a.P : 1)) = r.b;
     }
-    *reinterpret_cast<RVec<T, V>*>(y) = r.a;
-    *reinterpret_cast<RVec<T, V>*>(y + (INTER ? V : a.P)) = r.b;
+    *reinterpret_cast<RVec<T, W>*>(y) = r.a;
 }
 
-template <typename T, int V, bool INTER>
+template <typename T, int V, int MODE>
 __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeArgs a) {
     extern __shared__ double rope_lds[];
     double* freq = rope_lds;                                   // [P] turns per position step
     float2* cs = reinterpret_cast<float2*>(rope_lds + a.P);     // [tile][P]
-    const int b = blockIdx.x / a.tiles, n0 = (blockIdx.x - b * a.tiles) * a.tile;
+    const int grp = blockIdx.x / a.tiles, n0 = (blockIdx.x - grp * a.tiles) * a.tile;
+    const int b0 = grp * a.group, b1 = min(b0 + a.group, a.B);
     const int toks = min(a.tile, a.N - n0);
     const int total = toks * a.units_tok;
-    constexpr int K = 2;
-    RopeUnit<T, V> r[K];
+    constexpr int K = 3;
+    RopeUnit<T, V, MODE> r[K];
 #pragma unroll
-    for (int i = 0; i < K; ++i) rope_fetch<T, V, INTER>(a, r[i], (int)threadIdx.x + i * ROPE_THREADS, total, b, n0);
+    for (int i = 0; i < K; ++i) rope_fetch<T, V, MODE>(a, r[i], (int)threadIdx.x + i * ROPE_THREADS, total, b0, n0);
 
     if ((int)threadIdx.x < a.P) {
         const int p = threadIdx.x;
@@ -155,27 +146,37 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeArgs a) {
         const int tok = i / a.P, p = i - tok * a.P;
         int ax = 0;
         while (p >= a.first_pair[ax + 1]) ++ax;
-        float2 w = rope_cos_sin(rope_pos(a, b * a.ps[0] + (n0 + tok) * a.ps[1] + ax * a.ps[2]) * freq[p]);
+        float2 w = rope_cos_sin(rope_pos(a, b0 * a.ps[0] + (n0 + tok) * a.ps[1] + ax * a.ps[2]) * freq[p]);
         if (a.inverse) w.y = -w.y;
         cs[i] = w;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < K; ++i) rope_finish<T, V, INTER>(a, r[i], cs);
-    for (int u = (int)threadIdx.x + K * ROPE_THREADS; u < total; u += K * ROPE_THREADS) {
+    for (int i = 0; i < K; ++i) rope_finish<T, V, MODE>(a, r[i], cs);
+    for (int b = b0; b < b1; ++b)
+        for (int u = (int)threadIdx.x + (b == b0 ? K * ROPE_THREADS : 0); u < total; u += K * ROPE_THREADS) {
 #pragma unroll
-        for (int i = 0; i < K; ++i) rope_fetch<T, V, INTER>(a, r[i], u + i * ROPE_THREADS, total, b, n0);
+            for (int i = 0; i < K; ++i) rope_fetch<T, V, MODE>(a, r[i], u + i * ROPE_THREADS, total, b, n0);
 #pragma unroll
-        for (int i = 0; i < K; ++i) rope_finish<T, V, INTER>(a, r[i], cs);
-    }
+            for (int i = 0; i < K; ++i) rope_finish<T, V, MODE>(a, r[i], cs);
+        }
 }
 
-template <typename T, int V>
-void launch_rope(const RopeArgs& k, bool inter, unsigned blocks, size_t lds, hipStream_t s) {
-    if (inter)
-        hipLaunchKernelGGL((rope_kernel<T, V, true>), dim3(blocks), dim3(ROPE_THREADS), lds, s, k);
-    else
-        hipLaunchKernelGGL((rope_kernel<T, V, false>), dim3(blocks), dim3(ROPE_THREADS), lds, s, k);
+template <typename T>
+void launch_rope(const RopeArgs& k, int mode, int V, unsigned blocks, size_t lds, hipStream_t s) {
+#define ROPE_GO(v, m) hipLaunchKernelGGL((rope_kernel<T, v, m>), dim3(blocks), dim3(ROPE_THREADS), lds, s, k)
+    if (mode == ROPE_INTER_SCALAR) ROPE_GO(1, ROPE_INTER_SCALAR);
+    else if (mode == ROPE_INTER) {
+        if (V == 1) ROPE_GO(1, ROPE_INTER);
+        else if (V == 2) ROPE_GO(2, ROPE_INTER);
+        else if constexpr (sizeof(T) == 2) ROPE_GO(4, ROPE_INTER);
+    } else {
+        if (V == 1) ROPE_GO(1, ROPE_HALVES);
+        else if (V == 2) ROPE_GO(2, ROPE_HALVES);
+        else if (V == 4) ROPE_GO(4, ROPE_HALVES);
+        else if constexpr (sizeof(T) == 2) ROPE_GO(8, ROPE_HALVES);
+    }
+#undef ROPE_GO
 }
 
 }  // namespace
@@ -207,10 +208,11 @@ extern "C" int vitmi_rope_axes(const vitmi_rope_args* a, void* stream) {
 
     const int esz = a->dt == VITMI_F32 ? 4 : 2;
     const int nt = a->t[1].x ? 2 : 1;
-    // widest vector of V elements (16 bytes and below) that pairs, rest, strides and pointers are all multiples of
-    int V = a->dt == VITMI_F32 ? 4 : 8;
-    auto fits = [&](int v) {
-        if (P % v || (a->DH - 2 * P) % v) return false;
+    // V pairs a unit: the widest vectors (16 bytes and below) that pairs, rest, strides and pointers are multiples of
+    const bool inter = a->interleaved != 0;
+    auto fits = [&](int pairs) {
+        const int v = inter ? 2 * pairs : pairs;
+        if (P % pairs || (a->DH - 2 * P) % v) return false;
         for (int i = 0; i < nt; ++i) {
             const vitmi_rope_tensor& t = a->t[i];
             if ((reinterpret_cast<uintptr_t>(t.x) | reinterpret_cast<uintptr_t>(t.y)) % (v * esz)) return false;
@@ -219,8 +221,9 @@ extern "C" int vitmi_rope_axes(const vitmi_rope_args* a, void* stream) {
         }
         return true;
     };
-    if (V == 8 && !fits(8)) V = 4;
-    if (V == 4 && !fits(4)) V = 1;
+    int V = inter ? 8 / esz : 16 / esz;
+    while (V > 1 && !fits(V)) V >>= 1;
+    const int mode = !inter ? ROPE_HALVES : V == 1 && !fits(1) ? ROPE_INTER_SCALAR : ROPE_INTER;
     long long heads = 0;
     bool in_place = true;
     for (int i = 0; i < nt; ++i) {
@@ -245,29 +248,32 @@ extern "C" int vitmi_rope_axes(const vitmi_rope_args* a, void* stream) {
     k.shared = a->shared_ladder;
     k.inverse = a->inverse;
     k.units_rot = P / V;
-    k.units_head = k.units_rot + (in_place ? 0 : (a->DH - 2 * P) / V);
+    const int rest = (a->DH - 2 * P) / (mode == ROPE_INTER ? 2 * V : V);
+    k.units_head = k.units_rot + (in_place ? 0 : rest);
     const long long ut = heads * k.units_head;
-    VITMI_CHECK_ARG(ut * 8 < (1ll << 31), "vitmi_rope_axes: %lld heads of %d are beyond one call", heads, a->DH);
+    VITMI_CHECK_ARG(ut < 65536, "vitmi_rope_axes: %lld heads of %d are beyond one call", heads, a->DH);
     k.units_tok = (int)ut;
     k.units_0 = a->t[0].heads * k.units_head;
+    auto magic = [](int d) { return d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); };
+    k.div_tok = magic(k.units_tok);
+    k.div_head = magic(k.units_head);
     // tokens per workgroup: eight share one round of angles, fewer while that leaves compute units without work
     int tile = 8;
-    while (tile > 1 && (long long)a->B * ceil_div(a->N, tile) < 1024) tile >>= 1;
+    while (tile > 1 && ((long long)a->B * ceil_div(a->N, tile) < 1024 || tile * ut >= 65536)) tile >>= 1;
     k.tile = tile;
     k.tiles = ceil_div(a->N, tile);
-    const long long blocks = (long long)a->B * k.tiles;
+    // positions shared by the batch: a workgroup turns the same tokens of several samples by one set of angles, as long as
+    // four workgroups a compute unit remain
+    const bool same = a->pos_stride[0] == 0 || a->B == 1;
+    k.B = a->B;
+    k.group = same ? (int)std::max<long long>(1, std::min<long long>(a->B, (long long)a->B * k.tiles / 1024)) : 1;
+    const long long blocks = (long long)ceil_div(a->B, k.group) * k.tiles;
     VITMI_CHECK_ARG(blocks < (1ll << 32) / ROPE_THREADS, "vitmi_rope_axes: %lld tiles are beyond one launch", blocks);
     hipStream_t s = as_stream(stream);
     ProfScope prof(VITMI_FAM_OTHER, s, 2.0 * a->B * a->N * heads * a->DH * esz);
     const size_t lds = (size_t)P * 8 * (1 + tile);
-    if (a->dt == VITMI_F32) {
-        if (V == 4) launch_rope<float, 4>(k, a->interleaved, (unsigned)blocks, lds, s);
-        else launch_rope<float, 1>(k, a->interleaved, (unsigned)blocks, lds, s);
-    } else {
-        if (V == 8) launch_rope<bf16_t, 8>(k, a->interleaved, (unsigned)blocks, lds, s);
-        else if (V == 4) launch_rope<bf16_t, 4>(k, a->interleaved, (unsigned)blocks, lds, s);
-        else launch_rope<bf16_t, 1>(k, a->interleaved, (unsigned)blocks, lds, s);
-    }
+    if (a->dt == VITMI_F32) launch_rope<float>(k, mode, V, (unsigned)blocks, lds, s);
+    else launch_rope<bf16_t>(k, mode, V, (unsigned)blocks, lds, s);
     VITMI_LAUNCH_CHECK("vitmi_rope_axes");
     return VITMI_OK;
 }
