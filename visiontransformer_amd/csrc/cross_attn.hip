@@ -53,8 +53,6 @@ struct XaArgs {
     long long n_q, n_k;                   // elements of q and of k
 };
 
-typedef float xf32x4 __attribute__((ext_vector_type(4)));
-
 template <typename T> struct Mx;
 template <> struct Mx<bf16_t> {
     typedef bf16x8 frag;
@@ -82,13 +80,13 @@ template <> __device__ __forceinline__ int key_of_row<bf16_t>(int m) {
     const int g = m >> 3;
     return 16 * (g >> 1) + 8 * ((m >> 2) & 1) + 4 * (g & 1) + (m & 3);
 }
-template <> __device__ __forceinline__ int key_of_row<float>(int m) { return m; }
+template <> __device__ __forceinline__ int key_of_row<float>(int m) { return (m & 24) + 2 * (m & 3) + ((m >> 2) & 1); }
 template <typename T> __device__ __forceinline__ int key_of(int e, int h);
 template <> __device__ __forceinline__ int key_of<bf16_t>(int e, int h) {
     const int g = e >> 2;
     return 16 * (g >> 1) + 8 * h + 4 * (g & 1) + (e & 3);
 }
-template <> __device__ __forceinline__ int key_of<float>(int e, int h) { return 8 * (e >> 2) + 4 * h + (e & 3); }
+template <> __device__ __forceinline__ int key_of<float>(int e, int h) { return 8 * (e >> 2) + 2 * (e & 3) + h; }
 
 // registers of a 32 x 32 accumulator as B operand: group n of KD consecutive sequence indices
 __device__ __forceinline__ bf16x8 acc_frag(const f32x16& p, int n, bf16_t) {
@@ -111,34 +109,41 @@ template <typename T> __device__ __forceinline__ typename Mx<T>::frag zero_frag(
     return z;
 }
 
-// row of an LDS image in elements: DP plus 16 bytes, which spreads both kinds of read over the banks
-template <typename T, int DP> constexpr int ld_of() { return DP + 16 / (int)sizeof(T); }
+// LDS image of KT sequence rows: planes of 32 dims, [DP / 32][KT][32].  A row of a plane is CP 16-byte chunks, chunk c of
+// row r stored at c ^ swz(r).  With rows of 64 (bf16) or 128 bytes (fp32) both kinds of read then touch every bank once:
+// 16 rows of one chunk (the rows of a row read), and for bf16 4 rows of all chunks (a transposing read), for fp32 two
+// adjacent rows (a column read) -- and every address is a lane constant plus an immediate.
+template <typename T> constexpr int cp_of() { return 32 * (int)sizeof(T) / 16; }
+template <typename T> __device__ __forceinline__ int swz(int row) { return sizeof(T) == 2 ? (row >> 2) & 3 : (row >> 1) & 7; }
+template <typename T> __device__ __forceinline__ int img_off(int row, int chunk) { return row * 32 + ((chunk ^ swz<T>(row)) * Mx<T>::FE); }
 
-template <typename T, int DP>
+template <typename T, int KT>
 __device__ __forceinline__ typename Mx<T>::frag row_frag(const T* img, int row, int c, int h) {
-    return *reinterpret_cast<const typename Mx<T>::frag*>(img + row * ld_of<T, DP>() + c * Mx<T>::KD + h * Mx<T>::FE);
+    constexpr int PER = 32 / Mx<T>::KD;      // fragments a plane
+    return *reinterpret_cast<const typename Mx<T>::frag*>(img + (c / PER) * KT * 32 + img_off<T>(row, (c % PER) * 2 + h));
 }
-// A operand [32 columns col0.. as rows][KD sequence rows seq0..]: lane l holds column col0 + l % 32 of sequence rows
-// seq0 + FE (l / 32) + 0..FE-1
-template <int DP>
-__device__ __forceinline__ bf16x8 col_frag(const bf16_t* img, int seq0, int col0, int lane) {
-    const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
-    const bf16_t* a = img + (seq0 + 8 * (g >> 1) + q) * ld_of<bf16_t, DP>() + col0 + 16 * (g & 1) + 4 * p;
+// A operand [32 dims of plane db as rows][KD sequence rows seq0..]: lane l holds dim l % 32 of the sequence rows that
+// accumulator registers of half wave l / 32 hold (key_of)
+template <int KT>
+__device__ __forceinline__ bf16x8 col_frag(const bf16_t* img, int seq0, int db, int lane) {
+    const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3, row = 8 * (g >> 1) + q, chunk = 2 * (g & 1) + (p >> 1);
+    const bf16_t* plane = img + db * KT * 32 + seq0 * 32 + 4 * (p & 1);
     typedef __attribute__((address_space(3))) s16x4* lp;
     union {
         s16x4 h[2];
         bf16x8 v;
     } u;
-    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)a);
-    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(a + 4 * ld_of<bf16_t, DP>()));
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(plane + img_off<bf16_t>(row, chunk)));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(plane + img_off<bf16_t>(row + 4, chunk)));
     return u.v;
 }
-template <int DP>
-__device__ __forceinline__ f32x4 col_frag(const float* img, int seq0, int col0, int lane) {
-    const float* a = img + (seq0 + 4 * (lane >> 5)) * ld_of<float, DP>() + col0 + (lane & 31);
+template <int KT>
+__device__ __forceinline__ f32x4 col_frag(const float* img, int seq0, int db, int lane) {
+    const float* plane = img + db * KT * 32;
+    const int d = lane & 31;
     f32x4 r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = a[j * ld_of<float, DP>()];
+    for (int j = 0; j < 4; ++j) r[j] = plane[img_off<float>(seq0 + 2 * j + (lane >> 5), d >> 2) + (d & 3)];
     return r;
 }
 
@@ -161,68 +166,125 @@ __device__ __forceinline__ int keys_of(const XaArgs& a, int b) {
     const long long n = a.len64 ? ((const long long*)a.kv_len)[b] : (long long)((const int*)a.kv_len)[b];
     return (int)(n < 0 ? 0 : (n > a.Nk ? a.Nk : n));
 }
-// one bit per key of [key0, key0 + KT): allowed
-template <int KT>
-__device__ __forceinline__ unsigned long long tile_mask(const XaArgs& a, int b, int key0, int n, int lane) {
-    if (key0 >= n) return 0;
-    const int left = n - key0 < KT ? n - key0 : KT;
-    unsigned long long m = left >= 64 ? ~0ull : (1ull << left) - 1;
-    if (a.key_mask) {
-        const bool on = lane < left && a.key_mask[b * a.mask_stride + key0 + lane] != 0;
-        m &= __ballot(on);
-    }
-    return m;
-}
 template <int KT> constexpr unsigned long long full_mask() { return KT >= 64 ? ~0ull : (1ull << KT) - 1; }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
-// a tile of KT rows of two matrices on its way from global memory to LDS through registers, by TH threads
-template <typename T, int DP, bool VEC, int KT, int TH>
+__device__ __attribute__((aligned(16))) unsigned int xa_zero16[4] = {0u, 0u, 0u, 0u};
+
+// Starts a load of 16 bytes a lane straight into LDS, lane i's at byte `to` + 16 i (`to` the same in the whole wave).  Inline
+// assembly, because the compiler would hold every transposing LDS read back until such a load is complete, whichever
+// image it fills; wait_loads() and a barrier stand between a load and the reads of its image.
+__device__ __forceinline__ void load_to_lds(const void* from, unsigned to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ unsigned lds_addr(const void* p) {
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
+}
+
+// A tile of KT rows of two matrices into their LDS images.  DMA: 16-byte loads that land in LDS without a register between
+// (fetch starts them, they are complete after the next wait on vector memory), 64 lanes filling 1 KB of an image in
+// its own order: with 256 threads a load instruction is one plane, so that a thread keeps one row.  Otherwise: through
+// registers, fetched row by row, stored by store().  Rows whose mask bit is off and dims from D on are zeros.
+template <typename T, int DP, bool VEC, int KT, int TH, bool DMA>
 struct Stage {
-    static constexpr int CPR = DP / Mx<T>::FE, IT = KT * CPR / TH;
-    static_assert(KT * CPR % TH == 0, "a tile is a whole number of pieces per thread");
+    static constexpr int CP = cp_of<T>(), NP = DP / 32, RPI = TH / CP;
+    static constexpr int CPR = NP * CP, IT = DMA ? 1 : KT * CPR / TH;
+    static_assert(DMA ? RPI == KT && VEC : KT * CPR % TH == 0, "a tile is a whole number of pieces per thread");
     typename Mx<T>::frag x[IT], y[IT];
-    // rows row0 + r of two matrices with row strides lx, ly; rows from n on are not read
-    __device__ __forceinline__ void fetch(const T* px, long long lx, const T* py, long long ly, int row0, int n, int D, int t) {
+    // the thread's row of a tile (DMA), or row of piece i
+    __device__ __forceinline__ static int row_of(int i, int t) { return DMA ? t / CP : (t + i * TH) / CPR; }
+    // px / py: start of the row that row_of names, valid where ok
+    __device__ __forceinline__ void piece(int i, const T* px, const T* py, bool ok, T* ix, T* iy, int D, int t) {
+        if (DMA) {
+            const int r = t / CP, chunk = (t % CP) ^ swz<T>(r);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int d = 32 * p + chunk * Mx<T>::FE;
+                const bool on = ok && d < D;
+                const void* sx = on ? (const void*)(px + d) : (const void*)xa_zero16;
+                const void* sy = on ? (const void*)(py + d) : (const void*)xa_zero16;
+                const int o = p * KT * 32 + (t & ~63) * Mx<T>::FE;
+                load_to_lds(sx, lds_addr(ix + o));
+                load_to_lds(sy, lds_addr(iy + o));
+            }
+        } else {
+            const int d = ((t + i * TH) % CPR) * Mx<T>::FE;
+            x[i] = y[i] = zero_frag<T>();
+            if (ok) {
+                x[i] = global_piece<T, VEC>(px, d, D);
+                y[i] = global_piece<T, VEC>(py, d, D);
+            }
+        }
+    }
+    // key rows row0 + r with row strides lx, ly
+    __device__ __forceinline__ void fetch(const T* px, long long lx, const T* py, long long ly, int row0, unsigned long long mask, T* ix,
+                                          T* iy, int D, int t) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = t + i * TH, r = row0 + c / CPR, d = (c % CPR) * Mx<T>::FE;
-            x[i] = y[i] = zero_frag<T>();
-            if (r < n) {
-                x[i] = global_piece<T, VEC>(px + r * lx, d, D);
-                y[i] = global_piece<T, VEC>(py + r * ly, d, D);
-            }
+            const int r = row_of(i, t);
+            piece(i, px + (long long)(row0 + r) * lx, py + (long long)(row0 + r) * ly, (mask >> r) & 1, ix, iy, D, t);
         }
     }
     // query rows: row r of the flattened group is position r % Nq of head r / Nq
-    __device__ __forceinline__ void fetch_rows(const T* px, const long long* sx, const T* py, const long long* sy, int row0, int R, int Nq,
-                                               int D, int t) {
+    __device__ __forceinline__ void fetch_rows(const T* px, const long long* sx, const T* py, const long long* sy, int row0, int R, int Nq, T* ix,
+                                               T* iy, int D, int t) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = t + i * TH, r = row0 + c / CPR, d = (c % CPR) * Mx<T>::FE;
-            x[i] = y[i] = zero_frag<T>();
-            if (r < R) {
-                const int g = r / Nq, n = r - g * Nq;
-                x[i] = global_piece<T, VEC>(px + n * sx[1] + g * sx[2], d, D);
-                y[i] = global_piece<T, VEC>(py + n * sy[1] + g * sy[2], d, D);
-            }
+            const int r = row0 + row_of(i, t), g = r / Nq, n = r - g * Nq;
+            piece(i, px + n * sx[1] + g * sx[2], py + n * sy[1] + g * sy[2], r < R, ix, iy, D, t);
         }
     }
-    __device__ __forceinline__ void store(T* ix, T* iy, unsigned long long mask, int t) {
-        if (mask != full_mask<KT>()) {
-#pragma unroll
-            for (int i = 0; i < IT; ++i)
-                if (!((mask >> ((t + i * TH) / CPR)) & 1)) x[i] = y[i] = zero_frag<T>();
-        }
+    __device__ __forceinline__ void store(T* ix, T* iy, int t) {
+        if (DMA) return;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = t + i * TH, o = (c / CPR) * ld_of<T, DP>() + (c % CPR) * Mx<T>::FE;
+            const int c = t + i * TH, r = c / CPR, ch = c % CPR, o = (ch / CP) * KT * 32 + img_off<T>(r, ch % CP);
             *reinterpret_cast<typename Mx<T>::frag*>(ix + o) = x[i];
             *reinterpret_cast<typename Mx<T>::frag*>(iy + o) = y[i];
         }
     }
 };
+
+// The key mask of tiles t0, t0 + step, ..: cur is the running tile's, next the following one's; the mask bytes of the tile after
+// that are already on their way
+template <int KT>
+struct MaskWalk {
+    unsigned long long cur, next;
+    int byte, n, step, b;
+    __device__ __forceinline__ int load(const XaArgs& a, int tile, int lane) const {
+        const int key = tile * KT + lane;
+        return a.key_mask && lane < KT && key < n ? a.key_mask[b * a.mask_stride + key] : 0;
+    }
+    __device__ __forceinline__ unsigned long long bits(const XaArgs& a, int tile, int v) const {
+        const long long left = (long long)n - (long long)tile * KT;
+        if (left <= 0) return 0;
+        const unsigned long long m = left >= 64 ? ~0ull : (1ull << left) - 1;
+        return (a.key_mask ? __ballot(v != 0) : m) & m & full_mask<KT>();
+    }
+    __device__ __forceinline__ void start(const XaArgs& a, int b_, int n_, int t0, int step_, int lane) {
+        b = b_;
+        n = n_;
+        step = step_;
+        const int v0 = load(a, t0, lane), v1 = load(a, t0 + step, lane);
+        byte = load(a, t0 + 2 * step, lane);
+        cur = bits(a, t0, v0);
+        next = bits(a, t0 + step, v1);
+    }
+    __device__ __forceinline__ void advance(const XaArgs& a, int tile, int lane) {     // from tile to tile + step
+        cur = next;
+        next = bits(a, tile + 2 * step, byte);
+        byte = load(a, tile + 3 * step, lane);
+    }
+};
+
+// every vector-memory load of the wave has landed, the LDS-bound ones among them; the builtin (vmcnt 0, the other counters
+// free), so that the compiler knows it of its own loads too
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+    asm volatile("" ::: "memory");
+}
 
 // Workgroups are dealt to the 8 XCDs round-robin: this gives each XCD a contiguous range of tiles, whose keys it then
 // fetches into its own L2 once
@@ -232,13 +294,13 @@ __device__ __forceinline__ int xa_block() {
 }
 
 // scores of one 32-key block against the lane's query
-template <typename T, int DP>
+template <typename T, int DP, int KT>
 __device__ __forceinline__ void scores(f32x16& s, const T* img, int key0, const typename Mx<T>::frag (&f)[DP / Mx<T>::KD], int lane) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[e] = 0.f;
     const int row = key0 + key_of_row<T>(lane & 31);
 #pragma unroll
-    for (int c = 0; c < DP / Mx<T>::KD; ++c) mma(s, row_frag<T, DP>(img, row, c, lane >> 5), f[c]);
+    for (int c = 0; c < DP / Mx<T>::KD; ++c) mma(s, row_frag<T, KT>(img, row, c, lane >> 5), f[c]);
 }
 
 template <typename T>
@@ -262,7 +324,7 @@ __device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typen
     for (int cc = 0; cc < DP / Mx<T>::KD; ++cc)       // the blocks' accumulation chains take turns
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-            mma(s[kb], row_frag<T, DP>(kimg, 32 * kb + key_of_row<T>(lane & 31), cc, lane >> 5), qf[cc]);
+            mma(s[kb], row_frag<T, KT>(kimg, 32 * kb + key_of_row<T>(lane & 31), cc, lane >> 5), qf[cc]);
     if (mask != full_mask<KT>()) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) mask_scores<T>(s[kb], (unsigned)(mask >> (32 * kb)), lane >> 5);
@@ -296,7 +358,7 @@ __device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typen
         for (int n = 0; n < 32 / Mx<T>::KD; ++n) {
             const typename Mx<T>::frag pf = acc_frag(s[kb], n, T());
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<DP>(vimg, 32 * kb + n * Mx<T>::KD, 32 * d, lane), pf);
+            for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<KT>(vimg, 32 * kb + n * Mx<T>::KD, d, lane), pf);
         }
 }
 
@@ -360,7 +422,7 @@ __device__ __forceinline__ void split_range(int tiles, int splits, int split, in
 
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_kernel(XaArgs a) {
-    constexpr int KT = Mx<T>::KT, IMG = KT * ld_of<T, DP>();
+    constexpr int KT = Mx<T>::KT, IMG = KT * DP;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);        // K, V, K, V
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
@@ -391,20 +453,23 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     int t0, t1;
     split_range((n + KT - 1) / KT, a.splits, split, t0, t1);
-    Stage<T, DP, VEC, KT, XA_THREADS> st;
-    unsigned long long mask = 0;
+    Stage<T, DP, VEC, KT, XA_THREADS, VEC> st;
+    MaskWalk<KT> mw;
     if (t0 < t1) {
-        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, n, a.D, t);
-        mask = tile_mask<KT>(a, b, t0 * KT, n, lane);
+        mw.start(a, b, n, t0, 1, lane);
+        T* img = lds + (t0 & 1) * 2 * IMG;
+        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, mw.cur, img, img + IMG, a.D, t);
     }
     for (int kt = t0; kt < t1; ++kt) {
         T* img = lds + (kt & 1) * 2 * IMG;
-        const unsigned long long mk = mask;
-        st.store(img, img + IMG, mk, t);
+        const unsigned long long mk = mw.cur;
+        st.store(img, img + IMG, t);
+        wait_loads();
         __syncthreads();
         if (kt + 1 < t1) {
-            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, n, a.D, t);
-            mask = tile_mask<KT>(a, b, (kt + 1) * KT, n, lane);
+            T* nxt = lds + ((kt + 1) & 1) * 2 * IMG;
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t);
+            mw.advance(a, kt, lane);
         }
         if (mk) attend<T, DP, KT>(img, img + IMG, qf, mk, a.c, o, m, l, lane);
     }
@@ -421,7 +486,7 @@ __device__ __forceinline__ void wave_fence() {
 // up to 64 rows a problem: every wave walks 32-key tiles of its own for the same 32 rows
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
-    constexpr int KT = 32, IMG = KT * ld_of<T, DP>();
+    constexpr int KT = 32, IMG = KT * DP;
     extern __shared__ __align__(16) char xa_lds[];
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -438,11 +503,11 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     int t0, t1;
     split_range((n + KT - 1) / KT, a.splits, split, t0, t1);
-    Stage<T, DP, VEC, KT, 64> st;
-    unsigned long long mask = 0;
+    Stage<T, DP, VEC, KT, 64, false> st;
+    MaskWalk<KT> mw;
     if (t0 + wave < t1) {
-        st.fetch(kp, a.ks[1], vp, a.vs[1], (t0 + wave) * KT, n, a.D, lane);
-        mask = tile_mask<KT>(a, b, (t0 + wave) * KT, n, lane);
+        mw.start(a, b, n, t0 + wave, 4, lane);
+        st.fetch(kp, a.ks[1], vp, a.vs[1], (t0 + wave) * KT, mw.cur, nullptr, nullptr, a.D, lane);
     }
     typename Mx<T>::frag qf[DP / Mx<T>::KD];
     {
@@ -459,12 +524,12 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
     for (int kt = t0 + wave; kt < t1; kt += 4) {
-        const unsigned long long mk = mask;
-        st.store(img, img + IMG, mk, lane);
+        const unsigned long long mk = mw.cur;
+        st.store(img, img + IMG, lane);
         wave_fence();
         if (kt + 4 < t1) {
-            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, n, a.D, lane);
-            mask = tile_mask<KT>(a, b, (kt + 4) * KT, n, lane);
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, mw.next, nullptr, nullptr, a.D, lane);
+            mw.advance(a, kt, lane);
         }
         if (mk) attend<T, DP, KT>(img, img + IMG, qf, mk, a.c, o, m, l, lane);
         wave_fence();
@@ -574,7 +639,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long row
 // dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_kernel(XaArgs a) {
-    constexpr int KT = Mx<T>::KT, IMG = KT * ld_of<T, DP>(), NF = DP / Mx<T>::KD;
+    constexpr int KT = Mx<T>::KT, IMG = KT * DP, NF = DP / Mx<T>::KD;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
@@ -618,27 +683,30 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_k
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     int t0, t1;
     split_range(a.dq ? (n + KT - 1) / KT : 0, a.splits, split, t0, t1);      // without dq only delta is wanted
-    Stage<T, DP, VEC, KT, XA_THREADS> st;
-    unsigned long long mask = 0;
+    Stage<T, DP, VEC, KT, XA_THREADS, VEC> st;
+    MaskWalk<KT> mw;
     if (t0 < t1) {
-        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, n, a.D, t);
-        mask = tile_mask<KT>(a, b, t0 * KT, n, lane);
+        mw.start(a, b, n, t0, 1, lane);
+        T* img = lds + (t0 & 1) * 2 * IMG;
+        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, mw.cur, img, img + IMG, a.D, t);
     }
     for (int kt = t0; kt < t1; ++kt) {
         T* img = lds + (kt & 1) * 2 * IMG;
-        const unsigned long long mk = mask;
-        st.store(img, img + IMG, mk, t);
+        const unsigned long long mk = mw.cur;
+        st.store(img, img + IMG, t);
+        wait_loads();
         __syncthreads();
         if (kt + 1 < t1) {
-            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, n, a.D, t);
-            mask = tile_mask<KT>(a, b, (kt + 1) * KT, n, lane);
+            T* nxt = lds + ((kt + 1) & 1) * 2 * IMG;
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t);
+            mw.advance(a, kt, lane);
         }
         if (mk) {
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
                 f32x16 s, dp;
-                scores<T, DP>(s, img, 32 * kb, qf, lane);
-                scores<T, DP>(dp, img + IMG, 32 * kb, gf, lane);
+                scores<T, DP, KT>(s, img, 32 * kb, qf, lane);
+                scores<T, DP, KT>(dp, img + IMG, 32 * kb, gf, lane);
                 if (mk != full_mask<KT>()) mask_scores<T>(s, (unsigned)(mk >> (32 * kb)), h);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse)) * (dp[e] - delta);
@@ -646,7 +714,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_k
                 for (int g = 0; g < 32 / Mx<T>::KD; ++g) {
                     const typename Mx<T>::frag f = acc_frag(s, g, T());
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) mma(acc[d], col_frag<DP>(img, 32 * kb + g * Mx<T>::KD, 32 * d, lane), f);
+                    for (int d = 0; d < DP / 32; ++d) mma(acc[d], col_frag<KT>(img, 32 * kb + g * Mx<T>::KD, d, lane), f);
                 }
             }
         }
@@ -660,8 +728,8 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_k
 
 // dk and dv: four waves of 32 keys over the row tiles of the whole group
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(XA_THREADS, DP == 128 || sizeof(T) == 4 ? 1 : 2) void xattn_dkv_kernel(XaArgs a) {
-    constexpr int QT = Mx<T>::KT, IMG = QT * ld_of<T, DP>(), NF = DP / Mx<T>::KD;
+__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dkv_kernel(XaArgs a) {
+    constexpr int QT = Mx<T>::KT, IMG = QT * DP, NF = DP / Mx<T>::KD;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);                           // Q, dO, Q, dO
     float* const rows = reinterpret_cast<float*>(xa_lds + 4 * IMG * sizeof(T));   // [2][lse, delta][QT]
@@ -697,10 +765,11 @@ __global__ __launch_bounds__(XA_THREADS, DP == 128 || sizeof(T) == 4 ? 1 : 2) vo
     const T* qp = (const T*)a.q + b * a.qs[0] + (long long)hk * a.G * a.qs[2];
     const T* gp = (const T*)a.dout + b * a.dos[0] + (long long)hk * a.G * a.dos[2];
     const long long sti = ((long long)b * a.Hk + hk) * a.R;
-    Stage<T, DP, VEC, QT, XA_THREADS> st;
+    Stage<T, DP, VEC, QT, XA_THREADS, VEC> st;
     float stat = 0.f;                                     // threads 0..QT-1: lse, QT..2QT-1: delta
     auto fetch = [&](int tile) {
-        st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, a.D, t);
+        T* img = lds + (tile & 1) * 2 * IMG;
+        st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, img, img + IMG, a.D, t);
         if (t < 2 * QT) {
             const int r = tile * QT + (t < QT ? t : t - QT);
             stat = t < QT ? INFINITY : 0.f;
@@ -711,15 +780,16 @@ __global__ __launch_bounds__(XA_THREADS, DP == 128 || sizeof(T) == 4 ? 1 : 2) vo
     for (int qt = t0; qt < t1; ++qt) {
         T* img = lds + (qt & 1) * 2 * IMG;
         float* rs = rows + (qt & 1) * 2 * QT;
-        st.store(img, img + IMG, full_mask<QT>(), t);
+        st.store(img, img + IMG, t);
         if (t < 2 * QT) rs[t] = stat;
+        wait_loads();
         __syncthreads();
         if (qt + 1 < t1) fetch(qt + 1);
 #pragma unroll
         for (int qb = 0; qb < QT / 32; ++qb) {
             f32x16 s, dp;
-            scores<T, DP>(s, img, 32 * qb, kf, lane);
-            scores<T, DP>(dp, img + IMG, 32 * qb, vf, lane);
+            scores<T, DP, QT>(s, img, 32 * qb, kf, lane);
+            scores<T, DP, QT>(dp, img + IMG, 32 * qb, vf, lane);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int q = 32 * qb + key_of<T>(e, h);
@@ -731,8 +801,8 @@ __global__ __launch_bounds__(XA_THREADS, DP == 128 || sizeof(T) == 4 ? 1 : 2) vo
                 const typename Mx<T>::frag pf = acc_frag(s, g, T()), df = acc_frag(dp, g, T());
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
-                    mma(dv[d], col_frag<DP>(img + IMG, 32 * qb + g * Mx<T>::KD, 32 * d, lane), pf);
-                    mma(dk[d], col_frag<DP>(img, 32 * qb + g * Mx<T>::KD, 32 * d, lane), df);
+                    mma(dv[d], col_frag<QT>(img + IMG, 32 * qb + g * Mx<T>::KD, d, lane), pf);
+                    mma(dk[d], col_frag<QT>(img, 32 * qb + g * Mx<T>::KD, d, lane), df);
                 }
             }
         }
@@ -860,8 +930,8 @@ enum { XK_FWD, XK_FEW, XK_DQ, XK_DKV };
 
 template <typename T, int DP, bool VEC>
 int xa_launch(int kind, const XaArgs& a, long long blocks, hipStream_t s) {
-    constexpr size_t tile4 = 4ull * Mx<T>::KT * ld_of<T, DP>() * sizeof(T);
-    constexpr size_t few = std::max<size_t>(8ull * 32 * ld_of<T, DP>() * sizeof(T), (4ull * DP * 32 + 256) * sizeof(float));
+    constexpr size_t tile4 = 4ull * Mx<T>::KT * DP * sizeof(T);
+    constexpr size_t few = std::max<size_t>(8ull * 32 * DP * sizeof(T), (4ull * DP * 32 + 256) * sizeof(float));
     constexpr size_t dkv = tile4 + 4ull * Mx<T>::KT * sizeof(float);
     const size_t lds = kind == XK_FEW ? few : kind == XK_DKV ? dkv : tile4;
     const void* fn = kind == XK_FWD   ? (const void*)&xattn_fwd_kernel<T, DP, VEC>
