@@ -22,6 +22,7 @@
 // results in the workspace, joined by a second launch.
 // Masked keys: their K and V rows are staged as zeros whatever they hold, their scores are -inf.
 #include <algorithm>
+#include <atomic>
 
 #include "common.h"
 
@@ -49,8 +50,10 @@ struct XaArgs {
     long long dos[3];
     float* delta;                         // [B, Hk, R]
     void *dq, *dk, *dv;                   // dense, or NULL
-    float *part_dq, *part_dk, *part_dv;
-    long long n_q, n_k;                   // elements of q and of k
+    float *part_dq;
+    float* part_kv;                       // [workgroups][first, last share][dk, dv][128][D]
+    int B;
+    long long n_q;                        // elements of q
 };
 
 template <typename T> struct Mx;
@@ -101,6 +104,21 @@ __device__ __forceinline__ bf16x8 acc_frag(const f32x16& p, int n, bf16_t) {
 __device__ __forceinline__ f32x4 acc_frag(const f32x16& p, int n, float) {
     return f32x4{p[4 * n], p[4 * n + 1], p[4 * n + 2], p[4 * n + 3]};
 }
+
+// l plus the sum of a fragment of probabilities: the rounded ones that the output is summed of, two an instruction; fp32 adds its
+// own as they are formed
+__device__ __forceinline__ float add_frag(const bf16x8& p, float l) {
+    union {
+        bf16x8 v;
+        bf16x2 h[4];
+    } u;
+    u.v = p;
+    const bf16x2 one = {(bf16_t)1.f, (bf16_t)1.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) l = __builtin_amdgcn_fdot2_f32_bf16(u.h[i], one, l, false);
+    return l;
+}
+__device__ __forceinline__ float add_frag(const f32x4&, float l) { return l; }
 
 template <typename T> __device__ __forceinline__ typename Mx<T>::frag zero_frag() {
     typename Mx<T>::frag z;
@@ -166,7 +184,7 @@ __device__ __forceinline__ int keys_of(const XaArgs& a, int b) {
     const long long n = a.len64 ? ((const long long*)a.kv_len)[b] : (long long)((const int*)a.kv_len)[b];
     return (int)(n < 0 ? 0 : (n > a.Nk ? a.Nk : n));
 }
-template <int KT> constexpr unsigned long long full_mask() { return KT >= 64 ? ~0ull : (1ull << KT) - 1; }
+template <int KT> constexpr unsigned long long full_mask() { return ~0ull >> (64 - KT); }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
@@ -286,11 +304,15 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("" ::: "memory");
 }
 
-// Workgroups are dealt to the 8 XCDs round-robin: this gives each XCD a contiguous range of tiles, whose keys it then
-// fetches into its own L2 once
+// Workgroups are dealt to the 8 XCDs round-robin.  This cuts the launch into 16 contiguous pieces, two an XCD: neighbours in
+// a piece read the same keys, which the XCD's L2 then fetches once, and the second piece comes from the other half of the
+// batch, so that long and short samples even out over the XCDs.
 __device__ __forceinline__ int xa_block() {
-    const int n = gridDim.x, x = blockIdx.x & 7, slot = blockIdx.x >> 3, q = n >> 3, rem = n & 7;
-    return x * q + (x < rem ? x : rem) + slot;
+    const int n = gridDim.x, x = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int q = n >> 4, rem = n & 15;                        // pieces of q or q + 1
+    const int first = q + (x < rem);                           // XCD x's first piece is piece x, its second x + 8
+    const int p = slot < first ? x : x + 8, off = slot < first ? slot : slot - first;
+    return p * q + (p < rem ? p : rem) + off;
 }
 
 // scores of one 32-key block against the lane's query
@@ -310,30 +332,16 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned m, int h) {
         if (!((m >> key_of<T>(e, h)) & 1)) s[e] = -INFINITY;
 }
 
-// one staged tile against the lane's query: running softmax and o^T += V^T P^T
+// 32 staged keys (their images' rows from kimg, vimg on) against the lane's query: running softmax and o^T += V^T P^T
 template <typename T, int DP, int KT>
-__device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typename Mx<T>::frag (&qf)[DP / Mx<T>::KD],
-                                       unsigned long long mask, float c, f32x16 (&o)[DP / 32], float& m, float& l, int lane) {
-    constexpr int KB = KT / 32;
-    f32x16 s[KB];
+__device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typename Mx<T>::frag (&qf)[DP / Mx<T>::KD], unsigned mask, float c,
+                                       f32x16 (&o)[DP / 32], float& m, float& l, int lane) {
+    f32x16 s;
+    scores<T, DP, KT>(s, kimg, 0, qf, lane);
+    if (mask != ~0u) mask_scores<T>(s, mask, lane >> 5);
+    float mx = s[0];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
-#pragma unroll
-    for (int cc = 0; cc < DP / Mx<T>::KD; ++cc)       // the blocks' accumulation chains take turns
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-            mma(s[kb], row_frag<T, KT>(kimg, 32 * kb + key_of_row<T>(lane & 31), cc, lane >> 5), qf[cc]);
-    if (mask != full_mask<KT>()) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) mask_scores<T>(s[kb], (unsigned)(mask >> (32 * kb)), lane >> 5);
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
     mx *= c;
     if (__any(mx > m + XA_SLACK)) {
         const float mn = fmaxf(m, fmaxf(mx, other_half(mx)));
@@ -346,20 +354,17 @@ __device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typen
             for (int e = 0; e < 16; ++e) o[d][e] *= f;
     }
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -m));
+        if (sizeof(T) == 4) l += s[e];
+    }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            s[kb][e] = __builtin_amdgcn_exp2f(fmaf(s[kb][e], c, -m));
-            l += s[kb][e];
-        }
+    for (int n = 0; n < 32 / Mx<T>::KD; ++n) {
+        const typename Mx<T>::frag pf = acc_frag(s, n, T());
+        l = add_frag(pf, l);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int n = 0; n < 32 / Mx<T>::KD; ++n) {
-            const typename Mx<T>::frag pf = acc_frag(s[kb], n, T());
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<KT>(vimg, 32 * kb + n * Mx<T>::KD, d, lane), pf);
-        }
+        for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<KT>(vimg, n * Mx<T>::KD, d, lane), pf);
+    }
 }
 
 // four consecutive dims (8 g + 4 h ..) of an accumulator block to a dense row
@@ -434,6 +439,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
     idx /= a.splits;
     const int hk = idx % a.Hk, b = idx / a.Hk;
     const int r = rt * 128 + wave * 32 + (lane & 31);
+    const bool busy = rt * 128 + wave * 32 < a.R;         // the wave has a row; without one it only helps staging
     typename Mx<T>::frag qf[DP / Mx<T>::KD];
     {
         const int g = r / a.Nq, n = r - g * a.Nq;
@@ -471,7 +477,11 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
             st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t);
             mw.advance(a, kt, lane);
         }
-        if (mk) attend<T, DP, KT>(img, img + IMG, qf, mk, a.c, o, m, l, lane);
+        if (busy && mk) {
+#pragma unroll
+            for (int kb = 0; kb < KT / 32; ++kb)          // blocks of 32 keys without an allowed one are left out
+                if ((unsigned)(mk >> (32 * kb))) attend<T, DP, KT>(img + kb * 1024, img + IMG + kb * 1024, qf, (unsigned)(mk >> (32 * kb)), a.c, o, m, l, lane);
+        }
     }
     l += other_half(l);
     finish_rows<T, DP, VEC>(a, b, hk, r, split, o, m, l, h);
@@ -531,7 +541,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
             st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, mw.next, nullptr, nullptr, a.D, lane);
             mw.advance(a, kt, lane);
         }
-        if (mk) attend<T, DP, KT>(img, img + IMG, qf, mk, a.c, o, m, l, lane);
+        if (mk) attend<T, DP, KT>(img, img + IMG, qf, (unsigned)mk, a.c, o, m, l, lane);
         wave_fence();
     }
     l += other_half(l);
@@ -638,7 +648,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long row
 
 // dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles
 template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_kernel(XaArgs a) {
+__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xattn_dq_kernel(XaArgs a) {
     constexpr int KT = Mx<T>::KT, IMG = KT * DP, NF = DP / Mx<T>::KD;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);
@@ -701,9 +711,10 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_k
             st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t);
             mw.advance(a, kt, lane);
         }
-        if (mk) {
+        if (mk && rt * 128 + wave * 32 < a.R) {
 #pragma unroll
             for (int kb = 0; kb < KT / 32; ++kb) {
+                if (!(unsigned)(mk >> (32 * kb))) continue;
                 f32x16 s, dp;
                 scores<T, DP, KT>(s, img, 32 * kb, qf, lane);
                 scores<T, DP, KT>(dp, img + IMG, 32 * kb, gf, lane);
@@ -726,111 +737,257 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dq_k
         store_acc<float, VEC, DP>(a.part_dq + split * a.n_q + row, acc, 1.f, h, a.D);
 }
 
+// How the dk / dv launch cuts its work: a unit is one row tile against one live tile of 128 keys.  Streamed, every workgroup
+// takes an equal share of the units in a row -- the end of one key tile, whole ones, the start of another -- because whole
+// key tiles, of which there may be a few more than the chip holds at once, would leave it idle for up to half the time.
+// With three or more workgroups a key tile the shares end at tile borders.  Lengths per sample are only known here, so
+// each wave counts the live tiles itself (64 samples a step).
+__device__ __forceinline__ long long uniform(long long v) {       // a wave-uniform value into scalar registers
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)((unsigned long long)v >> 32));
+    return (long long)(((unsigned long long)hi << 32) | lo);
+}
+struct Stream {
+    long long units;      // in all
+    int rt, nb;           // row tiles a key tile, workgroups that share the units
+    __device__ __forceinline__ long long begin(int i) const { return units * i / nb; }
+    // the workgroup that holds unit x
+    __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * nb + units - 1) / units) - 1; }
+};
+__device__ __forceinline__ int lanes_scan(int v, int lane) {     // inclusive sums over the lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+__device__ __forceinline__ int live_tiles(const XaArgs& a, int b) { return (keys_of(a, b) + 127) >> 7; }
+__device__ __forceinline__ Stream stream_of(const XaArgs& a, int grid, int row_tiles, int lane) {
+    long long tiles = 0;
+    if (!a.kv_len) {
+        tiles = (long long)a.B * a.tiles;
+    } else {
+        for (int b0 = 0; b0 < a.B; b0 += 64)
+            tiles += __shfl(lanes_scan(b0 + lane < a.B ? live_tiles(a, b0 + lane) : 0, lane), 63, 64);
+    }
+    tiles = uniform(tiles * a.Hk);
+    Stream s;
+    s.rt = row_tiles;
+    s.units = tiles * row_tiles;
+    s.nb = tiles > 0 && grid >= 3 * tiles ? (int)(grid / tiles * tiles) : grid;
+    return s;
+}
+// sample, key head and key tile of live tile tau (samples in order, then heads, then tiles)
+__device__ __forceinline__ void stream_tile(const XaArgs& a, long long tau, int lane, int& b, int& hk, int& kt) {
+    if (!a.kv_len) {
+        kt = (int)(tau % a.tiles);
+        hk = (int)(tau / a.tiles % a.Hk);
+        b = (int)(tau / a.tiles / a.Hk);
+        return;
+    }
+    long long base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const int v = b0 + lane < a.B ? live_tiles(a, b0 + lane) : 0;
+        const int inc = lanes_scan(v, lane);
+        const long long tot = __shfl(inc, 63, 64);
+        if (tau < (base + tot) * a.Hk) {
+            // the first sample whose tiles reach beyond tau
+            const int l = __ffsll(__ballot((base + inc) * a.Hk > tau)) - 1;
+            const int vt = __shfl(v, l, 64);
+            const int rest = (int)(tau - (base + __shfl(inc, l, 64) - vt) * a.Hk);
+            b = b0 + l;
+            hk = rest / vt;
+            kt = rest - hk * vt;
+            return;
+        }
+        base += tot;
+    }
+    b = hk = kt = 0;
+}
+// first live tile of (b, hk)
+__device__ __forceinline__ long long stream_first(const XaArgs& a, int b, int hk, int lane) {
+    if (!a.kv_len) return ((long long)b * a.Hk + hk) * a.tiles;
+    long long base = 0;
+    for (int b0 = 0; b0 <= b; b0 += 64)
+        base += __shfl(lanes_scan(b0 + lane < b ? live_tiles(a, b0 + lane) : 0, lane), 63, 64);
+    return base * a.Hk + (long long)hk * live_tiles(a, b);
+}
+
 // dk and dv: four waves of 32 keys over the row tiles of the whole group
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_dkv_kernel(XaArgs a) {
+template <typename T, int DP, bool VEC, bool STREAM>
+__global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xattn_dkv_kernel(XaArgs a) {
     constexpr int QT = Mx<T>::KT, IMG = QT * DP, NF = DP / Mx<T>::KD;
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);                           // Q, dO, Q, dO
     float* const rows = reinterpret_cast<float*>(xa_lds + 4 * IMG * sizeof(T));   // [2][lse, delta][QT]
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    int idx = xa_block();
-    const int kt = idx % a.tiles;
-    idx /= a.tiles;
-    const int split = idx % a.splits;
-    idx /= a.splits;
-    const int hk = idx % a.Hk, b = idx / a.Hk;
-    const int key = kt * 128 + wave * 32 + (lane & 31);
-    const int n = keys_of(a, b);
-    const bool on = key < n && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0);
-    typename Mx<T>::frag kf[NF], vf[NF];
-    {
-        const T* kp = (const T*)a.k + b * a.ks[0] + key * a.ks[1] + hk * a.ks[2];
-        const T* vp = (const T*)a.v + b * a.vs[0] + key * a.vs[1] + hk * a.vs[2];
-#pragma unroll
-        for (int c = 0; c < NF; ++c) {
-            const int d = c * Mx<T>::KD + h * Mx<T>::FE;
-            kf[c] = on ? global_piece<T, VEC>(kp, d, a.D) : zero_frag<T>();
-            vf[c] = on ? global_piece<T, VEC>(vp, d, a.D) : zero_frag<T>();
-        }
+    const int blk = xa_block(), RT = (a.R + QT - 1) / QT;
+    long long u = 0, u1 = 1;                              // not streamed: one key tile a workgroup
+    if (STREAM) {
+        const Stream str = stream_of(a, gridDim.x, RT, lane);
+        if (blk >= str.nb) return;
+        u = str.begin(blk);
+        u1 = str.begin(blk + 1);
     }
-    f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
-    int t0 = 0, t1 = 0;
-    if (__syncthreads_or(on)) split_range((a.R + QT - 1) / QT, a.splits, split, t0, t1);
-    const T* qp = (const T*)a.q + b * a.qs[0] + (long long)hk * a.G * a.qs[2];
-    const T* gp = (const T*)a.dout + b * a.dos[0] + (long long)hk * a.G * a.dos[2];
-    const long long sti = ((long long)b * a.Hk + hk) * a.R;
-    Stage<T, DP, VEC, QT, XA_THREADS, VEC> st;
-    float stat = 0.f;                                     // threads 0..QT-1: lse, QT..2QT-1: delta
-    auto fetch = [&](int tile) {
-        T* img = lds + (tile & 1) * 2 * IMG;
-        st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, img, img + IMG, a.D, t);
-        if (t < 2 * QT) {
-            const int r = tile * QT + (t < QT ? t : t - QT);
-            stat = t < QT ? INFINITY : 0.f;
-            if (r < a.R) stat = t < QT ? a.lse[sti + r] : a.delta[sti + r];
+    int turn = 0;                                         // which of the two image pairs is next
+    for (int part = 0; u < u1; ++part) {
+        int b, hk, kt, t0 = 0, t1 = RT;
+        if (STREAM) {
+            const long long tau = u / RT;
+            t0 = (int)(u - tau * RT);
+            t1 = (int)(t0 + (u1 - u) < RT ? t0 + (u1 - u) : RT);
+            u += t1 - t0;
+            stream_tile(a, tau, lane, b, hk, kt);
+            b = __builtin_amdgcn_readfirstlane(b);
+            hk = __builtin_amdgcn_readfirstlane(hk);
+            kt = __builtin_amdgcn_readfirstlane(kt);
+        } else {
+            kt = blk % a.tiles;
+            hk = blk / a.tiles % a.Hk;
+            b = blk / a.tiles / a.Hk;
+            u = u1;
         }
-    };
-    if (t0 < t1) fetch(t0);
-    for (int qt = t0; qt < t1; ++qt) {
-        T* img = lds + (qt & 1) * 2 * IMG;
-        float* rs = rows + (qt & 1) * 2 * QT;
-        st.store(img, img + IMG, t);
-        if (t < 2 * QT) rs[t] = stat;
-        wait_loads();
-        __syncthreads();
-        if (qt + 1 < t1) fetch(qt + 1);
+        const int key = kt * 128 + wave * 32 + (lane & 31);
+        const int n = keys_of(a, b);
+        const bool on = key < n && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0);
+        typename Mx<T>::frag kf[NF], vf[NF];
+        {
+            const T* kp = (const T*)a.k + b * a.ks[0] + key * a.ks[1] + hk * a.ks[2];
+            const T* vp = (const T*)a.v + b * a.vs[0] + key * a.vs[1] + hk * a.vs[2];
 #pragma unroll
-        for (int qb = 0; qb < QT / 32; ++qb) {
-            f32x16 s, dp;
-            scores<T, DP, QT>(s, img, 32 * qb, kf, lane);
-            scores<T, DP, QT>(dp, img + IMG, 32 * qb, vf, lane);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int q = 32 * qb + key_of<T>(e, h);
-                s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -rs[q]));
-                dp[e] = s[e] * (dp[e] - rs[QT + q]);
-            }
-#pragma unroll
-            for (int g = 0; g < 32 / Mx<T>::KD; ++g) {
-                const typename Mx<T>::frag pf = acc_frag(s, g, T()), df = acc_frag(dp, g, T());
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    mma(dv[d], col_frag<QT>(img + IMG, 32 * qb + g * Mx<T>::KD, d, lane), pf);
-                    mma(dk[d], col_frag<QT>(img, 32 * qb + g * Mx<T>::KD, d, lane), df);
-                }
+            for (int c = 0; c < NF; ++c) {
+                const int d = c * Mx<T>::KD + h * Mx<T>::FE;
+                kf[c] = on ? global_piece<T, VEC>(kp, d, a.D) : zero_frag<T>();
+                vf[c] = on ? global_piece<T, VEC>(vp, d, a.D) : zero_frag<T>();
             }
         }
-    }
-    if (key >= a.Nk) return;
-    if (!on) {                                            // a masked key's lane worked on zeros: its gradients are zero
+        f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
-    }
-    const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
-    if (a.splits == 1) {
-        store_acc<T, VEC, DP>((T*)a.dk + row, dk, a.scale, h, a.D);
-        store_acc<T, VEC, DP>((T*)a.dv + row, dv, 1.f, h, a.D);
-    } else {
-        store_acc<float, VEC, DP>(a.part_dk + split * a.n_k + row, dk, 1.f, h, a.D);
-        store_acc<float, VEC, DP>(a.part_dv + split * a.n_k + row, dv, 1.f, h, a.D);
+        const T* qp = (const T*)a.q + b * a.qs[0] + (long long)hk * a.G * a.qs[2];
+        const T* gp = (const T*)a.dout + b * a.dos[0] + (long long)hk * a.G * a.dos[2];
+        const long long sti = ((long long)b * a.Hk + hk) * a.R;
+        Stage<T, DP, VEC, QT, XA_THREADS, VEC> st;
+        float stat = 0.f;                                 // threads 0..QT-1: lse, QT..2QT-1: delta
+        auto fetch = [&](int tile, int pair) {
+            T* img = lds + pair * 2 * IMG;
+            st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, img, img + IMG, a.D, t);
+            if (t < 2 * QT) {
+                const int r = tile * QT + (t < QT ? t : t - QT);
+                stat = t < QT ? INFINITY : 0.f;
+                if (r < a.R) stat = t < QT ? a.lse[sti + r] : a.delta[sti + r];
+            }
+        };
+        const bool work = __syncthreads_or(on);           // also: every wave has left the images of the part before
+        if (work) {
+            fetch(t0, turn);
+            for (int qt = t0; qt < t1; ++qt, turn ^= 1) {
+                T* img = lds + turn * 2 * IMG;
+                float* rs = rows + turn * 2 * QT;
+                st.store(img, img + IMG, t);
+                if (t < 2 * QT) rs[t] = stat;
+                wait_loads();
+                __syncthreads();
+                if (qt + 1 < t1) fetch(qt + 1, turn ^ 1);
+#pragma unroll
+                for (int qb = 0; qb < QT / 32; ++qb) {
+                    if (qb > 0 && qt * QT + 32 * qb >= a.R) continue;
+                    f32x16 s, dp;
+                    scores<T, DP, QT>(s, img, 32 * qb, kf, lane);
+                    scores<T, DP, QT>(dp, img + IMG, 32 * qb, vf, lane);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int q = 32 * qb + key_of<T>(e, h);
+                        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -rs[q]));
+                        dp[e] = s[e] * (dp[e] - rs[QT + q]);
+                    }
+#pragma unroll
+                    for (int g = 0; g < 32 / Mx<T>::KD; ++g) {
+                        const typename Mx<T>::frag pf = acc_frag(s, g, T()), df = acc_frag(dp, g, T());
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d) {
+                            mma(dv[d], col_frag<QT>(img + IMG, 32 * qb + g * Mx<T>::KD, d, lane), pf);
+                            mma(dk[d], col_frag<QT>(img, 32 * qb + g * Mx<T>::KD, d, lane), df);
+                        }
+                    }
+                }
+            }
+        }
+        if (key >= a.Nk) continue;
+        if (!on) {                                        // a masked key's lane worked on zeros: its gradients are zero
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+        }
+        if (!STREAM || (t0 == 0 && t1 == RT)) {
+            const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
+            store_acc<T, VEC, DP>((T*)a.dk + row, dk, a.scale, h, a.D);
+            store_acc<T, VEC, DP>((T*)a.dv + row, dv, 1.f, h, a.D);
+        } else {                                          // a workgroup's first and its last part may be shares of a tile
+            float* slot = a.part_kv + ((2ll * blk + (part > 0)) * 2 * 128 + wave * 32 + (lane & 31)) * a.D;
+            store_acc<float, VEC, DP>(slot, dk, 1.f, h, a.D);
+            store_acc<float, VEC, DP>(slot + 128ll * a.D, dv, 1.f, h, a.D);
+        }
     }
 }
 
-// out[i] = scale * sum over the splits, in split order; blockIdx.y picks one of two tensors of equal size
+// adds the shares of the key tiles that several workgroups of a streamed dk / dv launch worked on, in workgroup order, and clears
+// the rows of tiles without a live key; 8 keys a workgroup, four shares' loads in flight
 template <typename T>
-__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* p0, T* o0, float f0, const float* p1, T* o1, float f1, long long n,
-                                                        int splits) {
-    const float* p = blockIdx.y ? p1 : p0;
-    T* o = blockIdx.y ? o1 : o0;
-    const float f = blockIdx.y ? f1 : f0;
+__global__ __launch_bounds__(256) void xattn_dkv_join_kernel(XaArgs a, int grid, int row_tiles) {
+    const int lane = threadIdx.x & 63;
+    int idx = blockIdx.x >> 4;
+    const int kt = idx % a.tiles;
+    idx /= a.tiles;
+    const int hk = idx % a.Hk, b = idx / a.Hk;
+    const int k0 = kt * 128 + (blockIdx.x & 15) * 8;
+    if (k0 >= a.Nk) return;
+    const int keys = a.Nk - k0 < 8 ? a.Nk - k0 : 8;
+    const bool live = kt < live_tiles(a, b);
+    int i0 = 0, i1 = -1, part0 = 0;
+    if (live) {
+        const Stream str = stream_of(a, grid, row_tiles, lane);
+        const long long x0 = (stream_first(a, b, hk, lane) + kt) * row_tiles;
+        i0 = str.owner(x0);
+        i1 = str.owner(x0 + row_tiles - 1);
+        if (i0 == i1) return;                             // written in full by one workgroup
+        part0 = str.begin(i0) < x0;                       // the tile is the last, not the first, of that workgroup's share
+    }
+    const bool v4 = a.D % 4 == 0;
+    const int w = v4 ? 4 : 1, per = a.D / w;
+    for (int j = threadIdx.x; j < 2 * keys * per; j += 256) {
+        const int m = j / (keys * per), e = j - m * keys * per, key = e / per, d = (e - key * per) * w;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = i0; i <= i1; i += 4) {
+            float v[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float* p = a.part_kv + (((2ll * (i + c) + (i + c == i0 ? part0 : 0)) * 2 + m) * 128 + (blockIdx.x & 15) * 8 + key) * a.D + d;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[c][q] = 0.f;
+                if (i + c <= i1) {
+                    if (v4) *reinterpret_cast<f32x4*>(v[c]) = *reinterpret_cast<const f32x4*>(p);
+                    else v[c][0] = p[0];
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) s[q] += v[c][q];
+        }
+        const float f = m == 0 ? a.scale : 1.f;
+        T* o = (T*)(m == 0 ? a.dk : a.dv) + (((long long)b * a.Nk + k0 + key) * a.Hk + hk) * a.D + d;
+        for (int q = 0; q < w; ++q) o[q] = from_f32<T>(s[q] * f);
+    }
+}
+
+// out[i] = f * sum over the splits, in split order
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(const float* p, T* o, float f, long long n, int splits) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
         float s = 0.f;
         for (int k = 0; k < splits; ++k) s += p[k * n + i];
@@ -872,7 +1029,7 @@ int xa_width(int D, bool vec) { return !vec ? 128 : D <= 32 ? 32 : D <= 64 ? 64 
 
 struct XaPlan {
     bool few;
-    int fwd_tiles, fwd_splits, dq_tiles, dq_splits, dkv_tiles, dkv_splits;
+    int fwd_tiles, fwd_splits, dq_tiles, dq_splits, dkv_tiles, dkv_rt, dkv_grid;
 };
 
 int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -885,7 +1042,7 @@ int xa_splits(long long blocks, int steps, int least) {
     return (int)std::max<long long>(1, std::min<long long>({want, steps / least, 64}));
 }
 
-XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk) {
+XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     XaPlan p;
     const int R = Hq / Hk * Nq, KT = dt == VITMI_F32 ? 32 : 64;
     const long long bh = (long long)B * Hk;
@@ -894,8 +1051,14 @@ XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk) {
     p.fwd_splits = p.few ? xa_splits(bh * p.fwd_tiles, cdiv(Nk, 32), 8) : xa_splits(bh * p.fwd_tiles, cdiv(Nk, KT), 4);
     p.dq_tiles = cdiv(R, 128);
     p.dq_splits = xa_splits(bh * p.dq_tiles, cdiv(Nk, KT), 4);
+    // dk / dv: a workgroup a key tile where that keeps nine tenths of the chip busy to the end (registers allow three a compute
+    // unit in bf16 with heads up to 64, one in fp32 beyond that, else two), otherwise equal shares, of four row tiles or more
     p.dkv_tiles = cdiv(Nk, 128);
-    p.dkv_splits = xa_splits(bh * p.dkv_tiles, cdiv(R, KT), 4);
+    p.dkv_rt = cdiv(R, KT);
+    const long long tiles = bh * p.dkv_tiles, slots = 256 * (dt == VITMI_F32 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 3 : 2));
+    const bool even = 10 * tiles >= 9 * slots * ((tiles + slots - 1) / slots);
+    const long long grid = std::min<long long>(dt == VITMI_F32 ? slots : 512, tiles * p.dkv_rt / 4);
+    p.dkv_grid = even || p.dkv_rt < 8 || grid <= tiles / 2 ? 0 : (int)grid;
     return p;
 }
 
@@ -923,23 +1086,31 @@ void xa_fill(const vitmi_xattn_args* g, XaArgs* a) {
     a->dout = g->dout;
     a->dq = g->dq; a->dk = g->dk; a->dv = g->dv;
     a->n_q = (long long)g->B * g->Nq * g->Hq * g->D;
-    a->n_k = (long long)g->B * g->Nk * g->Hk * g->D;
+    a->B = g->B;
 }
 
-enum { XK_FWD, XK_FEW, XK_DQ, XK_DKV };
+enum { XK_FWD, XK_FEW, XK_DQ, XK_DKV, XK_DKV_STREAM };
 
 template <typename T, int DP, bool VEC>
 int xa_launch(int kind, const XaArgs& a, long long blocks, hipStream_t s) {
     constexpr size_t tile4 = 4ull * Mx<T>::KT * DP * sizeof(T);
     constexpr size_t few = std::max<size_t>(8ull * 32 * DP * sizeof(T), (4ull * DP * 32 + 256) * sizeof(float));
     constexpr size_t dkv = tile4 + 4ull * Mx<T>::KT * sizeof(float);
-    const size_t lds = kind == XK_FEW ? few : kind == XK_DKV ? dkv : tile4;
+    const size_t lds = kind == XK_FEW ? few : kind >= XK_DKV ? dkv : tile4;
     const void* fn = kind == XK_FWD   ? (const void*)&xattn_fwd_kernel<T, DP, VEC>
                      : kind == XK_FEW ? (const void*)&xattn_few_kernel<T, DP, VEC>
                      : kind == XK_DQ  ? (const void*)&xattn_dq_kernel<T, DP, VEC>
-                                      : (const void*)&xattn_dkv_kernel<T, DP, VEC>;
+                     : kind == XK_DKV ? (const void*)&xattn_dkv_kernel<T, DP, VEC, false>
+                                      : (const void*)&xattn_dkv_kernel<T, DP, VEC, true>;
     if (lds > 64 * 1024) {
-        hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        static std::atomic<unsigned long long> done[XK_DKV_STREAM + 1];      // a bit per device: the attribute is set once
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        const unsigned long long bit = 1ull << (dev & 63);
+        if (e == hipSuccess && (dev > 63 || !(done[kind].load() & bit))) {
+            e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e == hipSuccess && dev <= 63) done[kind].fetch_or(bit);
+        }
         if (e != hipSuccess) return vitmi_hip_fail(e, "vitmi_cross_attn: LDS size");
     }
     VITMI_CHECK_ARG(blocks < (1ll << 32) / XA_THREADS, "vitmi_cross_attn: %lld tiles are beyond one launch", blocks);
@@ -947,7 +1118,8 @@ int xa_launch(int kind, const XaArgs& a, long long blocks, hipStream_t s) {
     if (kind == XK_FWD) hipLaunchKernelGGL((xattn_fwd_kernel<T, DP, VEC>), grid, block, lds, s, a);
     else if (kind == XK_FEW) hipLaunchKernelGGL((xattn_few_kernel<T, DP, VEC>), grid, block, lds, s, a);
     else if (kind == XK_DQ) hipLaunchKernelGGL((xattn_dq_kernel<T, DP, VEC>), grid, block, lds, s, a);
-    else hipLaunchKernelGGL((xattn_dkv_kernel<T, DP, VEC>), grid, block, lds, s, a);
+    else if (kind == XK_DKV) hipLaunchKernelGGL((xattn_dkv_kernel<T, DP, VEC, false>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((xattn_dkv_kernel<T, DP, VEC, true>), grid, block, lds, s, a);
     VITMI_LAUNCH_CHECK("vitmi_cross_attn");
     return VITMI_OK;
 }
@@ -967,12 +1139,12 @@ int xa_run(int kind, int dt, const XaArgs& a, bool vec, long long blocks, hipStr
     return dt == VITMI_F32 ? xa_dispatch<float>(kind, a, vec, blocks, s) : xa_dispatch<bf16_t>(kind, a, vec, blocks, s);
 }
 
-int xa_sum(int dt, const float* p0, void* o0, float f0, const float* p1, void* o1, float f1, long long n, int splits, hipStream_t s) {
-    const dim3 grid((unsigned)std::min<long long>(4096, (n + 255) / 256), o1 ? 2 : 1);
+int xa_sum(int dt, const float* p, void* o, float f, long long n, int splits, hipStream_t s) {
+    const dim3 grid((unsigned)std::min<long long>(4096, (n + 255) / 256));
     if (dt == VITMI_F32)
-        hipLaunchKernelGGL((xattn_sum_kernel<float>), grid, dim3(256), 0, s, p0, (float*)o0, f0, p1, (float*)o1, f1, n, splits);
+        hipLaunchKernelGGL((xattn_sum_kernel<float>), grid, dim3(256), 0, s, p, (float*)o, f, n, splits);
     else
-        hipLaunchKernelGGL((xattn_sum_kernel<bf16_t>), grid, dim3(256), 0, s, p0, (bf16_t*)o0, f0, p1, (bf16_t*)o1, f1, n, splits);
+        hipLaunchKernelGGL((xattn_sum_kernel<bf16_t>), grid, dim3(256), 0, s, p, (bf16_t*)o, f, n, splits);
     VITMI_LAUNCH_CHECK("vitmi_cross_attn(sum)");
     return VITMI_OK;
 }
@@ -982,7 +1154,7 @@ int xa_sum(int dt, const float* p0, void* o0, float f0, const float* p1, void* o
 extern "C" long long vitmi_cross_attn_fwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
     if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
-    const int s = xa_plan(dt, B, Nq, Nk, Hq, Hk).fwd_splits;
+    const int s = xa_plan(dt, B, Nq, Nk, Hq, Hk, D).fwd_splits;
     if (s == 1) return 0;
     const long long rows = (long long)B * Nq * Hq;
     return up256(s * rows * D * 4) + up256(s * rows * 8);
@@ -993,7 +1165,7 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
     if (int rc = xa_check(who, g)) return rc;
     if (g->B == 0 || g->Nq == 0) return VITMI_OK;
     VITMI_CHECK_ARG(g->q && g->o && (g->Nk == 0 || (g->k && g->v)), "%s: null pointer", who);
-    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk);
+    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D);
     VITMI_CHECK_ARG(p.fwd_splits == 1 || workspace, "%s: this shape needs a workspace", who);
     XaArgs a;
     xa_fill(g, &a);
@@ -1020,10 +1192,9 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
 extern "C" long long vitmi_cross_attn_bwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
     if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
-    const XaPlan p = xa_plan(dt, B, Nq, Nk, Hq, Hk);
-    const long long rows = (long long)B * Nq * Hq, keys = (long long)B * Nk * Hk;
-    return up256(rows * 4) + (p.dq_splits > 1 ? up256(p.dq_splits * rows * D * 4) : 0) +
-           (p.dkv_splits > 1 ? 2 * up256(p.dkv_splits * keys * D * 4) : 0);
+    const XaPlan p = xa_plan(dt, B, Nq, Nk, Hq, Hk, D);
+    const long long rows = (long long)B * Nq * Hq;
+    return up256(rows * 4) + (p.dq_splits > 1 ? up256(p.dq_splits * rows * D * 4) : 0) + (long long)p.dkv_grid * 4 * 128 * D * 4;
 }
 
 extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, void* stream) {
@@ -1032,7 +1203,7 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
     VITMI_CHECK_ARG(g->B > 0 && g->Nq > 0 && g->Nk > 0, "%s: nothing to differentiate", who);
     VITMI_CHECK_ARG(g->q && g->k && g->v && g->o && g->dout && g->lse && workspace, "%s: null pointer", who);
     VITMI_CHECK_ARG((g->dk == nullptr) == (g->dv == nullptr), "%s: dk and dv come together", who);
-    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk);
+    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D);
     XaArgs a;
     xa_fill(g, &a);
     const long long rows = (long long)g->B * g->Nq * g->Hq;
@@ -1043,10 +1214,7 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
         a.part_dq = (float*)w;
         w += up256(p.dq_splits * a.n_q * 4);
     }
-    if (p.dkv_splits > 1) {
-        a.part_dk = (float*)w;
-        a.part_dv = (float*)(w + up256(p.dkv_splits * a.n_k * 4));
-    }
+    a.part_kv = (float*)w;
     const bool vec = xa_vec(g);
     hipStream_t s = as_stream(stream);
     ProfScope prof(VITMI_FAM_ATTN_BWD, s, 10.0 * rows * g->Nk * g->D);
@@ -1054,13 +1222,19 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
     a.splits = p.dq_splits;
     if (int rc = xa_run(XK_DQ, g->dt, a, vec, (long long)g->B * g->Hk * a.tiles * a.splits, s)) return rc;
     if (g->dq && a.splits > 1)
-        if (int rc = xa_sum(g->dt, a.part_dq, g->dq, g->scale, nullptr, nullptr, 0.f, a.n_q, a.splits, s)) return rc;
+        if (int rc = xa_sum(g->dt, a.part_dq, g->dq, g->scale, a.n_q, a.splits, s)) return rc;
     if (g->dk) {
         a.tiles = p.dkv_tiles;
-        a.splits = p.dkv_splits;
-        if (int rc = xa_run(XK_DKV, g->dt, a, vec, (long long)g->B * g->Hk * a.tiles * a.splits, s)) return rc;
-        if (a.splits > 1)
-            if (int rc = xa_sum(g->dt, a.part_dk, g->dk, g->scale, a.part_dv, g->dv, 1.f, a.n_k, a.splits, s)) return rc;
+        const long long tiles = (long long)g->B * g->Hk * a.tiles;
+        if (int rc = xa_run(p.dkv_grid ? XK_DKV_STREAM : XK_DKV, g->dt, a, vec, p.dkv_grid ? p.dkv_grid : tiles, s)) return rc;
+        if (p.dkv_grid) {
+            const dim3 grid((unsigned)(16 * tiles));
+            if (g->dt == VITMI_F32)
+                hipLaunchKernelGGL((xattn_dkv_join_kernel<float>), grid, dim3(256), 0, s, a, p.dkv_grid, p.dkv_rt);
+            else
+                hipLaunchKernelGGL((xattn_dkv_join_kernel<bf16_t>), grid, dim3(256), 0, s, a, p.dkv_grid, p.dkv_rt);
+            VITMI_LAUNCH_CHECK(who);
+        }
     }
     return VITMI_OK;
 }

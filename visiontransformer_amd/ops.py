@@ -4,8 +4,10 @@ Every function here moves raw device pointers, shapes and the current HIP stream
 boundary; tensors are allocated by PyTorch's caching allocator.  There is no CPU or eager
 fallback: CPU tensors raise.
 """
+import functools
 import math
 import os
+import struct
 import weakref
 
 import torch
@@ -1630,32 +1632,50 @@ class _NgrArgs(_ct.Structure):
                 ("D", _ct.c_int), ("post", _ct.c_int), ("pre", _ct.c_int), ("res_scale", _ct.c_float), ("eps", _ct.c_float)]
 
 
-class _on_device:
-    """Makes t's device the current one for a launch when it is not already."""
-    __slots__ = ("guard",)
+def _packer(cls):
+    """One struct.pack for all fields of an argument struct: a third of the time that setting them one by one takes."""
+    codes = {_ct.c_void_p: "P", _ct.c_longlong: "q", _ct.c_double: "d", _ct.c_float: "f", _ct.c_int: "i"}
 
-    def __init__(self, t):
-        cur = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-        self.guard = None if t.device.index == cur else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+    def fmt(t):
+        if t in codes:
+            return codes[t]
+        if issubclass(t, _ct.Array):
+            return fmt(t._type_) * t._length_
+        return "".join(fmt(f) for _, f in t._fields_)
+    st = struct.Struct("@" + fmt(cls))
+    assert st.size == _ct.sizeof(cls), cls
+    return st.pack
 
 
-def _same_device(first, *rest):
+_pack_rope, _pack_xattn, _pack_ngr = _packer(_RopeArgs), _packer(_XattnArgs), _packer(_NgrArgs)
+_get_device = _raw_device if _raw_device is not None else torch.cuda.current_device
+
+
+def _call(device, fn, name, *args):
+    """fn(*args, current stream) with `device` as the current one."""
+    if device != _get_device():
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream())
+    else:
+        rc = fn(*args, _stream())
+    if rc:
+        check(rc, name)
+
+
+def _one_device(first, *rest):
+    """The device index that all tensors of a call live on."""
+    d = first.get_device()
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
+            _need_gpu(first, *rest)
             raise ValueError(f"all tensors of a call live on one device, got {first.device} and {t.device}")
+    if d < 0:
+        _need_gpu(first)
+    return d
 
 
-def _builds_graph(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _dense(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _heads4(name, t):
@@ -1665,64 +1685,69 @@ def _heads4(name, t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 or t.numel() == 0 else t.contiguous()
 
 
-def _s3(t):
-    s = t.stride()
-    return s[:3]
-
-
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_NO_TENSOR = (0,) * 10
 
 
-def _rope_launch(xs, outs, pos, sections, log2_base, interleaved, shared, inverse):
-    a = _RopeArgs()
-    B, N, _, DH = xs[0].shape
-    for i, (x, y) in enumerate(zip(xs, outs)):
-        t = a.t[i]
-        t.x, t.y, t.heads = x.data_ptr(), y.data_ptr(), x.shape[2]
-        t.xs[:] = _s3(x)
-        t.ys[:] = _s3(y)
+@functools.lru_cache(maxsize=256)
+def _rope_ladder(sections, base, shared):
+    """(sections, log2 of the bases, pairs) of checked arguments, as the argument struct takes them."""
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= 4 or min(sections) < 1 or sum(sections) > 256:
+        raise ValueError(f"sections {sections}: one to four axes of at least one pair each, at most 256 pairs")
+    bases = base if isinstance(base, tuple) else (base,) * len(sections)
+    if len(bases) != len(sections) or not all(1.0 < b < float("inf") for b in bases):
+        raise ValueError(f"base {base}: one number above 1, or one per axis")
+    if shared and len(set(bases)) > 1:
+        raise ValueError("a shared ladder has one base")
+    pad = 4 - len(sections)
+    return sections, tuple(math.log2(b) for b in bases) + (0.0,) * pad + sections + (0,) * pad + (len(sections),), sum(sections)
+
+
+def _rope_launch(device, xs, outs, pos, ladder, interleaved, shared, inverse):
+    x = xs[0]
+    B, N, H, D = x.shape
+    sx, sy = x.stride(), outs[0].stride()
+    first = (x.data_ptr(), outs[0].data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], H, 0)
+    second = _NO_TENSOR
+    if len(xs) > 1:
+        x, y = xs[1], outs[1]
+        sx, sy = x.stride(), y.stride()
+        second = (x.data_ptr(), y.data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], x.shape[2], 0)
     ps = pos.stride()
-    a.pos = pos.data_ptr()
-    a.pos_stride[:] = ps if pos.dim() == 3 else (0,) + ps
-    n = len(sections)
-    a.log2_base[:n] = log2_base
-    a.sections[:n] = sections
-    a.axes, a.pos_type, a.dt, a.B, a.N, a.DH = n, _POS_TYPES[pos.dtype], _dt(xs[0]), B, N, DH
-    a.interleaved, a.shared_ladder, a.inverse = interleaved, shared, inverse
-    with _on_device(xs[0]):
-        check(lib.vitmi_rope_axes(_ct.addressof(a), _stream()), "vitmi_rope_axes")
-    return outs
+    if len(ps) == 2:
+        ps = (0, ps[0], ps[1])
+    _call(device, lib.vitmi_rope_axes, "vitmi_rope_axes",
+          _pack_rope(*first, *second, pos.data_ptr(), *ps, *ladder, _POS_TYPES[pos.dtype], _DT[x.dtype], B, N, D, interleaved,
+                     shared, inverse, 0))
 
 
 class RopeAxesFn(torch.autograd.Function):
     """The node behind rope_axes; the backward pass is the same launch with the angles turned round."""
 
     @staticmethod
-    def forward(ctx, q, k, pos, sections, log2_base, interleaved, shared):
-        xs = [t for t in (q, k) if t is not None]
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
-        _rope_launch(xs, outs, pos, sections, log2_base, interleaved, shared, False)
+    def forward(ctx, q, k, pos, device, ladder, interleaved, shared):
+        xs = (q,) if k is None else (q, k)
+        outs = tuple(_dense(t) for t in xs)
+        _rope_launch(device, xs, outs, pos, ladder, interleaved, shared, False)
         ctx.save_for_backward(pos)
-        ctx.meta = (sections, log2_base, interleaved, shared, k is not None)
+        ctx.meta = (device, ladder, interleaved, shared)
         ctx.set_materialize_grads(False)
-        return tuple(outs) if k is not None else outs[0]
+        return outs if k is not None else outs[0]
 
     @staticmethod
-    def backward(ctx, *grads):
+    def backward(ctx, dq, dk=None):
         if _PS2 is not None:                # a replay forms no input gradients
-            return tuple(None if g is None else _no_grad_like(g.shape, g.dtype, g.device) for g in grads) + \
-                (None,) * (7 - len(grads))
+            return tuple(None if g is None else _no_grad_like(g.shape, g.dtype, g.device) for g in (dq, dk)) + (None,) * 5
         pos, = ctx.saved_tensors
-        sections, log2_base, interleaved, shared, two = ctx.meta
-        res = [None, None]
-        want = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
-        if want:
-            gs = [_heads4("gradient", grads[i]) for i in want]
-            outs = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in gs]
-            _rope_launch(gs, outs, pos, sections, log2_base, interleaved, shared, True)
-            for i, o in zip(want, outs):
-                res[i] = o
-        return res[0], res[1], None, None, None, None, None
+        device, ladder, interleaved, shared = ctx.meta
+        gs = [None if g is None or not need else _heads4("gradient", g)
+              for g, need in zip((dq, dk), ctx.needs_input_grad)]
+        outs = [None if g is None else _dense(g) for g in gs]
+        live = [i for i in (0, 1) if gs[i] is not None]
+        if live:
+            _rope_launch(device, [gs[i] for i in live], [outs[i] for i in live], pos, ladder, interleaved, shared, True)
+        return outs[0], outs[1], None, None, None, None, None
 
 
 def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladder=False, inplace=False):
@@ -1735,82 +1760,66 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     pos * base^(-p / P).  A pair is dims (p, P + p), or (2p, 2p + 1) with interleaved; dims from 2P on pass through.
     q and k may be strided views (the slots of a packed projection); the results are dense.  inplace rotates q and k
     where they lie, outside of autograd only."""
-    q = _heads4("q", q) if not inplace else q
-    if k is not None:
-        k = _heads4("k", k) if not inplace else k
-        if k.dtype != q.dtype or (k.shape[0], k.shape[1], k.shape[3]) != (q.shape[0], q.shape[1], q.shape[3]):
-            raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in everything but heads")
-    _dt(q)
-    B, N, _, D = q.shape
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= 4 or min(sections) < 1:
-        raise ValueError(f"sections {sections}: one to four axes of at least one pair each")
-    if 2 * sum(sections) > D or sum(sections) > 256:
-        raise ValueError(f"sections {sections} turn {2 * sum(sections)} dims, the head has {D} (at most 256 pairs)")
-    if pos.dtype not in _POS_TYPES:
-        raise TypeError(f"positions are int32, int64 or float32, not {pos.dtype}")
-    if tuple(pos.shape) not in ((N, len(sections)), (B, N, len(sections))):
-        raise ValueError(f"pos {tuple(pos.shape)} must be [{N}, {len(sections)}] or [{B}, {N}, {len(sections)}]")
-    bases = tuple(float(b) for b in base) if isinstance(base, (tuple, list)) else (float(base),) * len(sections)
-    if len(bases) != len(sections) or not all(1.0 < b < float("inf") for b in bases):
-        raise ValueError(f"base {base}: one number above 1, or one per axis")
-    if shared_ladder and len(set(bases)) > 1:
-        raise ValueError("a shared ladder has one base")
-    log2_base = tuple(math.log2(b) for b in bases)
-    _same_device(q, k, pos)
-    xs = [t for t in (q, k) if t is not None]
+    xs = (q,) if k is None else (q, k)
     if inplace:
-        if _builds_graph(q, k):
-            raise RuntimeError("rope_axes(inplace=True) is for tensors outside of autograd")
         for t in xs:
-            if t.dim() != 4 or (t.stride(3) != 1 and D > 1):
+            if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
                 raise ValueError("inplace needs [batch, tokens, heads, head dim] with unit stride over the head dim")
             if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise ValueError("inplace on a broadcast tensor would turn the same memory several times")
+    else:
+        xs = tuple(_heads4(n, t) for n, t in zip("qk", xs))
+    x = xs[0]
+    B, N, _, D = x.shape
+    _dt(x)
+    if k is not None:
+        bk, nk, _, d_k = xs[1].shape
+        if bk != B or nk != N or d_k != D or k.dtype != q.dtype:
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in everything but heads")
+    sections, ladder, pairs = _rope_ladder(tuple(sections), tuple(base) if isinstance(base, list) else base, shared_ladder)
+    if 2 * pairs > D:
+        raise ValueError(f"sections {sections} turn {2 * pairs} dims, the head has {D}")
+    if pos.dtype not in _POS_TYPES:
+        raise TypeError(f"positions are int32, int64 or float32, not {pos.dtype}")
+    ps = tuple(pos.shape)
+    if ps != (N, len(sections)) and ps != (B, N, len(sections)):
+        raise ValueError(f"pos {ps} must be [{N}, {len(sections)}] or [{B}, {N}, {len(sections)}]")
+    graph = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    if inplace:
+        if graph:
+            raise RuntimeError("rope_axes(inplace=True) is for tensors outside of autograd")
         if k is not None and q.data_ptr() == k.data_ptr() and q.numel():
             raise ValueError("inplace needs q and k apart")
-        _need_gpu(q, k, pos)
-        _rope_launch(xs, xs, pos, sections, log2_base, interleaved, shared_ladder, False)
-        for t in xs:
-            torch.autograd.graph.increment_version(t)
-        return (q, k) if k is not None else q
-    _need_gpu(q, k, pos)
-    if _builds_graph(q, k):
-        return RopeAxesFn.apply(q, k, pos, sections, log2_base, interleaved, shared_ladder)
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
-    _rope_launch(xs, outs, pos, sections, log2_base, interleaved, shared_ladder, False)
-    return tuple(outs) if k is not None else outs[0]
+    device = _one_device(q, k, pos)
+    if graph:
+        return RopeAxesFn.apply(x, xs[1] if k is not None else None, pos, device, ladder, interleaved, shared_ladder)
+    outs = xs if inplace else tuple(_dense(t) for t in xs)
+    _rope_launch(device, xs, outs, pos, ladder, interleaved, shared_ladder, False)
+    if inplace:
+        torch.autograd.graph.increment_version(xs)
+        outs = (q, k)
+    return outs if k is not None else outs[0]
 
 
-def _xattn_args(q, k, v, o, kv_len, key_mask, scale, lse):
-    a = _XattnArgs()
-    a.q, a.k, a.v, a.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
-    a.qs[:] = _s3(q)
-    a.ks[:] = _s3(k)
-    a.vs[:] = _s3(v)
-    if kv_len is not None:
-        a.kv_len, a.kv_len_i64 = kv_len.data_ptr(), kv_len.dtype == torch.int64
-    if key_mask is not None:
-        a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    a.dt = _dt(q)
-    a.B, a.Nq, a.Hq, a.D = q.shape
-    a.Nk, a.Hk = k.shape[1], k.shape[2]
-    a.scale = scale
-    return a
-
-
-def _xattn_fwd(q, k, v, kv_len, key_mask, scale, keep_lse):
+def _xattn_pack(q, k, v, o, kv_len, key_mask, scale, lse, do=None, dq=None, dk=None, dv=None):
     B, Nq, Hq, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    o = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=q.device)
+    _, Nk, Hk, _ = k.shape
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    sd = do.stride() if do is not None else (0, 0, 0)
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    return _pack_xattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
+                       ptr(kv_len), ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), ptr(lse), ptr(do), sd[0], sd[1],
+                       sd[2], ptr(dq), ptr(dk), ptr(dv), kv_len is not None and kv_len.dtype == torch.int64, _DT[q.dtype], B, Nq, Nk,
+                       Hq, Hk, D, scale, 0)
+
+
+def _xattn_fwd(device, q, k, v, kv_len, key_mask, scale, keep_lse):
+    B, Nq, Hq, D = q.shape
+    o = _dense(q)
     lse = torch.empty((B, Hq * Nq), dtype=torch.float32, device=q.device) if keep_lse else None
-    a = _xattn_args(q, k, v, o, kv_len, key_mask, scale, lse)
-    with _on_device(q):
-        n = lib.vitmi_cross_attn_fwd_workspace_bytes(a.dt, B, Nq, Nk, Hq, Hk, D)
-        ws = _ws(n, q.device) if n else None
-        check(lib.vitmi_cross_attn_fwd(_ct.addressof(a), _p(ws), _stream()), "vitmi_cross_attn_fwd")
+    n = lib.vitmi_cross_attn_fwd_workspace_bytes(_DT[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D)
+    ws = _ws(n, q.device) if n else None
+    _call(device, lib.vitmi_cross_attn_fwd, "vitmi_cross_attn_fwd", _xattn_pack(q, k, v, o, kv_len, key_mask, scale, lse), _p(ws))
     return o, lse
 
 
@@ -1818,35 +1827,32 @@ class CrossAttnFn(torch.autograd.Function):
     """The node behind cross_attn: keeps q, k, v, the output and a log-sum-exp per row; probabilities are formed again."""
 
     @staticmethod
-    def forward(ctx, q, k, v, kv_len, key_mask, scale):
-        o, lse = _xattn_fwd(q, k, v, kv_len, key_mask, scale, True)
+    def forward(ctx, q, k, v, kv_len, key_mask, scale, device):
+        o, lse = _xattn_fwd(device, q, k, v, kv_len, key_mask, scale, True)
         ctx.save_for_backward(q, k, v, o, lse, kv_len, key_mask)
-        ctx.scale = scale
+        ctx.meta = (scale, device)
         return o
 
     @staticmethod
     def backward(ctx, do):
         q, k, v, o, lse, kv_len, key_mask = ctx.saved_tensors
         if _PS2 is not None:                # a replay forms no input gradients
-            return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None, None, None)
-        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_kv else None
+            return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None,) * 4
+        scale, device = ctx.meta
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+        dq = _dense(q) if need_q else None
+        dk, dv = (_dense(k), _dense(v)) if need_k or need_v else (None, None)
         if q.numel() == 0 or k.numel() == 0:
             for t in (dq, dk, dv):
                 if t is not None:
                     t.zero_()
-            return dq, dk, dv, None, None, None
-        do = _heads4("gradient", do)
-        a = _xattn_args(q, k, v, o, kv_len, key_mask, ctx.scale, lse)
-        a.dout = do.data_ptr()
-        a.dos[:] = _s3(do)
-        a.dq, a.dk, a.dv = _p(dq), _p(dk), _p(dv)
-        with _on_device(q):
-            ws = _ws(lib.vitmi_cross_attn_bwd_workspace_bytes(a.dt, a.B, a.Nq, a.Nk, a.Hq, a.Hk, a.D), q.device)
-            check(lib.vitmi_cross_attn_bwd(_ct.addressof(a), _p(ws), _stream()), "vitmi_cross_attn_bwd")
-        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
+        else:
+            do = _heads4("gradient", do)
+            B, Nq, Hq, D = q.shape
+            ws = _ws(lib.vitmi_cross_attn_bwd_workspace_bytes(_DT[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D), q.device)
+            _call(device, lib.vitmi_cross_attn_bwd, "vitmi_cross_attn_bwd",
+                  _xattn_pack(q, k, v, o, kv_len, key_mask, scale, lse, do, dq, dk, dv), ws.data_ptr())
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
 
 
 def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
@@ -1862,8 +1868,8 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
         raise TypeError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     _dt(q)
     B, Nq, Hq, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    Bk, Nk, Hk, Dk = k.shape
+    if Bk != B or Dk != D or k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [{B}, Nk, Hk, {D}] for q {tuple(q.shape)}")
     if Hk == 0 or Hq == 0 or D == 0 or Hq % Hk:
         raise ValueError(f"{Hq} query heads cannot share {Hk} key heads of {D}")
@@ -1883,41 +1889,32 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
     scale = float(D) ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale {scale} must be positive and finite")
-    _same_device(q, k, v, kv_len, key_mask)
-    _need_gpu(q, k, v, kv_len, key_mask)
-    if _builds_graph(q, k, v):
-        return CrossAttnFn.apply(q, k, v, kv_len, key_mask, scale)
-    return _xattn_fwd(q, k, v, kv_len, key_mask, scale, False)[0]
+    device = _one_device(q, k, v, kv_len, key_mask)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return CrossAttnFn.apply(q, k, v, kv_len, key_mask, scale, device)
+    return _xattn_fwd(device, q, k, v, kv_len, key_mask, scale, False)[0]
 
 
 _NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 
 
-def _ngr_args(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, stats):
+def _ngr_pack(x, u, params, meta, y, h, stats, dy=None, dh=None, grads=(None,) * 7):
+    gate, branch_scale, post_w, post_b, pre_w, pre_b = params
     res_scale, post, pre, eps = meta
-    a = _NgrArgs()
     B, N, D = x.shape
-    a.x, a.u = x.data_ptr(), u.data_ptr()
-    a.xs[:] = x.stride()[:2]
-    a.us[:] = u.stride()[:2]
-    if gate is not None:
-        a.gate, a.gate_dt = gate.data_ptr(), _dt(gate)
-        a.gate_stride = gate.stride(0) if gate.dim() == 2 else 0
-    a.branch_scale, a.post_w, a.post_b, a.pre_w, a.pre_b = (_p(branch_scale), _p(post_w), _p(post_b), _p(pre_w), _p(pre_b))
-    a.stats = _p(stats)
-    a.dt_x, a.dt_u, a.B, a.N, a.D, a.post, a.pre = _dt(x), _dt(u), B, N, D, _NORM_KINDS[post], _NORM_KINDS[pre]
-    a.res_scale, a.eps = res_scale, eps
-    return a
+    sx, su = x.stride(), u.stride()
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    gate_stride = gate.stride(0) if gate is not None and gate.dim() == 2 else 0
+    return _pack_ngr(x.data_ptr(), u.data_ptr(), sx[0], sx[1], su[0], su[1], ptr(y), ptr(h), ptr(gate), gate_stride, ptr(branch_scale),
+                     ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(stats), ptr(dy), ptr(dh), *map(ptr, grads),
+                     0 if gate is None else _DT[gate.dtype], _DT[x.dtype], _DT[u.dtype], B, N, D, post, pre, res_scale, eps)
 
 
-def _ngr_fwd(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, keep):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=u.dtype, device=x.device) if meta[2] is not None else None
+def _ngr_fwd(device, x, u, params, meta, keep):
+    y = _dense(x)
+    h = (_dense(x) if x.dtype == u.dtype else _dense(u)) if meta[2] else None
     stats = torch.empty((4, x.shape[0] * x.shape[1]), dtype=torch.float32, device=x.device) if keep else None
-    a = _ngr_args(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, stats)
-    a.y, a.h = y.data_ptr(), _p(h)
-    with _on_device(x):
-        check(lib.vitmi_norm_gate_residual_fwd(_ct.addressof(a), _stream()), "vitmi_norm_gate_residual_fwd")
+    _call(device, lib.vitmi_norm_gate_residual_fwd, "vitmi_norm_gate_residual_fwd", _ngr_pack(x, u, params, meta, y, h, stats))
     return y, h, stats
 
 
@@ -1925,46 +1922,43 @@ class NormGateResidualFn(torch.autograd.Function):
     """The node behind norm_gate_residual: keeps its inputs and four fp32 statistics a row."""
 
     @staticmethod
-    def forward(ctx, x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta):
-        y, h, stats = _ngr_fwd(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, True)
-        ctx.save_for_backward(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, stats)
-        ctx.meta = meta
+    def forward(ctx, x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, device):
+        params = (gate, branch_scale, post_w, post_b, pre_w, pre_b)
+        y, h, stats = _ngr_fwd(device, x, u, params, meta, True)
+        ctx.save_for_backward(x, u, *params, stats)
+        ctx.meta = (meta, device)
         ctx.set_materialize_grads(False)
         return (y, h) if h is not None else y
 
     @staticmethod
     def backward(ctx, dy, dh=None):
-        x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, stats = ctx.saved_tensors
+        x, u, *params, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         if (_PS is not None or _PS2 is not None) and any(need[i] for i in (2, 4, 5, 6, 7)):
             raise NotImplementedError("per-sample norms of norm_gate_residual's gate and norm parameters")
         if _PS2 is not None:                # a replay forms no input gradients
-            return (_no_grad_like(x.shape, x.dtype, x.device), _no_grad_like(u.shape, u.dtype, u.device)) + (None,) * 7
+            return (_no_grad_like(x.shape, x.dtype, x.device), _no_grad_like(u.shape, u.dtype, u.device)) + (None,) * 8
         if dy is None and dh is None:
-            return (None,) * 9
-
-        def new(i, t, dtype=None):
-            return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device) if need[i] else None
-        dx, du, dgate = new(0, x), new(1, u), new(2, gate)
-        dw = [new(i, t) for i, t in ((4, post_w), (5, post_b), (6, pre_w), (7, pre_b))]
-        grads = [dx, du, dgate, None, *dw, None]
+            return (None,) * 10
+        meta, device = ctx.meta
+        # dx, du, dgate and the norms' parameters; branch_scale has none
+        grads = [_dense(t) if need[i] else None for i, t in ((0, x), (1, u), (2, params[0]), (4, params[2]), (5, params[3]),
+                                                             (6, params[4]), (7, params[5]))]
         if x.numel() == 0:
             for t in grads:
                 if t is not None:
                     t.zero_()
-            return tuple(grads)
-        a = _ngr_args(x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, ctx.meta, stats)
-        dy = dy.contiguous() if dy is not None else None
-        dh = dh.contiguous() if dh is not None else None
-        a.dy, a.dh, a.dx, a.du, a.dgate = _p(dy), _p(dh), _p(dx), _p(du), _p(dgate)
-        a.dpost_w, a.dpost_b, a.dpre_w, a.dpre_b = (_p(t) for t in dw)
-        with _on_device(x):
+        else:
+            dy = dy.contiguous() if dy is not None else None
+            dh = dh.contiguous() if dh is not None else None
             ws = None
-            if dgate is not None or any(t is not None for t in dw):
-                ws = _ws(lib.vitmi_norm_gate_residual_bwd_workspace_bytes(a.B, a.N, a.D, gate is not None and gate.dim() == 2),
-                         x.device)
-            check(lib.vitmi_norm_gate_residual_bwd(_ct.addressof(a), _p(ws), _stream()), "vitmi_norm_gate_residual_bwd")
-        return tuple(grads)
+            if any(t is not None for t in grads[2:]):
+                B, N, D = x.shape
+                gate = params[0]
+                ws = _ws(lib.vitmi_norm_gate_residual_bwd_workspace_bytes(B, N, D, gate is not None and gate.dim() == 2), x.device)
+            _call(device, lib.vitmi_norm_gate_residual_bwd, "vitmi_norm_gate_residual_bwd",
+                  _ngr_pack(x, u, params, meta, None, None, stats, dy, dh, grads), _p(ws))
+        return (*grads[:3], None, *grads[3:], None, None)
 
 
 def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=None, post_weight=None, post_bias=None,
@@ -1982,18 +1976,21 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
     B, N, D = x.shape
     if _dt(x) == BF16 and _dt(u) == F32:
         raise TypeError("a bf16 residual stream takes bf16 branches")
+    _dt(u)
     if not 1 <= D <= 8192:
         raise ValueError(f"rows of {D} are outside 1 .. 8192")
+    vectors = []
     for name, kind, w, b in (("post", post, post_weight, post_bias), ("pre", pre, pre_weight, pre_bias)):
         if kind not in _NORM_KINDS:
             raise ValueError(f'{name}={kind!r}: "layer", "rms" or None')
         for what, t in (("weight", w), ("bias", b)):
-            if t is None:
-                continue
-            if kind is None:
-                raise ValueError(f"{name}_{what} without {name}")
-            if tuple(t.shape) != (D,) or t.dtype != torch.float32:
-                raise ValueError(f"{name}_{what} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
+            if t is not None:
+                if kind is None:
+                    raise ValueError(f"{name}_{what} without {name}")
+                if t.dim() != 1 or t.shape[0] != D or t.dtype != torch.float32:
+                    raise ValueError(f"{name}_{what} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
+                t = t.contiguous()
+            vectors.append(t)
     if gate is not None:
         _dt(gate)
         if tuple(gate.shape) not in ((D,), (B, D)):
@@ -2006,14 +2003,12 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
         if branch_scale.requires_grad:
             raise ValueError("branch_scale is not differentiated")
         branch_scale = branch_scale.contiguous()
-    x, u = (t if t.stride(2) == 1 or D == 1 else t.contiguous() for t in (x, u))
-    post_weight, post_bias, pre_weight, pre_bias = (t if t is None or t.is_contiguous() else t.contiguous()
-                                                    for t in (post_weight, post_bias, pre_weight, pre_bias))
-    meta = (float(res_scale), post, pre, float(eps))
-    _same_device(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias)
-    _need_gpu(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias)
-    if _builds_graph(x, u, gate, post_weight, post_bias, pre_weight, pre_bias):
-        res = NormGateResidualFn.apply(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias, meta)
+    if D > 1:
+        x = x if x.stride(2) == 1 else x.contiguous()
+        u = u if u.stride(2) == 1 else u.contiguous()
+    meta = (float(res_scale), _NORM_KINDS[post], _NORM_KINDS[pre], float(eps))
+    device = _one_device(x, u, gate, branch_scale, *vectors)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, u, gate, *vectors)):
+        res = NormGateResidualFn.apply(x, u, gate, branch_scale, *vectors, meta, device)
         return res if pre is not None else (res, None)
-    y, h, _ = _ngr_fwd(x, u, gate, branch_scale, post_weight, post_bias, pre_weight, pre_bias, meta, False)
-    return y, h
+    return _ngr_fwd(device, x, u, (gate, branch_scale, *vectors), meta, False)[:2]
