@@ -195,6 +195,9 @@ XATTN = [  # B, Nq, Nk, Hq, Hk, D, mask
     (2, 64, 31, 3, 3, 16, "empty"), (1, 65, 64, 1, 1, 80, "len"), (2, 17, 50, 2, 1, 13, "keys"), (1, 3, 700, 2, 2, 1, "len"),
     (2, 300, 1, 1, 1, 64, "none"), (1, 128, 128, 2, 2, 128, "none"), (1, 600, 70, 4, 2, 72, "empty"),
     (1, 2, 4100, 1, 1, 64, "sparse"), (4, 70, 260, 1, 1, 127, "len"),
+    # backward passes with all keys in one workgroup (whole and in row shares) and in equal shares of many tiles
+    (2, 150, 200, 2, 1, 128, "keys"), (1, 700, 100, 1, 1, 64, "none"), (2, 40, 256, 1, 1, 24, "sparse"), (1, 520, 130, 2, 2, 96, "len"),
+    (1, 700, 520, 2, 1, 64, "len"), (3, 300, 900, 4, 2, 96, "len"), (70, 10, 300, 1, 1, 16, "len"), (1, 1030, 260, 1, 1, 128, "sparse"),
 ]
 
 
@@ -215,7 +218,7 @@ def xattn_inputs(case, dtype, seed=0):
         keep[0] = False
     elif mask == "sparse":                                  # whole tiles without a key, one key in the last
         keep = torch.zeros(B, Nk, dtype=torch.bool)
-        keep[:, 70:75] = keep[:, Nk - 1] = True
+        keep[:, min(70, Nk // 3):75] = keep[:, Nk - 1] = True
     return q, kv, do, lens, keep
 
 

@@ -42,7 +42,7 @@ struct XaArgs {
     int len64;
     float* lse;                           // [B, Hk, R], log2 domain; +inf: nothing to attend to
     float *part_o, *part_ml;              // [splits][B, Nq, Hq, D], [splits][B, Hk, R][2]
-    int Nq, Nk, Hq, Hk, G, R, D, splits, tiles;
+    int Nq, Nk, Hq, Hk, G, R, D, splits, tiles, whole;
     float c;                              // scale * log2(e)
     float scale;
     // backward
@@ -53,7 +53,7 @@ struct XaArgs {
     float *part_dq;
     float* part_kv;                       // [workgroups][first, last share][dk, dv][128][D]
     int B;
-    long long n_q;                        // elements of q
+    long long n_q, n_k;                   // elements of q and of k
 };
 
 template <typename T> struct Mx;
@@ -184,6 +184,8 @@ __device__ __forceinline__ int keys_of(const XaArgs& a, int b) {
     const long long n = a.len64 ? ((const long long*)a.kv_len)[b] : (long long)((const int*)a.kv_len)[b];
     return (int)(n < 0 ? 0 : (n > a.Nk ? a.Nk : n));
 }
+// the same for a sample that the whole wave works on, in a scalar register
+__device__ __forceinline__ int keys_of_wave(const XaArgs& a, int b) { return __builtin_amdgcn_readfirstlane(keys_of(a, b)); }
 template <int KT> constexpr unsigned long long full_mask() { return ~0ull >> (64 - KT); }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
@@ -200,25 +202,33 @@ __device__ __forceinline__ unsigned lds_addr(const void* p) {
     return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 
+// query row r of a group is position m of head g; without shared heads there is nothing to divide
+__device__ __forceinline__ void split_row(int Nq, int R, int r, int& g, int& m) {
+    g = 0;
+    if (Nq != R) g = r / Nq;
+    m = r - g * Nq;
+}
+__device__ __forceinline__ void split_row(const XaArgs& a, int r, int& g, int& m) { split_row(a.Nq, a.R, r, g, m); }
+
 // A tile of KT rows of two matrices into their LDS images.  DMA: 16-byte loads that land in LDS without a register between
 // (fetch starts them, they are complete after the next wait on vector memory), 64 lanes filling 1 KB of an image in
-// its own order: with 256 threads a load instruction is one plane, so that a thread keeps one row.  Otherwise: through
+// its own order: a load instruction of 256 threads is PPI planes, so that a thread keeps one row.  Otherwise: through
 // registers, fetched row by row, stored by store().  Rows whose mask bit is off and dims from D on are zeros.
 template <typename T, int DP, bool VEC, int KT, int TH, bool DMA>
 struct Stage {
-    static constexpr int CP = cp_of<T>(), NP = DP / 32, RPI = TH / CP;
+    static constexpr int CP = cp_of<T>(), NP = DP / 32, PPI = TH / (KT * CP) > 0 ? TH / (KT * CP) : 1;
     static constexpr int CPR = NP * CP, IT = DMA ? 1 : KT * CPR / TH;
-    static_assert(DMA ? RPI == KT && VEC : KT * CPR % TH == 0, "a tile is a whole number of pieces per thread");
+    static_assert(DMA ? PPI * KT * CP == TH && NP % PPI == 0 && VEC : KT * CPR % TH == 0, "a tile is a whole number of pieces per thread");
     typename Mx<T>::frag x[IT], y[IT];
     // the thread's row of a tile (DMA), or row of piece i
-    __device__ __forceinline__ static int row_of(int i, int t) { return DMA ? t / CP : (t + i * TH) / CPR; }
+    __device__ __forceinline__ static int row_of(int i, int t) { return DMA ? t % (KT * CP) / CP : (t + i * TH) / CPR; }
     // px / py: start of the row that row_of names, valid where ok
     __device__ __forceinline__ void piece(int i, const T* px, const T* py, bool ok, T* ix, T* iy, int D, int t) {
         if (DMA) {
-            const int r = t / CP, chunk = (t % CP) ^ swz<T>(r);
+            const int r = row_of(0, t), chunk = (t % CP) ^ swz<T>(r);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                const int d = 32 * p + chunk * Mx<T>::FE;
+            for (int p = 0; p < NP; p += PPI) {
+                const int d = 32 * (p + t / (KT * CP)) + chunk * Mx<T>::FE;
                 const bool on = ok && d < D;
                 const void* sx = on ? (const void*)(px + d) : (const void*)xa_zero16;
                 const void* sy = on ? (const void*)(py + d) : (const void*)xa_zero16;
@@ -249,7 +259,9 @@ struct Stage {
                                                T* iy, int D, int t) {
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int r = row0 + row_of(i, t), g = r / Nq, n = r - g * Nq;
+            const int r = row0 + row_of(i, t);
+            int g, n;
+            split_row(Nq, R, r, g, n);
             piece(i, px + n * sx[1] + g * sx[2], py + n * sy[1] + g * sy[2], r < R, ix, iy, D, t);
         }
     }
@@ -397,7 +409,8 @@ __device__ __forceinline__ void store_acc(T* row, const f32x16 (&o)[DP / 32], fl
 
 // element offset of query row r of problem (b, hk) in a dense [B, Nq, Hq, D]
 __device__ __forceinline__ long long dense_row(const XaArgs& a, int b, int hk, int r) {
-    const int g = r / a.Nq, n = r - g * a.Nq;
+    int g, n;
+    split_row(a, r, g, n);
     return (((long long)b * a.Nq + n) * a.Hq + hk * a.G + g) * a.D;
 }
 
@@ -442,7 +455,8 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
     const bool busy = rt * 128 + wave * 32 < a.R;         // the wave has a row; without one it only helps staging
     typename Mx<T>::frag qf[DP / Mx<T>::KD];
     {
-        const int g = r / a.Nq, n = r - g * a.Nq;
+        int g, n;
+        split_row(a, r, g, n);
         const T* qp = (const T*)a.q + b * a.qs[0] + n * a.qs[1] + (hk * a.G + g) * a.qs[2];
 #pragma unroll
         for (int c = 0; c < DP / Mx<T>::KD; ++c)
@@ -454,7 +468,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const int n = keys_of(a, b);
+    const int n = keys_of_wave(a, b);
     const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     int t0, t1;
@@ -508,7 +522,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     idx /= a.splits;
     const int hk = idx % a.Hk, b = idx / a.Hk;
     const int r = rt * 32 + (lane & 31);
-    const int n = keys_of(a, b);
+    const int n = keys_of_wave(a, b);
     const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     int t0, t1;
@@ -521,7 +535,8 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     }
     typename Mx<T>::frag qf[DP / Mx<T>::KD];
     {
-        const int g = r / a.Nq, nn = r - g * a.Nq;
+        int g, nn;
+        split_row(a, r, g, nn);
         const T* qp = (const T*)a.q + b * a.qs[0] + nn * a.qs[1] + (hk * a.G + g) * a.qs[2];
 #pragma unroll
         for (int c = 0; c < DP / Mx<T>::KD; ++c)
@@ -666,7 +681,8 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
     typename Mx<T>::frag qf[NF], gf[NF];
     float lse = INFINITY, delta = 0.f;
     {
-        const int g = r / a.Nq, n = r - g * a.Nq;
+        int g, n;
+        split_row(a, r, g, n);
         const T* qp = (const T*)a.q + b * a.qs[0] + n * a.qs[1] + (hk * a.G + g) * a.qs[2];
         const T* gp = (const T*)a.dout + b * a.dos[0] + n * a.dos[1] + (hk * a.G + g) * a.dos[2];
         const T* op = (const T*)a.o + row;
@@ -688,7 +704,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
-    const int n = keys_of(a, b);
+    const int n = keys_of_wave(a, b);
     const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
     const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     int t0, t1;
@@ -736,6 +752,254 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
     else
         store_acc<float, VEC, DP>(a.part_dq + split * a.n_q + row, acc, 1.f, h, a.D);
 }
+
+// dq, dk and dv of up to 32 NW keys in one launch (bf16): all keys of a problem fit the registers of one workgroup, wave w
+// owning keys 32 w .. with their K and V fragments and their dk and dv, and an image of K in LDS.  The workgroup walks
+// tiles of 32 SUB query rows; S, dP and dS of a tile are formed once (the two-launch form pays for the exponentials twice, and
+// at heads of 64 they take longer than the products) and feed dk and dv as in xattn_dkv_kernel.  Every wave also leaves its dS
+// as [key][row] in LDS -- the packed fragments as they are, two 16-byte writes a lane -- from where the tile's dq^T =
+// K^T dS^T is formed over all keys, in pieces of 32 dims that the waves take in turns, a tile behind (NOW: a piece a wave, at
+// once, which needs one dS image in place of two).  delta is formed from dO and O on the way in.
+template <int DP, int NW, int SUB>
+__global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
+    typedef bf16_t T;
+    constexpr int TH = 64 * NW, NK = 32 * NW, QT = 32 * SUB, NP = DP / 32, NF = DP / 16, IMG = QT * DP, DS = NK * QT;
+    constexpr bool NOW = NP * SUB == NW;
+    constexpr int TPR = TH / QT, NPC = (DP / 8 + TPR - 1) / TPR;
+    extern __shared__ __align__(16) char xa_lds[];
+    T* const kimg = reinterpret_cast<T*>(xa_lds);
+    T* const lds = kimg + NK * DP;                        // Q, dO, Q, dO
+    T* const dsi = lds + 4 * IMG;
+    float* const rows = reinterpret_cast<float*>(dsi + (NOW ? 1 : 2) * DS);     // [2][lse, delta][QT]
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // the first a.whole problems have a workgroup each, the others share their rows among a.splits
+    const int idx = xa_block();
+    const bool shared = idx >= a.whole;
+    const int sh = shared ? (idx - a.whole) / a.splits : 0, split = shared ? (idx - a.whole) - sh * a.splits : 0;
+    const int bh = shared ? a.whole + sh : idx, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int n = keys_of_wave(a, b), RT = (a.R + QT - 1) / QT;
+    int t0, t1;
+    split_range(RT, shared ? a.splits : 1, split, t0, t1);
+    const T* kp = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* vp = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    const T* qp = (const T*)a.q + b * a.qs[0] + (long long)hk * a.G * a.qs[2];
+    const T* gp = (const T*)a.dout + b * a.dos[0] + (long long)hk * a.G * a.dos[2];
+    const long long sti = ((long long)b * a.Hk + hk) * a.R;
+    auto allowed = [&](int key) { return key < n && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0); };
+
+    // 1 KB of an image (16 rows of one plane) a load instruction; a wave keeps 16 of a tile's rows
+    const int lrow = lane >> 2;
+    auto piece = [&](const T* row, bool ok, int plane, int r, T* img, int rows_img, int r0) {
+        const int d = 32 * plane + ((lane & 3) ^ swz<T>(r)) * 8;
+        load_to_lds(ok && d < a.D ? (const void*)(row + d) : (const void*)xa_zero16, lds_addr(img + plane * rows_img * 32 + r0 * 32));
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r0 = 16 * (2 * wave + i), r = r0 + lrow;
+        const bool ok = allowed(r);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) piece(kp + r * a.ks[1], ok, p, r, kimg, NK, r0);
+    }
+    bf16x8 dof[NPC], of[NPC];
+    float lse = INFINITY;
+    auto issue = [&](int tile, int pair) {
+        T* img = lds + pair * 2 * IMG;
+        {
+            const int r0 = 16 * (wave % (2 * SUB)), lr = r0 + lrow, r = tile * QT + lr;
+            int g, m;
+            split_row(a, r, g, m);
+            const T *q = qp + m * a.qs[1] + g * a.qs[2], *d = gp + m * a.dos[1] + g * a.dos[2];
+#pragma unroll
+            for (int u = wave / (2 * SUB); u < 2 * NP; u += NW / (2 * SUB)) {
+                if (u < NP) piece(q, r < a.R, u, lr, img, QT, r0);
+                else piece(d, r < a.R, u - NP, lr, img + IMG, QT, r0);
+            }
+        }
+        const int r = tile * QT + t / TPR;
+        int g, m;
+        split_row(a, r, g, m);
+        const T* d = gp + m * a.dos[1] + g * a.dos[2];
+        const T* o = (const T*)a.o + (((long long)b * a.Nq + m) * a.Hq + hk * a.G + g) * a.D;
+        lse = INFINITY;
+#pragma unroll
+        for (int i = 0; i < NPC; ++i) {
+            const int c = (t % TPR + TPR * i) * 8;
+            dof[i] = of[i] = zero_frag<T>();
+            if (r < a.R && c < a.D) {
+                dof[i] = *reinterpret_cast<const bf16x8*>(d + c);
+                of[i] = *reinterpret_cast<const bf16x8*>(o + c);
+            }
+        }
+        if (r < a.R && t % TPR == 0) lse = a.lse[sti + r];
+    };
+    auto leave_stats = [&](int pair) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NPC; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf(to_f32(dof[i][j]), to_f32(of[i][j]), s);
+#pragma unroll
+        for (int o = 1; o < TPR; o <<= 1) s += __shfl_xor(s, o, 64);
+        if (t % TPR == 0) {
+            rows[pair * 2 * QT + t / TPR] = lse;
+            rows[pair * 2 * QT + QT + t / TPR] = s;
+        }
+    };
+    if (t0 < t1) issue(t0, t0 & 1);
+
+    const int key = wave * 32 + (lane & 31);
+    const bool on = allowed(key);
+    const bool all_on = __all(on), any_on = __any(on);
+    constexpr bool KL = DP == 128;                        // K fragments out of the image: registers for them run out
+    bf16x8 kf[KL ? 1 : NF], vf[NF];
+#pragma unroll
+    for (int c = 0; c < NF; ++c) {
+        if (!KL) kf[KL ? 0 : c] = on ? global_piece<T, true>(kp + key * a.ks[1], c * 16 + h * 8, a.D) : zero_frag<T>();
+        vf[c] = on ? global_piece<T, true>(vp + key * a.vs[1], c * 16 + h * 8, a.D) : zero_frag<T>();
+    }
+    f32x16 dk[NP], dv[NP];
+#pragma unroll
+    for (int d = 0; d < NP; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+    auto ds_at = [&](int pair, int sub, int c) { return reinterpret_cast<bf16x8*>(dsi + (NOW ? 0 : pair * DS) + sub * NK * 32 + img_off<T>(key, c)); };
+    if (!any_on) {                                        // a wave without a key leaves no dS: zeros stand in for it
+#pragma unroll
+        for (int p = 0; p < (NOW ? 1 : 2) * SUB; ++p) *ds_at(p / SUB, p % SUB, 2 * h) = *ds_at(p / SUB, p % SUB, 2 * h + 1) = zero_frag<T>();
+    }
+    const int blocks = (n + 31) >> 5;
+    auto dq_piece = [&](int tile, int sub, int j) {
+        const T* di = dsi + (NOW ? 0 : (tile & 1) * DS) + sub * NK * 32;
+        f32x16 acc, alt;                                  // two chains: one would wait for itself
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] = alt[e] = 0.f;
+#pragma unroll 2
+        for (int kb = 0; kb < blocks; ++kb) {
+            mma(acc, col_frag<NK>(kimg + kb * 1024, 0, j, lane), col_frag<NK>(di + kb * 1024, 0, 0, lane));
+            mma(alt, col_frag<NK>(kimg + kb * 1024, 16, j, lane), col_frag<NK>(di + kb * 1024, 16, 0, lane));
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] += alt[e];
+        const int r = tile * QT + 32 * sub + (lane & 31);
+        if (r < a.R) {
+            T* row = (T*)a.dq + dense_row(a, b, hk, r);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                store4<T, true>(row, 32 * j + 8 * g + 4 * h, a.D, acc[4 * g] * a.scale, acc[4 * g + 1] * a.scale,
+                                acc[4 * g + 2] * a.scale, acc[4 * g + 3] * a.scale);
+        }
+    };
+    // the pieces of a tile's dq go round the waves (left to the waves without a key alone they hold the others up: 104 us for 75
+    // at 32 x 12 heads, 576 rows, 197 keys)
+    auto dq_tile = [&](int tile) {
+        if (a.dq)
+            for (int j = 0; j < NP * SUB; ++j)
+                if ((tile * NP * SUB + j) % NW == wave && 32 * (j % NP) < a.D) dq_piece(tile, j / NP, j % NP);
+    };
+    for (int qt = t0; qt < t1; ++qt) {
+        const int pair = qt & 1;
+        T* img = lds + pair * 2 * IMG;
+        const float* rs = rows + pair * 2 * QT;
+        leave_stats(pair);
+        wait_loads();
+        __syncthreads();
+        if (qt + 1 < t1) issue(qt + 1, pair ^ 1);
+        if (!NOW && qt > t0) dq_tile(qt - 1);
+        if (any_on) {
+            // the sub-tiles' products take turns, so that one's chain runs while the other's waits
+            f32x16 s[SUB], dp[SUB];
+#pragma unroll
+            for (int sub = 0; sub < SUB; ++sub)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[sub][e] = dp[sub][e] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NF; ++c) {
+                const bf16x8 k = KL ? row_frag<T, NK>(kimg, key, c, h) : kf[KL ? 0 : c];
+#pragma unroll
+                for (int sub = 0; sub < SUB; ++sub) {
+                    mma(s[sub], row_frag<T, QT>(img, 32 * sub + key_of_row<T>(lane & 31), c, h), k);
+                    mma(dp[sub], row_frag<T, QT>(img + IMG, 32 * sub + key_of_row<T>(lane & 31), c, h), vf[c]);
+                }
+            }
+#pragma unroll
+            for (int sub = 0; sub < SUB; ++sub) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int q = 32 * sub + key_of<T>(e, h);
+                    s[sub][e] = __builtin_amdgcn_exp2f(fmaf(s[sub][e], a.c, -rs[q]));
+                    dp[sub][e] = dp[sub][e] - rs[QT + q];
+                }
+                if (!all_on) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[sub][e] = on ? s[sub][e] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dp[sub][e] *= s[sub][e];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const bf16x8 pf = acc_frag(s[sub], g, T()), df = acc_frag(dp[sub], g, T());
+                    *ds_at(pair, sub, 2 * g + h) = df;
+#pragma unroll
+                    for (int d = 0; d < NP; ++d) {
+                        mma(dv[d], col_frag<QT>(img + IMG, 32 * sub + 16 * g, d, lane), pf);
+                        mma(dk[d], col_frag<QT>(img, 32 * sub + 16 * g, d, lane), df);
+                    }
+                }
+            }
+        }
+        if (NOW) {
+            __syncthreads();
+            dq_tile(qt);
+        }
+    }
+    if (!NOW && t0 < t1) {
+        __syncthreads();
+        dq_tile(t1 - 1);
+    }
+    if (key >= a.Nk || !a.dk) return;
+    const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
+    if (!shared || a.splits == 1) {
+        store_acc<T, true, DP>((T*)a.dk + row, dk, a.scale, h, a.D);
+        store_acc<T, true, DP>((T*)a.dv + row, dv, 1.f, h, a.D);
+    } else {                                              // [problem][split][dk, dv][Nk][D]
+        float* slot = a.part_kv + ((((long long)sh * a.splits + split) * 2) * a.Nk + key) * a.D;
+        store_acc<float, true, DP>(slot, dk, 1.f, h, a.D);
+        store_acc<float, true, DP>(slot + (long long)a.Nk * a.D, dv, 1.f, h, a.D);
+    }
+}
+
+// adds the shares of the problems from a.whole on, in order: a workgroup takes 4096 elements of one problem's dk and dv
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_short_join_kernel(XaArgs a, int per) {
+    const int sh = blockIdx.x / per, piece = blockIdx.x - sh * per, bh = a.whole + sh, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const long long n = 2ll * a.Nk * a.D;
+    const float* p = a.part_kv + (long long)sh * a.splits * n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long e = piece * 4096ll + (i * 256 + threadIdx.x) * 4;      // D is a multiple of 8: four elements of a row
+        if (e >= n) break;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < a.splits; k0 += 4) {
+            f32x4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (k0 + k < a.splits) v[k] = *reinterpret_cast<const f32x4*>(p + (k0 + k) * n + e);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) s[q] += v[k][q];
+        }
+        const bool second = e >= n / 2;
+        const int r = (int)(second ? e - n / 2 : e), key = r / a.D, d = r - key * a.D;
+        const float f = second ? 1.f : a.scale;
+        store4<T, true>((T*)(second ? a.dv : a.dk) + (((long long)b * a.Nk + key) * a.Hk + hk) * a.D, d, a.D, s[0] * f, s[1] * f, s[2] * f,
+                        s[3] * f);
+    }
+}
+
 
 // How the dk / dv launch cuts its work: a unit is one row tile against one live tile of 128 keys.  Streamed, every workgroup
 // takes an equal share of the units in a row -- the end of one key tile, whole ones, the start of another -- because whole
@@ -813,13 +1077,19 @@ __device__ __forceinline__ long long stream_first(const XaArgs& a, int b, int hk
     return base * a.Hk + (long long)hk * live_tiles(a, b);
 }
 
-// dk and dv: four waves of 32 keys over the row tiles of the whole group
+// dk and dv: four waves of 32 keys over the row tiles of the whole group.  At bf16 heads beyond 96 the accumulators and both
+// operands would take more than the 256 registers that two waves a SIMD have: V then stays in LDS and the row tiles are
+// half as long (4096 rows of 16 heads, 2 x ~4000 keys: 636 us, 655 with part of it in scratch memory).
+template <typename T, int DP, bool VEC> constexpr bool v_in_lds() { return sizeof(T) == 2 && DP == 128 && VEC; }
+template <typename T, int DP, bool VEC> constexpr int row_tile() { return v_in_lds<T, DP, VEC>() ? 32 : Mx<T>::KT; }
 template <typename T, int DP, bool VEC, bool STREAM>
 __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xattn_dkv_kernel(XaArgs a) {
-    constexpr int QT = Mx<T>::KT, IMG = QT * DP, NF = DP / Mx<T>::KD;
+    constexpr int QT = row_tile<T, DP, VEC>(), IMG = QT * DP, NF = DP / Mx<T>::KD;
+    constexpr bool VL = v_in_lds<T, DP, VEC>();
     extern __shared__ __align__(16) char xa_lds[];
     T* const lds = reinterpret_cast<T*>(xa_lds);                           // Q, dO, Q, dO
-    float* const rows = reinterpret_cast<float*>(xa_lds + 4 * IMG * sizeof(T));   // [2][lse, delta][QT]
+    T* const vimg = lds + 4 * IMG;
+    float* const rows = reinterpret_cast<float*>(vimg + (VL ? 128 * DP : 0));   // [2][lse, delta][QT]
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int blk = xa_block(), RT = (a.R + QT - 1) / QT;
@@ -849,9 +1119,9 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
             u = u1;
         }
         const int key = kt * 128 + wave * 32 + (lane & 31);
-        const int n = keys_of(a, b);
+        const int n = keys_of_wave(a, b);
         const bool on = key < n && (!a.key_mask || a.key_mask[b * a.mask_stride + key] != 0);
-        typename Mx<T>::frag kf[NF], vf[NF];
+        typename Mx<T>::frag kf[NF], vf[VL ? 1 : NF];
         {
             const T* kp = (const T*)a.k + b * a.ks[0] + key * a.ks[1] + hk * a.ks[2];
             const T* vp = (const T*)a.v + b * a.vs[0] + key * a.vs[1] + hk * a.vs[2];
@@ -859,7 +1129,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
             for (int c = 0; c < NF; ++c) {
                 const int d = c * Mx<T>::KD + h * Mx<T>::FE;
                 kf[c] = on ? global_piece<T, VEC>(kp, d, a.D) : zero_frag<T>();
-                vf[c] = on ? global_piece<T, VEC>(vp, d, a.D) : zero_frag<T>();
+                if (!VL) vf[VL ? 0 : c] = on ? global_piece<T, VEC>(vp, d, a.D) : zero_frag<T>();
             }
         }
         f32x16 dk[DP / 32], dv[DP / 32];
@@ -883,6 +1153,19 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
         };
         const bool work = __syncthreads_or(on);           // also: every wave has left the images of the part before
         if (work) {
+            if (VL) {                                     // a wave loads the rows that it reads itself
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int vr = wave * 32 + 16 * i + (lane >> 2), vk = kt * 128 + vr;
+                    const bool ok = vk < n && (!a.key_mask || a.key_mask[b * a.mask_stride + vk] != 0);
+                    const T* vp = (const T*)a.v + b * a.vs[0] + vk * a.vs[1] + hk * a.vs[2];
+#pragma unroll
+                    for (int p = 0; p < DP / 32; ++p) {
+                        const int d = 32 * p + ((lane & 3) ^ swz<T>(vr)) * Mx<T>::FE;
+                        load_to_lds(ok && d < a.D ? (const void*)(vp + d) : (const void*)xa_zero16, lds_addr(vimg + (p * 128 + wave * 32 + 16 * i) * 32));
+                    }
+                }
+            }
             fetch(t0, turn);
             for (int qt = t0; qt < t1; ++qt, turn ^= 1) {
                 T* img = lds + turn * 2 * IMG;
@@ -897,7 +1180,16 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
                     if (qb > 0 && qt * QT + 32 * qb >= a.R) continue;
                     f32x16 s, dp;
                     scores<T, DP, QT>(s, img, 32 * qb, kf, lane);
-                    scores<T, DP, QT>(dp, img + IMG, 32 * qb, vf, lane);
+                    if constexpr (VL) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) dp[e] = 0.f;
+#pragma unroll
+                        for (int c = 0; c < NF; ++c)
+                            mma(dp, row_frag<T, QT>(img + IMG, 32 * qb + key_of_row<T>(lane & 31), c, h),
+                                row_frag<T, 128>(vimg, wave * 32 + (lane & 31), c, h));
+                    } else {
+                        scores<T, DP, QT>(dp, img + IMG, 32 * qb, vf, lane);
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int q = 32 * qb + key_of<T>(e, h);
@@ -985,12 +1277,18 @@ __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(XaArgs a, int grid,
     }
 }
 
-// out[i] = f * sum over the splits, in split order
+// o[i] = f * sum over the splits, in split order
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* p, T* o, float f, long long n, int splits) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
         float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += p[k * n + i];
+        for (int k0 = 0; k0 < splits; k0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k0 + k < splits ? p[(k0 + k) * n + i] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
         o[i] = from_f32<T>(s * f);
     }
 }
@@ -1029,7 +1327,7 @@ int xa_width(int D, bool vec) { return !vec ? 128 : D <= 32 ? 32 : D <= 64 ? 64 
 
 struct XaPlan {
     bool few;
-    int fwd_tiles, fwd_splits, dq_tiles, dq_splits, dkv_tiles, dkv_rt, dkv_grid;
+    int fwd_tiles, fwd_splits, dq_tiles, dq_splits, dkv_tiles, dkv_rt, dkv_grid, short_splits, short_whole;
 };
 
 int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -1042,19 +1340,27 @@ int xa_splits(long long blocks, int steps, int least) {
     return (int)std::max<long long>(1, std::min<long long>({want, steps / least, 64}));
 }
 
-XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
+XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D, bool vec) {
     XaPlan p;
     const int R = Hq / Hk * Nq, KT = dt == VITMI_F32 ? 32 : 64;
     const long long bh = (long long)B * Hk;
     p.few = R <= 64;
     p.fwd_tiles = cdiv(R, p.few ? 32 : 128);
     p.fwd_splits = p.few ? xa_splits(bh * p.fwd_tiles, cdiv(Nk, 32), 8) : xa_splits(bh * p.fwd_tiles, cdiv(Nk, KT), 4);
+    // all keys in one workgroup (bf16; two of four waves a compute unit, one of eight): the problems of a last round that would
+    // leave half of the chip or more idle share their rows, eight tiles of 32 each
+    p.short_splits = p.short_whole = 0;
+    if (dt == VITMI_BF16 && vec && Nk <= 256) {
+        const long long slots = Nk > 128 ? 256 : 512, rest = bh % slots;
+        p.short_splits = rest == 0 ? 1 : (int)std::max<long long>(1, std::min<long long>({slots / rest, cdiv(R, 32) / 8, 64}));
+        p.short_whole = (int)(p.short_splits > 1 ? bh - rest : bh);
+    }
     p.dq_tiles = cdiv(R, 128);
     p.dq_splits = xa_splits(bh * p.dq_tiles, cdiv(Nk, KT), 4);
     // dk / dv: a workgroup a key tile where that keeps nine tenths of the chip busy to the end (registers allow three a compute
     // unit in bf16 with heads up to 64, one in fp32 beyond that, else two), otherwise equal shares, of four row tiles or more
     p.dkv_tiles = cdiv(Nk, 128);
-    p.dkv_rt = cdiv(R, KT);
+    p.dkv_rt = cdiv(R, dt == VITMI_BF16 && D > 96 && vec ? row_tile<bf16_t, 128, true>() : KT);
     const long long tiles = bh * p.dkv_tiles, slots = 256 * (dt == VITMI_F32 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 3 : 2));
     const bool even = 10 * tiles >= 9 * slots * ((tiles + slots - 1) / slots);
     const long long grid = std::min<long long>(dt == VITMI_F32 ? slots : 512, tiles * p.dkv_rt / 4);
@@ -1087,6 +1393,20 @@ void xa_fill(const vitmi_xattn_args* g, XaArgs* a) {
     a->dq = g->dq; a->dk = g->dk; a->dv = g->dv;
     a->n_q = (long long)g->B * g->Nq * g->Hq * g->D;
     a->B = g->B;
+    a->n_k = (long long)g->B * g->Nk * g->Hk * g->D;
+}
+
+// more than 64 KB of LDS a workgroup is asked for once per kernel and device (a bit of *done each)
+int xa_need_lds(const void* fn, size_t lds, std::atomic<unsigned long long>* done) {
+    if (lds <= 64 * 1024) return VITMI_OK;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (e == hipSuccess && (dev > 63 || !(done->load() & bit))) {
+        e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e == hipSuccess && dev <= 63) done->fetch_or(bit);
+    }
+    return e == hipSuccess ? VITMI_OK : vitmi_hip_fail(e, "vitmi_cross_attn: LDS size");
 }
 
 enum { XK_FWD, XK_FEW, XK_DQ, XK_DKV, XK_DKV_STREAM };
@@ -1095,24 +1415,15 @@ template <typename T, int DP, bool VEC>
 int xa_launch(int kind, const XaArgs& a, long long blocks, hipStream_t s) {
     constexpr size_t tile4 = 4ull * Mx<T>::KT * DP * sizeof(T);
     constexpr size_t few = std::max<size_t>(8ull * 32 * DP * sizeof(T), (4ull * DP * 32 + 256) * sizeof(float));
-    constexpr size_t dkv = tile4 + 4ull * Mx<T>::KT * sizeof(float);
+    constexpr size_t dkv = (4ull * row_tile<T, DP, VEC>() + (v_in_lds<T, DP, VEC>() ? 128 : 0)) * DP * sizeof(T) + 4ull * row_tile<T, DP, VEC>() * sizeof(float);
     const size_t lds = kind == XK_FEW ? few : kind >= XK_DKV ? dkv : tile4;
     const void* fn = kind == XK_FWD   ? (const void*)&xattn_fwd_kernel<T, DP, VEC>
                      : kind == XK_FEW ? (const void*)&xattn_few_kernel<T, DP, VEC>
                      : kind == XK_DQ  ? (const void*)&xattn_dq_kernel<T, DP, VEC>
                      : kind == XK_DKV ? (const void*)&xattn_dkv_kernel<T, DP, VEC, false>
                                       : (const void*)&xattn_dkv_kernel<T, DP, VEC, true>;
-    if (lds > 64 * 1024) {
-        static std::atomic<unsigned long long> done[XK_DKV_STREAM + 1];      // a bit per device: the attribute is set once
-        int dev = 0;
-        hipError_t e = hipGetDevice(&dev);
-        const unsigned long long bit = 1ull << (dev & 63);
-        if (e == hipSuccess && (dev > 63 || !(done[kind].load() & bit))) {
-            e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-            if (e == hipSuccess && dev <= 63) done[kind].fetch_or(bit);
-        }
-        if (e != hipSuccess) return vitmi_hip_fail(e, "vitmi_cross_attn: LDS size");
-    }
+    static std::atomic<unsigned long long> done[XK_DKV_STREAM + 1];
+    if (int rc = xa_need_lds(fn, lds, &done[kind])) return rc;
     VITMI_CHECK_ARG(blocks < (1ll << 32) / XA_THREADS, "vitmi_cross_attn: %lld tiles are beyond one launch", blocks);
     const dim3 grid((unsigned)blocks), block(XA_THREADS);
     if (kind == XK_FWD) hipLaunchKernelGGL((xattn_fwd_kernel<T, DP, VEC>), grid, block, lds, s, a);
@@ -1149,12 +1460,39 @@ int xa_sum(int dt, const float* p, void* o, float f, long long n, int splits, hi
     return VITMI_OK;
 }
 
+template <int DP, int NW>
+int xa_launch_short(const XaArgs& a, long long blocks, hipStream_t s) {
+    // 64 rows a tile where LDS holds them (128 KB beside eight waves of heads up to 64): half the barriers
+    constexpr int SUB = NW == 8 && DP <= 64 ? 2 : 1, QT = 32 * SUB;
+    constexpr size_t lds = (32ull * NW * DP + 4ull * QT * DP + (DP / 32 * SUB == NW ? 1 : 2) * 32ull * NW * QT) * 2 + 4 * QT * sizeof(float);
+    const void* fn = (const void*)&xattn_bwd_short_kernel<DP, NW, SUB>;
+    static std::atomic<unsigned long long> done;
+    if (int rc = xa_need_lds(fn, lds, &done)) return rc;
+    VITMI_CHECK_ARG(blocks < (1ll << 32) / (64 * NW), "vitmi_cross_attn: %lld problems are beyond one launch", blocks);
+    hipLaunchKernelGGL((xattn_bwd_short_kernel<DP, NW, SUB>), dim3((unsigned)blocks), dim3(64 * NW), lds, s, a);
+    VITMI_LAUNCH_CHECK("vitmi_cross_attn(short)");
+    return VITMI_OK;
+}
+int xa_run_short(const XaArgs& a, long long blocks, hipStream_t s) {
+    const int w = xa_width(a.D, true);
+    if (a.Nk <= 128) {
+        if (w == 32) return xa_launch_short<32, 4>(a, blocks, s);
+        if (w == 64) return xa_launch_short<64, 4>(a, blocks, s);
+        if (w == 96) return xa_launch_short<96, 4>(a, blocks, s);
+        return xa_launch_short<128, 4>(a, blocks, s);
+    }
+    if (w == 32) return xa_launch_short<32, 8>(a, blocks, s);
+    if (w == 64) return xa_launch_short<64, 8>(a, blocks, s);
+    if (w == 96) return xa_launch_short<96, 8>(a, blocks, s);
+    return xa_launch_short<128, 8>(a, blocks, s);
+}
+
 }  // namespace
 
 extern "C" long long vitmi_cross_attn_fwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
     if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
-    const int s = xa_plan(dt, B, Nq, Nk, Hq, Hk, D).fwd_splits;
+    const int s = xa_plan(dt, B, Nq, Nk, Hq, Hk, D, true).fwd_splits;
     if (s == 1) return 0;
     const long long rows = (long long)B * Nq * Hq;
     return up256(s * rows * D * 4) + up256(s * rows * 8);
@@ -1165,7 +1503,8 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
     if (int rc = xa_check(who, g)) return rc;
     if (g->B == 0 || g->Nq == 0) return VITMI_OK;
     VITMI_CHECK_ARG(g->q && g->o && (g->Nk == 0 || (g->k && g->v)), "%s: null pointer", who);
-    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D);
+    const bool vec = xa_vec(g);
+    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D, vec);
     VITMI_CHECK_ARG(p.fwd_splits == 1 || workspace, "%s: this shape needs a workspace", who);
     XaArgs a;
     xa_fill(g, &a);
@@ -1177,7 +1516,7 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
     hipStream_t s = as_stream(stream);
     ProfScope prof(VITMI_FAM_ATTN_FWD, s, 4.0 * rows * g->Nk * g->D);
     const long long blocks = (long long)g->B * g->Hk * a.tiles * a.splits;
-    if (int rc = xa_run(p.few ? XK_FEW : XK_FWD, g->dt, a, xa_vec(g), blocks, s)) return rc;
+    if (int rc = xa_run(p.few ? XK_FEW : XK_FWD, g->dt, a, vec, blocks, s)) return rc;
     if (a.splits > 1) {
         const dim3 grid((unsigned)((rows + 3) / 4));
         if (g->dt == VITMI_F32)
@@ -1192,9 +1531,16 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
 extern "C" long long vitmi_cross_attn_bwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
     if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
-    const XaPlan p = xa_plan(dt, B, Nq, Nk, Hq, Hk, D);
     const long long rows = (long long)B * Nq * Hq;
-    return up256(rows * 4) + (p.dq_splits > 1 ? up256(p.dq_splits * rows * D * 4) : 0) + (long long)p.dkv_grid * 4 * 128 * D * 4;
+    long long most = 0;
+    for (bool vec : {false, true}) {                      // room for either alignment of the operands
+        const XaPlan p = xa_plan(dt, B, Nq, Nk, Hq, Hk, D, vec);
+        const long long n = vec && p.short_splits
+                                ? ((long long)B * Hk - p.short_whole) * p.short_splits * 2 * Nk * D * 4
+                                : up256(rows * 4) + (p.dq_splits > 1 ? up256(p.dq_splits * rows * D * 4) : 0) + (long long)p.dkv_grid * 4 * 128 * D * 4;
+        most = std::max(most, n);
+    }
+    return std::max(most, 256ll);
 }
 
 extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, void* stream) {
@@ -1203,10 +1549,26 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
     VITMI_CHECK_ARG(g->B > 0 && g->Nq > 0 && g->Nk > 0, "%s: nothing to differentiate", who);
     VITMI_CHECK_ARG(g->q && g->k && g->v && g->o && g->dout && g->lse && workspace, "%s: null pointer", who);
     VITMI_CHECK_ARG((g->dk == nullptr) == (g->dv == nullptr), "%s: dk and dv come together", who);
-    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D);
+    const bool vec = xa_vec(g);
+    const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D, vec);
     XaArgs a;
     xa_fill(g, &a);
     const long long rows = (long long)g->B * g->Nq * g->Hq;
+    hipStream_t s = as_stream(stream);
+    ProfScope prof(VITMI_FAM_ATTN_BWD, s, 10.0 * rows * g->Nk * g->D);
+    if (p.short_splits) {
+        a.splits = p.short_splits;
+        a.whole = p.short_whole;
+        a.part_kv = (float*)workspace;
+        const long long shared = (long long)g->B * g->Hk - a.whole;
+        if (int rc = xa_run_short(a, a.whole + shared * a.splits, s)) return rc;
+        if (g->dk && shared > 0) {
+            const int per = cdiv(2ll * g->Nk * g->D, 4096);
+            hipLaunchKernelGGL((xattn_short_join_kernel<bf16_t>), dim3((unsigned)(shared * per)), dim3(256), 0, s, a, per);
+            VITMI_LAUNCH_CHECK(who);
+        }
+        return VITMI_OK;
+    }
     char* w = (char*)workspace;
     a.delta = (float*)w;
     w += up256(rows * 4);
@@ -1215,9 +1577,6 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
         w += up256(p.dq_splits * a.n_q * 4);
     }
     a.part_kv = (float*)w;
-    const bool vec = xa_vec(g);
-    hipStream_t s = as_stream(stream);
-    ProfScope prof(VITMI_FAM_ATTN_BWD, s, 10.0 * rows * g->Nk * g->D);
     a.tiles = p.dq_tiles;
     a.splits = p.dq_splits;
     if (int rc = xa_run(XK_DQ, g->dt, a, vec, (long long)g->B * g->Hk * a.tiles * a.splits, s)) return rc;
