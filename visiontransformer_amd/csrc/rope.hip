@@ -5,7 +5,8 @@
 //     y1 = x1 cos(theta) - x2 sin(theta),   y2 = x2 cos(theta) + x1 sin(theta),
 // the pair being dims (p, P + p) or (2p, 2p + 1); dims from 2P on pass through.  The backward pass is the same with -theta.
 //
-// Bound by HBM: every element is read once and written once, three operations each.  A workgroup takes a tile of
+// Bound by HBM: every element is read once and written once, three operations each (256 x 197 tokens of 24 bf16 heads of 64:
+// 62 us a pass, 5.0 TB/s; 2 x 21601 of 20 fp32 heads of 80: 103 us, 5.4 TB/s).  A workgroup takes a tile of
 // tokens of one sample and ALL heads of both tensors, so that the angles of a token (the only expensive arithmetic) are
 // formed once per tile and shared by the heads through LDS; its first row loads are on their way meanwhile.
 // The angle is formed in turns in 64 bits and reduced to an eighth of a turn there -- a far position times a frequency
@@ -30,10 +31,9 @@ struct RopeArgs {
     long long ps[3];          // batch, token, axis strides
     double log2_base[4];
     int first_pair[5];        // first pair of each axis; [axes] = P
-    int axes, pos_type, P, DH, B, N, tile, tiles;
-    int group;                // samples a workgroup takes with one set of angles (positions shared by the batch)
-    unsigned div_tok, div_head;
-    int units_tok, units_0;   // units per token, of which the first tensor's
+    int axes, pos_type, P, DH, N, tile, tiles;
+    unsigned div_tok[2], div_head;
+    int units_tok[2];         // units per token of each tensor
     int units_head, units_rot;
     int copy_rest;            // the pass-through dims are copied (not in place)
     int shared, inverse;
@@ -51,9 +51,8 @@ enum { ROPE_HALVES = 0, ROPE_INTER = 1, ROPE_INTER_SCALAR = 2 };
 template <typename T, int V, int MODE>
 struct RopeUnit {
     RVec<T, MODE == ROPE_INTER ? 2 * V : V> a, b;
-    long long out;            // element offset of the unit's first vector in y
-    int tok, pair;            // pair < 0: a pass-through unit (vector a only)
-    int which;                // 0 / 1: tensor; -1: no unit
+    T* y;                     // the unit's first vector in the output; NULL: no unit
+    int cs;                   // where its angles start; < 0: a pass-through unit (vector a only)
 };
 
 // n / d for n, d < 2^16 with m = ceil(2^32 / d): a division would cost more than the rest of a unit's addressing
@@ -76,35 +75,29 @@ __device__ __forceinline__ float2 rope_cos_sin(double turns) {
     return (k & 2) ? make_float2(-c1, -s1) : make_float2(c1, s1);
 }
 
-template <typename T, int V, int MODE>
-__device__ __forceinline__ void rope_fetch(const RopeArgs& a, RopeUnit<T, V, MODE>& r, int u, int total, int b, int n0) {
-    r.which = -1;
+// unit u of a tile of tensor W, whose first token's rows start at x and y
+template <typename T, int V, int MODE, int W>
+__device__ __forceinline__ void rope_fetch(const RopeArgs& a, RopeUnit<T, V, MODE>& r, int u, int total, const T* x, T* y) {
+    r.y = nullptr;
     if (u >= total) return;
-    const int tok = div16(u, a.div_tok);
-    int rem = u - tok * a.units_tok;
-    const int w = rem >= a.units_0;
-    if (w) rem -= a.units_0;
+    const int tok = div16(u, a.div_tok[W]), rem = u - tok * a.units_tok[W];
     const int head = div16(rem, a.div_head), c = rem - head * a.units_head;
-    const RopeTensor& t = w ? a.t[1] : a.t[0];
-    constexpr int W = MODE == ROPE_INTER ? 2 * V : V;
+    constexpr int N = MODE == ROPE_INTER ? 2 * V : V;
     const bool rot = c < a.units_rot;
-    const int d = rot ? c * (MODE == ROPE_HALVES ? V : 2 * V) : 2 * a.P + (c - a.units_rot) * W;
-    const T* x = (const T*)t.x + b * t.xs[0] + (n0 + tok) * t.xs[1] + head * t.xs[2] + d;
-    r.out = b * t.ys[0] + (n0 + tok) * t.ys[1] + head * t.ys[2] + d;
-    r.which = w;
-    r.tok = tok;
-    r.pair = rot ? c * V : -1;
-    r.a = *reinterpret_cast<const RVec<T, W>*>(x);
-    if (MODE != ROPE_INTER && rot) r.b = *reinterpret_cast<const RVec<T, W>*>(x + (MODE == ROPE_HALVES ? a.P : 1));
+    const int d = rot ? c * (MODE == ROPE_HALVES ? V : 2 * V) : 2 * a.P + (c - a.units_rot) * N;
+    x += tok * a.t[W].xs[1] + head * a.t[W].xs[2] + d;
+    r.y = y + tok * a.t[W].ys[1] + head * a.t[W].ys[2] + d;
+    r.cs = rot ? tok * a.P + c * V : -1;
+    r.a = *reinterpret_cast<const RVec<T, N>*>(x);
+    if (MODE != ROPE_INTER && rot) r.b = *reinterpret_cast<const RVec<T, N>*>(x + (MODE == ROPE_HALVES ? a.P : 1));
 }
 
 template <typename T, int V, int MODE>
 __device__ __forceinline__ void rope_finish(const RopeArgs& a, RopeUnit<T, V, MODE>& r, const float2* cs) {
-    if (r.which < 0) return;
-    constexpr int W = MODE == ROPE_INTER ? 2 * V : V;
-    T* y = (T*)(r.which ? a.t[1].y : a.t[0].y) + r.out;
-    if (r.pair >= 0) {
-        const float2* w = cs + r.tok * a.P + r.pair;
+    if (!r.y) return;
+    constexpr int N = MODE == ROPE_INTER ? 2 * V : V;
+    if (r.cs >= 0) {
+        const float2* w = cs + r.cs;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float2 t = w[j];
@@ -114,9 +107,24 @@ __device__ __forceinline__ void rope_finish(const RopeArgs& a, RopeUnit<T, V, MO
             e1 = from_f32<T>(p * t.x - q * t.y);
             e2 = from_f32<T>(q * t.x + p * t.y);
         }
-        if (MODE != ROPE_INTER) *reinterpret_cast<RVec<T, W>*>(y + (MODE == ROPE_HALVES ? a.P : 1)) = r.b;
+        if (MODE != ROPE_INTER) *reinterpret_cast<RVec<T, N>*>(r.y + (MODE == ROPE_HALVES ? a.P : 1)) = r.b;
     }
-    *reinterpret_cast<RVec<T, W>*>(y) = r.a;
+    *reinterpret_cast<RVec<T, N>*>(r.y) = r.a;
+}
+
+// units from `first` on of one sample's tile, K a thread in flight
+template <typename T, int V, int MODE, int W, int K>
+__device__ __forceinline__ void rope_walk(const RopeArgs& a, RopeUnit<T, V, MODE> (&r)[K], int first, int toks, int b, int n0, const float2* cs) {
+    const RopeTensor& t = a.t[W];
+    const int total = toks * a.units_tok[W];
+    const T* x = (const T*)t.x + b * t.xs[0] + n0 * t.xs[1];
+    T* y = (T*)t.y + b * t.ys[0] + n0 * t.ys[1];
+    for (int u = first; u < total; u += K * ROPE_THREADS) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) rope_fetch<T, V, MODE, W>(a, r[i], u + i * ROPE_THREADS, total, x, y);
+#pragma unroll
+        for (int i = 0; i < K; ++i) rope_finish<T, V, MODE>(a, r[i], cs);
+    }
 }
 
 template <typename T, int V, int MODE>
@@ -124,42 +132,37 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(RopeArgs a) {
     extern __shared__ double rope_lds[];
     double* freq = rope_lds;                                   // [P] turns per position step
     float2* cs = reinterpret_cast<float2*>(rope_lds + a.P);     // [tile][P]
-    const int grp = blockIdx.x / a.tiles, n0 = (blockIdx.x - grp * a.tiles) * a.tile;
-    const int b0 = grp * a.group, b1 = min(b0 + a.group, a.B);
-    const int toks = min(a.tile, a.N - n0);
-    const int total = toks * a.units_tok;
+    const int b = blockIdx.x / a.tiles, n0 = (blockIdx.x - b * a.tiles) * a.tile;
+    const int toks = min(a.tile, a.N - n0), t = threadIdx.x;
     constexpr int K = 3;
     RopeUnit<T, V, MODE> r[K];
+    {
+        const T* x = (const T*)a.t[0].x + b * a.t[0].xs[0] + n0 * a.t[0].xs[1];
+        T* y = (T*)a.t[0].y + b * a.t[0].ys[0] + n0 * a.t[0].ys[1];
 #pragma unroll
-    for (int i = 0; i < K; ++i) rope_fetch<T, V, MODE>(a, r[i], (int)threadIdx.x + i * ROPE_THREADS, total, b0, n0);
-
-    if ((int)threadIdx.x < a.P) {
-        const int p = threadIdx.x;
+        for (int i = 0; i < K; ++i) rope_fetch<T, V, MODE, 0>(a, r[i], t + i * ROPE_THREADS, toks * a.units_tok[0], x, y);
+    }
+    if (t < a.P) {
         int ax = 0;
-        while (p >= a.first_pair[ax + 1]) ++ax;
-        const double e = a.shared ? (double)p / a.P
-                                  : (double)(p - a.first_pair[ax]) / (a.first_pair[ax + 1] - a.first_pair[ax]);
-        freq[p] = exp2(-e * a.log2_base[ax]) * 0.15915494309189533577;   // 1 / (2 pi)
+        while (t >= a.first_pair[ax + 1]) ++ax;
+        const double e = a.shared ? (double)t / a.P
+                                  : (double)(t - a.first_pair[ax]) / (a.first_pair[ax + 1] - a.first_pair[ax]);
+        freq[t] = exp2(-e * a.log2_base[ax]) * 0.15915494309189533577;   // 1 / (2 pi)
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < toks * a.P; i += ROPE_THREADS) {
+    for (int i = t; i < toks * a.P; i += ROPE_THREADS) {
         const int tok = i / a.P, p = i - tok * a.P;
         int ax = 0;
         while (p >= a.first_pair[ax + 1]) ++ax;
-        float2 w = rope_cos_sin(rope_pos(a, b0 * a.ps[0] + (n0 + tok) * a.ps[1] + ax * a.ps[2]) * freq[p]);
+        float2 w = rope_cos_sin(rope_pos(a, b * a.ps[0] + (n0 + tok) * a.ps[1] + ax * a.ps[2]) * freq[p]);
         if (a.inverse) w.y = -w.y;
         cs[i] = w;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < K; ++i) rope_finish<T, V, MODE>(a, r[i], cs);
-    for (int b = b0; b < b1; ++b)
-        for (int u = (int)threadIdx.x + (b == b0 ? K * ROPE_THREADS : 0); u < total; u += K * ROPE_THREADS) {
-#pragma unroll
-            for (int i = 0; i < K; ++i) rope_fetch<T, V, MODE>(a, r[i], u + i * ROPE_THREADS, total, b, n0);
-#pragma unroll
-            for (int i = 0; i < K; ++i) rope_finish<T, V, MODE>(a, r[i], cs);
-        }
+    rope_walk<T, V, MODE, 0, K>(a, r, t + K * ROPE_THREADS, toks, b, n0, cs);
+    if (a.t[1].x) rope_walk<T, V, MODE, 1, K>(a, r, t, toks, b, n0, cs);
 }
 
 template <typename T>
@@ -250,24 +253,24 @@ extern "C" int vitmi_rope_axes(const vitmi_rope_args* a, void* stream) {
     k.units_rot = P / V;
     const int rest = (a->DH - 2 * P) / (mode == ROPE_INTER ? 2 * V : V);
     k.units_head = k.units_rot + (in_place ? 0 : rest);
-    const long long ut = heads * k.units_head;
-    VITMI_CHECK_ARG(ut < 65536, "vitmi_rope_axes: %lld heads of %d are beyond one call", heads, a->DH);
-    k.units_tok = (int)ut;
-    k.units_0 = a->t[0].heads * k.units_head;
     auto magic = [](int d) { return d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); };
-    k.div_tok = magic(k.units_tok);
+    long long ut = 1;                 // the larger tensor's units per token
+    for (int i = 0; i < nt; ++i) {
+        const long long n = (long long)a->t[i].heads * k.units_head;
+        VITMI_CHECK_ARG(n < 65536, "vitmi_rope_axes: %d heads of %d are beyond one call", a->t[i].heads, a->DH);
+        k.units_tok[i] = (int)n;
+        k.div_tok[i] = magic((int)n);
+        ut = std::max(ut, n);
+    }
     k.div_head = magic(k.units_head);
-    // tokens per workgroup: eight share one round of angles, fewer while that leaves compute units without work
-    int tile = 8;
-    while (tile > 1 && ((long long)a->B * ceil_div(a->N, tile) < 1024 || tile * ut >= 65536)) tile >>= 1;
+    // tokens per workgroup: as many as 24 KB of rows share one round of angles (256 x 197 tokens of 24 bf16 heads of 64: 62 us
+    // with 8 tokens, 67 with 4, 66 with 16; 2 x 21601 of 20 fp32 heads of 80: 103 with 2, 107 with 4, 117 with 8), fewer while
+    // that leaves compute units without work
+    int tile = 16;
+    while (tile > 1 && ((long long)a->B * ceil_div(a->N, tile) < 1024 || tile * ut >= 65536 || tile * heads * a->DH * esz > 24 * 1024)) tile >>= 1;
     k.tile = tile;
     k.tiles = ceil_div(a->N, tile);
-    // positions shared by the batch: a workgroup turns the same tokens of several samples by one set of angles, as long as
-    // four workgroups a compute unit remain
-    const bool same = a->pos_stride[0] == 0 || a->B == 1;
-    k.B = a->B;
-    k.group = same ? (int)std::max<long long>(1, std::min<long long>(a->B, (long long)a->B * k.tiles / 1024)) : 1;
-    const long long blocks = (long long)ceil_div(a->B, k.group) * k.tiles;
+    const long long blocks = (long long)a->B * k.tiles;
     VITMI_CHECK_ARG(blocks < (1ll << 32) / ROPE_THREADS, "vitmi_rope_axes: %lld tiles are beyond one launch", blocks);
     hipStream_t s = as_stream(stream);
     ProfScope prof(VITMI_FAM_OTHER, s, 2.0 * a->B * a->N * heads * a->DH * esz);
