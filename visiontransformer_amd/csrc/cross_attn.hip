@@ -1332,12 +1332,31 @@ struct XaPlan {
 
 int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Splits of an inner loop of `steps` tiles over workgroups: none while the launch fills the chip twice over, else enough for
-// that, each with `least` tiles or more
-int xa_splits(long long blocks, int steps, int least) {
-    if (blocks >= 512 || steps < 2 * least) return 1;
-    const long long want = (512 + blocks - 1) / blocks;
-    return (int)std::max<long long>(1, std::min<long long>({want, steps / least, 64}));
+// Splits of the key loop of the few-row kernel, `steps` tiles of 32 keys, which only memory bounds: none while the launch fills
+// the chip twice over, else enough for that, each with eight tiles or more
+int xa_few_splits(long long blocks, int steps) {
+    if (blocks >= 512 || steps < 16) return 1;
+    return (int)std::max<long long>(1, std::min<long long>({(512 + blocks - 1) / blocks, steps / 8, 64}));
+}
+
+// Splits of the key loop of the row kernels: the number with the shortest estimated time, in microseconds -- rounds of
+// workgroups (two a compute unit share it in bf16, fp32 products leave nothing over beside one) times tiles a split, and
+// for more than one split the joining launch with the partial rows' way to memory and back.  8 x 6 heads of 64 fp32, 333 rows,
+// 257 keys: one split takes 32 us, two with their join 42.
+int xa_splits(int dt, long long blocks, int steps, long long rows, int D) {
+    const double tile = dt == VITMI_F32 ? D / 32.0 : 0.5 + D / 160.0, slots = dt == VITMI_F32 ? 256 : 512;
+    if (blocks >= 4 * slots) return 1;
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 64 && (s == 1 || steps / s >= 2); ++s) {
+        const double rounds = (double)(long long)((blocks * s + slots - 1) / slots);
+        const double t = rounds * tile * (cdiv(steps, s) + 2) + (s > 1 ? 4 + s * (double)rows * D * 8 / 3e6 : 0);
+        if (t < least) {
+            least = t;
+            best = s;
+        }
+    }
+    return best;
 }
 
 XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D, bool vec) {
@@ -1346,7 +1365,8 @@ XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D, bool vec) {
     const long long bh = (long long)B * Hk;
     p.few = R <= 64;
     p.fwd_tiles = cdiv(R, p.few ? 32 : 128);
-    p.fwd_splits = p.few ? xa_splits(bh * p.fwd_tiles, cdiv(Nk, 32), 8) : xa_splits(bh * p.fwd_tiles, cdiv(Nk, KT), 4);
+    const long long rows = bh * R;
+    p.fwd_splits = p.few ? xa_few_splits(bh * p.fwd_tiles, cdiv(Nk, 32)) : xa_splits(dt, bh * p.fwd_tiles, cdiv(Nk, KT), rows, D);
     // all keys in one workgroup (bf16; two of four waves a compute unit, one of eight): the problems of a last round that would
     // leave half of the chip or more idle share their rows, eight tiles of 32 each
     p.short_splits = p.short_whole = 0;
@@ -1356,12 +1376,12 @@ XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D, bool vec) {
         p.short_whole = (int)(p.short_splits > 1 ? bh - rest : bh);
     }
     p.dq_tiles = cdiv(R, 128);
-    p.dq_splits = xa_splits(bh * p.dq_tiles, cdiv(Nk, KT), 4);
+    p.dq_splits = xa_splits(dt, bh * p.dq_tiles, cdiv(Nk, KT), rows, D);
     // dk / dv: a workgroup a key tile where that keeps nine tenths of the chip busy to the end (registers allow three a compute
-    // unit in bf16 with heads up to 64, one in fp32 beyond that, else two), otherwise equal shares, of four row tiles or more
+    // unit in bf16 with heads up to 64, else two; fp32 products leave nothing over beside one), otherwise equal shares, of four row tiles or more
     p.dkv_tiles = cdiv(Nk, 128);
     p.dkv_rt = cdiv(R, dt == VITMI_BF16 && D > 96 && vec ? row_tile<bf16_t, 128, true>() : KT);
-    const long long tiles = bh * p.dkv_tiles, slots = 256 * (dt == VITMI_F32 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 3 : 2));
+    const long long tiles = bh * p.dkv_tiles, slots = 256 * (dt == VITMI_F32 ? 1 : D <= 64 ? 3 : 2);
     const bool even = 10 * tiles >= 9 * slots * ((tiles + slots - 1) / slots);
     const long long grid = std::min<long long>(dt == VITMI_F32 ? slots : 512, tiles * p.dkv_rt / 4);
     p.dkv_grid = even || p.dkv_rt < 8 || grid <= tiles / 2 ? 0 : (int)grid;

@@ -11,8 +11,8 @@
 // db_pre = E.  uh and yh are formed again from x and u in 32 bits (the stored y is rounded), the four row statistics
 // are kept by the forward pass.
 //
-// Bound by HBM (forward x, u -> y, h; backward dy, dh, x, u -> dx, du).  A row lives in the registers of one wave up to
-// 1024 elements, of 4 or 8 waves beyond, and is read once; parameters and column sums stay in registers while
+// Bound by HBM (forward x, u -> y, h; backward dy, dh, x, u -> dx, du; 256 x 197 rows of 768 bf16: 64 and 100 us, 4.7 TB/s).
+// A row lives in the registers of one wave up to 1024 elements, of 4 or 8 waves beyond, and is read once; parameters and column sums stay in registers while
 // a wave walks its rows.  Column sums are added over the workgroup's rows, written once per workgroup and reduced in a
 // fixed order by a second launch: no atomics, results are bitwise reproducible.
 #include <algorithm>
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void ngr_bwd_kernel(NgAr
     const float inv_d = 1.f / (float)a.D;
     const bool pre = a.pre != NG_NONE && a.dh;
     // the next row's loads are in flight behind a row's arithmetic where their registers (dy, x, dh, u as stored) leave room
-    constexpr bool AHEAD = ITERS * V * (sizeof(TX) + sizeof(TU)) / 2 <= 40;
+    constexpr bool AHEAD = ITERS * V * (sizeof(TX) + sizeof(TU)) / 2 <= 48;
     NVec<TX, V> nx[ITERS], ndy[ITERS];
     NVec<TU, V> nu[ITERS], ndh[ITERS];
     float ns = 1.f, nmu = 0.f, nru = 0.f, nmy = 0.f, nry = 0.f;
@@ -468,16 +468,21 @@ __device__ __forceinline__ float gate_at(const NgFinal& f, int seg, int c) {
 constexpr int NF_COLS = 16, NF_GROUPS = 64;
 
 __device__ __forceinline__ void final_pair(float& p, float& q, float (*red)[2][NF_COLS], int col, int grp) {
-    red[grp][0][col] = p;
-    red[grp][1][col] = q;
-    __syncthreads();
-    p = q = 0.f;
-    if (grp == 0)
-        for (int g = 0; g < NF_GROUPS; ++g) {
-            p += red[g][0][col];
-            q += red[g][1][col];
+    for (int n = NF_GROUPS; n > 1; n >>= 3) {            // eight into one, twice
+        if (grp < n) {
+            red[grp][0][col] = p;
+            red[grp][1][col] = q;
         }
-    __syncthreads();
+        __syncthreads();
+        p = q = 0.f;
+        if (grp < n / 8)
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                p += red[grp * 8 + g][0][col];
+                q += red[grp * 8 + g][1][col];
+            }
+        __syncthreads();
+    }
 }
 
 __global__ __launch_bounds__(NF_COLS* NF_GROUPS) void ngr_final_kernel(NgFinal f) {
@@ -542,13 +547,14 @@ struct NgPlan {
     int V, iters, wpr;
 };
 
-// A row goes to the fewest waves that hold it in sixteen values per lane
+// A row goes to one wave while sixteen values a lane hold it, to four or eight while eight do, then to eight: 4096 columns by
+// four waves of sixteen values took 189 us forwards and 303 back (4 x 4099 rows, fp32 stream), by eight of eight 151 and 256
 bool ng_plan(int D, bool vec, NgPlan* p) {
     p->V = vec ? 4 : 1;
-    const int cap = vec ? 4 : 16;                    // vectors per lane
-    for (int w : {1, 4, 8}) {
-        const int iters = ceil_div(D, 64 * w * p->V);
-        if (iters <= cap) {
+    const int values[4][2] = {{1, 16}, {4, 8}, {8, 8}, {8, 16}};      // waves, values per lane
+    for (auto& v : values) {
+        const int w = v[0], iters = ceil_div(D, 64 * w * p->V);
+        if (iters * p->V <= v[1]) {
             p->wpr = w;
             p->iters = iters;
             return true;
@@ -575,30 +581,34 @@ void ng_launch(const NgArgs& a, bool fwd, unsigned blocks, hipStream_t s) {
         hipLaunchKernelGGL((ngr_bwd_kernel<TX, TU, V, ITERS, WPR>), dim3(blocks), dim3(THREADS), 0, s, a);
 }
 
-template <typename TX, typename TU, int V, int WPR>
-void ng_iters(const NgArgs& a, int iters, bool fwd, unsigned blocks, hipStream_t s) {
-    if (V == 4) {
-        if (iters <= 1) ng_launch<TX, TU, 4, 1, WPR>(a, fwd, blocks, s);
-        else if (iters == 2) ng_launch<TX, TU, 4, 2, WPR>(a, fwd, blocks, s);
-        else if (iters == 3) ng_launch<TX, TU, 4, 3, WPR>(a, fwd, blocks, s);
-        else ng_launch<TX, TU, 4, 4, WPR>(a, fwd, blocks, s);
-    } else {
-        if (iters <= 4) ng_launch<TX, TU, 1, 4, WPR>(a, fwd, blocks, s);
-        else ng_launch<TX, TU, 1, 16, WPR>(a, fwd, blocks, s);
-    }
-}
-
 template <typename TX, typename TU>
 void ng_dispatch(const NgArgs& a, const NgPlan& p, bool fwd, unsigned blocks, hipStream_t s) {
-#define NG_W(V)                                                                    \
-    do {                                                                           \
-        if (p.wpr == 1) ng_iters<TX, TU, V, 1>(a, p.iters, fwd, blocks, s);        \
-        else if (p.wpr == 4) ng_iters<TX, TU, V, 4>(a, p.iters, fwd, blocks, s);   \
-        else ng_iters<TX, TU, V, 8>(a, p.iters, fwd, blocks, s);                   \
-    } while (0)
-    if (p.V == 4) NG_W(4);
-    else NG_W(1);
-#undef NG_W
+    // the pairs of waves and vectors per lane that ng_plan gives: (1, 1..4), (4, 2), (8, 2..4) of four values, and single values
+    // in sizes of 4, 8 and 16
+#define NG(V, I, W) ng_launch<TX, TU, V, I, W>(a, fwd, blocks, s)
+    if (p.V == 4) {
+        if (p.wpr == 1) {
+            if (p.iters <= 1) NG(4, 1, 1);
+            else if (p.iters == 2) NG(4, 2, 1);
+            else if (p.iters == 3) NG(4, 3, 1);
+            else NG(4, 4, 1);
+        } else if (p.wpr == 4) {
+            NG(4, 2, 4);
+        } else {
+            if (p.iters <= 2) NG(4, 2, 8);
+            else if (p.iters == 3) NG(4, 3, 8);
+            else NG(4, 4, 8);
+        }
+    } else if (p.wpr == 1) {
+        if (p.iters <= 4) NG(1, 4, 1);
+        else NG(1, 16, 1);
+    } else if (p.wpr == 4) {
+        NG(1, 8, 4);
+    } else {
+        if (p.iters <= 8) NG(1, 8, 8);
+        else NG(1, 16, 8);
+    }
+#undef NG
 }
 
 bool ng_types_ok(int dx, int du) {
