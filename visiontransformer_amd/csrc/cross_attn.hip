@@ -198,6 +198,15 @@ __device__ __attribute__((aligned(16))) unsigned int xa_zero16[4] = {0u, 0u, 0u,
 __device__ __forceinline__ void load_to_lds(const void* from, unsigned to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(to) : "memory", "m0");
 }
+// the same from a wave-uniform address plus a lane's byte offset: no vector arithmetic per load
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned offset, unsigned to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ long long uniform(long long v) {       // a wave-uniform value into scalar registers
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)((unsigned long long)v >> 32));
+    return (long long)(((unsigned long long)hi << 32) | lo);
+}
+template <typename P> __device__ __forceinline__ P* uniform(P* p) { return reinterpret_cast<P*>(uniform((long long)p)); }
 __device__ __forceinline__ unsigned lds_addr(const void* p) {
     return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
@@ -220,6 +229,30 @@ struct Stage {
     static constexpr int CPR = NP * CP, IT = DMA ? 1 : KT * CPR / TH;
     static_assert(DMA ? PPI * KT * CP == TH && NP % PPI == 0 && VEC : KT * CPR % TH == 0, "a tile is a whole number of pieces per thread");
     typename Mx<T>::frag x[IT], y[IT];
+    unsigned ox, oy;      // DMA: byte offsets of the thread's piece of plane 0 from a tile's first row
+    int tail;             // DMA: dims from here on are beyond D in the thread's chunk of a plane that ends there
+    bool near;            // a tile spans less than 4 GB of either matrix
+    __device__ __forceinline__ void init(long long lx, long long ly, int D, int t) {
+        if (!DMA) return;
+        const int r = row_of(0, t), d = 32 * (t / (KT * CP)) + ((t % CP) ^ swz<T>(r)) * Mx<T>::FE;
+        ox = (unsigned)((r * lx + d) * sizeof(T));
+        oy = (unsigned)((r * ly + d) * sizeof(T));
+        tail = D - d;
+        near = uniform((lx > ly ? lx : ly) * KT * (long long)sizeof(T)) < (1ll << 32) - 4096;
+    }
+    // a whole tile whose first rows start at bx / by: only lanes beyond D have nothing to load, and their place in LDS holds the
+    // zeros that the general form left there
+    __device__ __forceinline__ void whole(const T* bx, const T* by, T* ix, T* iy, int D, int t) {
+        bx = uniform(bx);
+        by = uniform(by);
+        const unsigned lx = lds_addr(ix + (t & ~63) * Mx<T>::FE), ly = lds_addr(iy + (t & ~63) * Mx<T>::FE);
+#pragma unroll
+        for (int p = 0; p < NP; p += PPI)
+            if (32 * (p + PPI) <= D || 32 * p < tail) {
+                load_to_lds(bx + 32 * p, ox, lx + p * KT * 32 * (unsigned)sizeof(T));
+                load_to_lds(by + 32 * p, oy, ly + p * KT * 32 * (unsigned)sizeof(T));
+            }
+    }
     // the thread's row of a tile (DMA), or row of piece i
     __device__ __forceinline__ static int row_of(int i, int t) { return DMA ? t % (KT * CP) / CP : (t + i * TH) / CPR; }
     // px / py: start of the row that row_of names, valid where ok
@@ -245,9 +278,13 @@ struct Stage {
             }
         }
     }
-    // key rows row0 + r with row strides lx, ly
+    // key rows row0 + r with row strides lx, ly; `clean`: the images' places beyond D hold zeros already
     __device__ __forceinline__ void fetch(const T* px, long long lx, const T* py, long long ly, int row0, unsigned long long mask, T* ix,
-                                          T* iy, int D, int t) {
+                                          T* iy, int D, int t, bool clean) {
+        if (DMA && mask == full_mask<KT>() && near && (clean || D == DP)) {
+            whole(px + row0 * lx, py + row0 * ly, ix, iy, D, t);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int r = row_of(i, t);
@@ -256,7 +293,15 @@ struct Stage {
     }
     // query rows: row r of the flattened group is position r % Nq of head r / Nq
     __device__ __forceinline__ void fetch_rows(const T* px, const long long* sx, const T* py, const long long* sy, int row0, int R, int Nq, T* ix,
-                                               T* iy, int D, int t) {
+                                               T* iy, int D, int t, bool clean) {
+        if (DMA && near && (clean || D == DP)) {
+            int g0, n0;
+            split_row(Nq, R, row0, g0, n0);
+            if (n0 + KT <= Nq) {                          // all of one head
+                whole(px + n0 * sx[1] + g0 * sx[2], py + n0 * sy[1] + g0 * sy[2], ix, iy, D, t);
+                return;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int r = row0 + row_of(i, t);
@@ -397,14 +442,43 @@ __device__ __forceinline__ void store4(T* row, int d, int D, float v0, float v1,
             if (d + j < D) row[d + j] = from_f32<T>(v[j]);
     }
 }
+// a 32-dim block of an accumulator to dims d0.. of a dense row.  bf16: the half waves hold four dims of every eight each and
+// swap one group of a pair, so that a lane stores 16 bytes and a row 32 together.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_block(T* row, int d0, const f32x16& o, float f, int h, int D) {
+    if constexpr (VEC && sizeof(T) == 2) {
+#pragma unroll
+        for (int g = 0; g < 4; g += 2) {
+            union {
+                bf16x2 v[2];
+                unsigned w[2];
+            } x, y;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x.v[i] = __builtin_convertvector(f32x2{o[4 * g + 2 * i] * f, o[4 * g + 2 * i + 1] * f}, bf16x2);
+                y.v[i] = __builtin_convertvector(f32x2{o[4 * g + 4 + 2 * i] * f, o[4 * g + 5 + 2 * i] * f}, bf16x2);
+            }
+            u32x4 out;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const auto r = __builtin_amdgcn_permlane32_swap(x.w[i], y.w[i], false, false);
+                out[i] = r[0];
+                out[2 + i] = r[1];
+            }
+            const int d = d0 + 8 * (g + h);
+            if (row && d < D) *reinterpret_cast<u32x4*>(row + d) = out;
+        }
+    } else if (row) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            store4<T, VEC>(row, d0 + 8 * g + 4 * h, D, o[4 * g] * f, o[4 * g + 1] * f, o[4 * g + 2] * f, o[4 * g + 3] * f);
+    }
+}
+// a NULL row is not stored, but its lane takes part in the exchange
 template <typename T, bool VEC, int DP>
 __device__ __forceinline__ void store_acc(T* row, const f32x16 (&o)[DP / 32], float f, int h, int D) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            store4<T, VEC>(row, 32 * db + 8 * g + 4 * h, D, o[db][4 * g] * f, o[db][4 * g + 1] * f, o[db][4 * g + 2] * f,
-                           o[db][4 * g + 3] * f);
+    for (int db = 0; db < DP / 32; ++db) store_block<T, VEC>(row, 32 * db, o[db], f, h, D);
 }
 
 // element offset of query row r of problem (b, hk) in a dense [B, Nq, Hq, D]
@@ -418,14 +492,14 @@ __device__ __forceinline__ long long dense_row(const XaArgs& a, int b, int hk, i
 template <typename T, int DP, bool VEC>
 __device__ __forceinline__ void finish_rows(const XaArgs& a, int b, int hk, int r, int split, const f32x16 (&o)[DP / 32], float m, float l,
                                             int h) {
-    if (r >= a.R) return;
-    const long long row = dense_row(a, b, hk, r), st = ((long long)b * a.Hk + hk) * a.R + r;
+    const bool in = r < a.R;
+    const long long row = in ? dense_row(a, b, hk, r) : 0, st = ((long long)b * a.Hk + hk) * a.R + r;
     if (a.splits == 1) {
-        store_acc<T, VEC, DP>((T*)a.o + row, o, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), h, a.D);
-        if (a.lse && h == 0) a.lse[st] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
+        store_acc<T, VEC, DP>(in ? (T*)a.o + row : nullptr, o, l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l), h, a.D);
+        if (in && a.lse && h == 0) a.lse[st] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
     } else {
-        store_acc<float, VEC, DP>(a.part_o + split * a.n_q + row, o, 1.f, h, a.D);
-        if (h == 0) {
+        store_acc<float, VEC, DP>(in ? a.part_o + split * a.n_q + row : nullptr, o, 1.f, h, a.D);
+        if (in && h == 0) {
             float2* ml = reinterpret_cast<float2*>(a.part_ml) + (long long)split * (a.n_q / a.D) + st;
             *ml = make_float2(m, l);
         }
@@ -475,10 +549,11 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
     split_range((n + KT - 1) / KT, a.splits, split, t0, t1);
     Stage<T, DP, VEC, KT, XA_THREADS, VEC> st;
     MaskWalk<KT> mw;
+    st.init(a.ks[1], a.vs[1], a.D, t);
     if (t0 < t1) {
         mw.start(a, b, n, t0, 1, lane);
         T* img = lds + (t0 & 1) * 2 * IMG;
-        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, mw.cur, img, img + IMG, a.D, t);
+        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, mw.cur, img, img + IMG, a.D, t, false);
     }
     for (int kt = t0; kt < t1; ++kt) {
         T* img = lds + (kt & 1) * 2 * IMG;
@@ -488,7 +563,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 ? 1 : 2) void xattn_fwd_
         __syncthreads();
         if (kt + 1 < t1) {
             T* nxt = lds + ((kt + 1) & 1) * 2 * IMG;
-            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t);
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t, kt > t0);
             mw.advance(a, kt, lane);
         }
         if (busy && mk) {
@@ -531,7 +606,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     MaskWalk<KT> mw;
     if (t0 + wave < t1) {
         mw.start(a, b, n, t0 + wave, 4, lane);
-        st.fetch(kp, a.ks[1], vp, a.vs[1], (t0 + wave) * KT, mw.cur, nullptr, nullptr, a.D, lane);
+        st.fetch(kp, a.ks[1], vp, a.vs[1], (t0 + wave) * KT, mw.cur, nullptr, nullptr, a.D, lane, false);
     }
     typename Mx<T>::frag qf[DP / Mx<T>::KD];
     {
@@ -553,7 +628,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
         st.store(img, img + IMG, lane);
         wave_fence();
         if (kt + 4 < t1) {
-            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, mw.next, nullptr, nullptr, a.D, lane);
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, mw.next, nullptr, nullptr, a.D, lane, false);
             mw.advance(a, kt, lane);
         }
         if (mk) attend<T, DP, KT>(img, img + IMG, qf, (unsigned)mk, a.c, o, m, l, lane);
@@ -711,10 +786,11 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
     split_range(a.dq ? (n + KT - 1) / KT : 0, a.splits, split, t0, t1);      // without dq only delta is wanted
     Stage<T, DP, VEC, KT, XA_THREADS, VEC> st;
     MaskWalk<KT> mw;
+    st.init(a.ks[1], a.vs[1], a.D, t);
     if (t0 < t1) {
         mw.start(a, b, n, t0, 1, lane);
         T* img = lds + (t0 & 1) * 2 * IMG;
-        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, mw.cur, img, img + IMG, a.D, t);
+        st.fetch(kp, a.ks[1], vp, a.vs[1], t0 * KT, mw.cur, img, img + IMG, a.D, t, false);
     }
     for (int kt = t0; kt < t1; ++kt) {
         T* img = lds + (kt & 1) * 2 * IMG;
@@ -724,7 +800,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
         __syncthreads();
         if (kt + 1 < t1) {
             T* nxt = lds + ((kt + 1) & 1) * 2 * IMG;
-            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t);
+            st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 1) * KT, mw.next, nxt, nxt + IMG, a.D, t, kt > t0);
             mw.advance(a, kt, lane);
         }
         if (mk && rt * 128 + wave * 32 < a.R) {
@@ -746,11 +822,11 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
             }
         }
     }
-    if (!in || !a.dq) return;
+    if (!a.dq) return;
     if (a.splits == 1)
-        store_acc<T, VEC, DP>((T*)a.dq + row, acc, a.scale, h, a.D);
+        store_acc<T, VEC, DP>(in ? (T*)a.dq + row : nullptr, acc, a.scale, h, a.D);
     else
-        store_acc<float, VEC, DP>(a.part_dq + split * a.n_q + row, acc, 1.f, h, a.D);
+        store_acc<float, VEC, DP>(in ? a.part_dq + split * a.n_q + row : nullptr, acc, 1.f, h, a.D);
 }
 
 // dq, dk and dv of up to 32 NW keys in one launch (bf16): all keys of a problem fit the registers of one workgroup, wave w
@@ -882,13 +958,7 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] += alt[e];
         const int r = tile * QT + 32 * sub + (lane & 31);
-        if (r < a.R) {
-            T* row = (T*)a.dq + dense_row(a, b, hk, r);
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                store4<T, true>(row, 32 * j + 8 * g + 4 * h, a.D, acc[4 * g] * a.scale, acc[4 * g + 1] * a.scale,
-                                acc[4 * g + 2] * a.scale, acc[4 * g + 3] * a.scale);
-        }
+        store_block<T, true>(r < a.R ? (T*)a.dq + dense_row(a, b, hk, r) : nullptr, 32 * j, acc, a.scale, h, a.D);
     };
     // the pieces of a tile's dq go round the waves (left to the waves without a key alone they hold the others up: 104 us for 75
     // at 32 x 12 heads, 576 rows, 197 keys)
@@ -957,15 +1027,16 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
         __syncthreads();
         dq_tile(t1 - 1);
     }
-    if (key >= a.Nk || !a.dk) return;
+    if (!a.dk) return;
+    const bool in = key < a.Nk;
     const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
     if (!shared || a.splits == 1) {
-        store_acc<T, true, DP>((T*)a.dk + row, dk, a.scale, h, a.D);
-        store_acc<T, true, DP>((T*)a.dv + row, dv, 1.f, h, a.D);
+        store_acc<T, true, DP>(in ? (T*)a.dk + row : nullptr, dk, a.scale, h, a.D);
+        store_acc<T, true, DP>(in ? (T*)a.dv + row : nullptr, dv, 1.f, h, a.D);
     } else {                                              // [problem][split][dk, dv][Nk][D]
         float* slot = a.part_kv + ((((long long)sh * a.splits + split) * 2) * a.Nk + key) * a.D;
-        store_acc<float, true, DP>(slot, dk, 1.f, h, a.D);
-        store_acc<float, true, DP>(slot + (long long)a.Nk * a.D, dv, 1.f, h, a.D);
+        store_acc<float, true, DP>(in ? slot : nullptr, dk, 1.f, h, a.D);
+        store_acc<float, true, DP>(in ? slot + (long long)a.Nk * a.D : nullptr, dv, 1.f, h, a.D);
     }
 }
 
@@ -1006,10 +1077,6 @@ __global__ __launch_bounds__(256) void xattn_short_join_kernel(XaArgs a, int per
 // key tiles, of which there may be a few more than the chip holds at once, would leave it idle for up to half the time.
 // With three or more workgroups a key tile the shares end at tile borders.  Lengths per sample are only known here, so
 // each wave counts the live tiles itself (64 samples a step).
-__device__ __forceinline__ long long uniform(long long v) {       // a wave-uniform value into scalar registers
-    const unsigned lo = __builtin_amdgcn_readfirstlane((int)(unsigned)v), hi = __builtin_amdgcn_readfirstlane((int)(unsigned)((unsigned long long)v >> 32));
-    return (long long)(((unsigned long long)hi << 32) | lo);
-}
 struct Stream {
     long long units;      // in all
     int rt, nb;           // row tiles a key tile, workgroups that share the units
@@ -1141,10 +1208,11 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
         const T* gp = (const T*)a.dout + b * a.dos[0] + (long long)hk * a.G * a.dos[2];
         const long long sti = ((long long)b * a.Hk + hk) * a.R;
         Stage<T, DP, VEC, QT, XA_THREADS, VEC> st;
+        st.init(a.qs[1], a.dos[1], a.D, t);
         float stat = 0.f;                                 // threads 0..QT-1: lse, QT..2QT-1: delta
         auto fetch = [&](int tile, int pair) {
             T* img = lds + pair * 2 * IMG;
-            st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, img, img + IMG, a.D, t);
+            st.fetch_rows(qp, a.qs, gp, a.dos, tile * QT, a.R, a.Nq, img, img + IMG, a.D, t, tile > t0 + 1);
             if (t < 2 * QT) {
                 const int r = tile * QT + (t < QT ? t : t - QT);
                 stat = t < QT ? INFINITY : 0.f;
@@ -1208,7 +1276,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
                 }
             }
         }
-        if (key >= a.Nk) continue;
+        const bool in = key < a.Nk;
         if (!on) {                                        // a masked key's lane worked on zeros: its gradients are zero
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -1217,12 +1285,12 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
         }
         if (!STREAM || (t0 == 0 && t1 == RT)) {
             const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
-            store_acc<T, VEC, DP>((T*)a.dk + row, dk, a.scale, h, a.D);
-            store_acc<T, VEC, DP>((T*)a.dv + row, dv, 1.f, h, a.D);
+            store_acc<T, VEC, DP>(in ? (T*)a.dk + row : nullptr, dk, a.scale, h, a.D);
+            store_acc<T, VEC, DP>(in ? (T*)a.dv + row : nullptr, dv, 1.f, h, a.D);
         } else {                                          // a workgroup's first and its last part may be shares of a tile
             float* slot = a.part_kv + ((2ll * blk + (part > 0)) * 2 * 128 + wave * 32 + (lane & 31)) * a.D;
-            store_acc<float, VEC, DP>(slot, dk, 1.f, h, a.D);
-            store_acc<float, VEC, DP>(slot + 128ll * a.D, dv, 1.f, h, a.D);
+            store_acc<float, VEC, DP>(in ? slot : nullptr, dk, 1.f, h, a.D);
+            store_acc<float, VEC, DP>(in ? slot + 128ll * a.D : nullptr, dv, 1.f, h, a.D);
         }
     }
 }
