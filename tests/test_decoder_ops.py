@@ -250,6 +250,62 @@ def test_c_abi_checks_and_sizes(sanitized):
     assert r.returncode == 0 and r.stdout.strip().endswith("ok"), (r.returncode, r.stdout, r.stderr[-2000:])
 
 
+MORE_CHECKS = r"""
+import ctypes, os, sys
+sys.path.insert(0, sys.argv[2])
+if sys.argv[1]:
+    os.environ["VITMI_LIB"] = sys.argv[1]
+from visiontransformer_amd import _lib, ops
+lib, at = _lib.lib, ctypes.addressof
+assert lib.vitmi_cross_attn_fwd.restype is ctypes.c_int
+x = ops._XattnArgs(q=64, k=64, v=64, o=64, lse=64, dout=64, dt=1, B=1, Nq=100, Nk=8000, Hq=1, Hk=1, D=64, scale=1.0)
+f, b = lib.vitmi_cross_attn_fwd, lib.vitmi_cross_attn_bwd
+said = lambda: lib.vitmi_last_error().decode()
+assert lib.vitmi_cross_attn_fwd_workspace_bytes(1, 1, 100, 8000, 1, 1, 64) > 0
+for fn in (f, b):                       # nothing is launched: every call ends at a check
+    assert fn(at(x), 0, None) == -1 and ("workspace" in said() or "null" in said())
+    assert fn(at(x), 264, None) == -1 and "aligned" in said(), said()
+    for name in ("qs", "ks", "vs", "dos"):
+        s = getattr(x, name)
+        s[1] = -64
+        assert fn(at(x), 256, None) == -1 and "negative" in said(), said()
+        s[1] = 0
+    x.Nk = 2 ** 31 - 4096               # tiles looked at ahead would pass the largest int
+    assert fn(at(x), 256, None) == -1 and "lengths" in said(), said()
+    x.Nk = 8000
+n = ops._NgrArgs(x=64, u=64, stats=64, dy=64, dpost_w=64, dt_x=1, dt_u=1, B=1, N=1, D=8, post=1, eps=1e-6, res_scale=1.0)
+assert lib.vitmi_norm_gate_residual_bwd(at(n), 264, None) == -1 and "aligned" in said(), said()
+n.eps = -1e-6
+assert lib.vitmi_norm_gate_residual_bwd(at(n), 256, None) == -1 and "eps" in said(), said()
+assert lib.vitmi_norm_gate_residual_fwd(at(n), None) == -1 and "eps" in said(), said()
+print("ok")
+"""
+
+
+@pytest.mark.parametrize("sanitized", [False, True])
+def test_c_abi_refuses_what_no_kernel_covers(sanitized):
+    path = os.path.join(ROOT, "visiontransformer_amd", "libvitmi_hip_hostsan.so") if sanitized else ""
+    if sanitized and not os.path.exists(path):
+        pytest.skip("host-sanitized library not built")
+    r = subprocess.run([sys.executable, "-c", MORE_CHECKS, path, ROOT], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), (r.returncode, r.stdout, r.stderr[-2000:])
+
+
+def test_in_place_rotation_of_shared_memory_and_negative_eps_are_refused():
+    buf, pos = torch.zeros(200), torch.zeros(3, 1)
+    a, b = buf[:96].view(2, 3, 2, 8), buf[90:186].view(2, 3, 2, 8)
+    with pytest.raises(ValueError, match="apart"):
+        ops.rope_axes(a, b, pos, (2,), inplace=True)
+    with pytest.raises(ValueError, match="apart"):
+        ops.rope_axes(a, a, pos, (2,), inplace=True)
+    with pytest.raises(RuntimeError, match="ROCm device tensors"):       # neighbours are apart: the next check speaks
+        ops.rope_axes(a, buf[96:192].view(2, 3, 2, 8), pos, (2,), inplace=True)
+    x = torch.zeros(2, 3, 8)
+    for eps in (-1e-6, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            ops.norm_gate_residual(x, x, post="rms", eps=eps)
+
+
 def test_argument_structs_match_the_header(tmp_path):
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include "%s/include/vitmi.h"\nint main(void) { printf("%%zu %%zu %%zu %%zu", '

@@ -334,6 +334,57 @@ def test_cross_attn_states_beyond_32_bit_offsets():
     assert torch.equal(ops().cross_attn(q, sl, sl, key_mask=keep), ops().cross_attn(q, small, small, key_mask=keep))
 
 
+@pytest.mark.parametrize("Nq,Nk,D,dtype", [(90, 200, 64, H), (40, 100, 128, H), (700, 520, 64, H), (130, 300, 128, H), (90, 200, 64, F),
+                                           (90, 60, 33, H)], ids=str)
+def test_cross_attn_masked_keys_have_no_gradient_whatever_the_others_hold(Nq, Nk, D, dtype):
+    """Infinities and NaN in the output's gradient and in one sample's queries reach the allowed keys alone."""
+    g = gen(21)
+    q, k, v, do = (torch.randn(2, n, 2, D, generator=g).to(DEV, dtype) for n in (Nq, Nk, Nk, Nq))
+    do[0, 1], do[0, Nq - 1, :, 3], q[1, 0] = float("inf"), float("nan"), float("nan")
+    keep = (torch.rand(2, Nk, generator=g) < 0.5).to(DEV)
+    args = [t.requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(ops().cross_attn(*args, key_mask=keep), args, do)
+    for t in (dk, dv):
+        assert not t[~keep].any() and not t[keep].isfinite().all()
+    assert dq[0, 2:Nq - 1].isfinite().all() and dq[1, 1:].isfinite().all()
+
+
+def test_cross_attn_rows_more_than_4_gb_apart_within_a_tile():
+    """Row strides that no 32-bit offset within a tile of rows reaches, in every operand and both directions."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    step, rows = 40_000_000, 70                             # 64 rows span 5.1 GB
+    far = torch.empty(step * rows, dtype=H, device=DEV)
+    for Nk in (70, 300):                                    # one workgroup a problem, and key tiles of their own
+        small = [torch.randn(1, n, 1, 64, generator=g, device=DEV).to(H) for n in (70, min(Nk, 70), 70)]
+        views = [torch.as_strided(far, t.shape, (step * rows, step, 64, 1), 128 * i) for i, t in enumerate(small)]
+        for a, b in zip(views, small):
+            a.copy_(b)
+        if Nk > 70:                                         # the queries and their gradient far apart, many keys close together
+            small[1] = views[1] = torch.randn(1, Nk, 1, 64, generator=g, device=DEV).to(H)
+        got = []
+        for q, k, do in (small, views):
+            leaves = [t.detach().requires_grad_() for t in (q, k)]
+            o = ops().cross_attn(*leaves, leaves[1])
+            got.append((o,) + torch.autograd.grad(o, leaves, do))
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("Nk", [45, 300])
+def test_cross_attn_gradient_off_a_border(Nk):
+    """Aligned operands with an upper gradient that is not: the backward pass takes another form than the size query of
+    aligned operands alone would show."""
+    g = gen(12)
+    q, k, v, wide = (torch.randn(2, n, 2, d, generator=g).to(DEV, H) for n, d in ((150, 32), (Nk, 32), (Nk, 32), (150, 33)))
+    args = [t.requires_grad_() for t in (q, k, v)]
+    o = ops().cross_attn(*args)
+    got = (o,) + torch.autograd.grad(o, args, wide[..., 1:])
+    ref, tol = attention_bounds(*(t.detach().double().cpu() for t in (q, k, v)), torch.ones(2, Nk, dtype=torch.bool),
+                                wide[..., 1:].double().cpu(), H, half_step(o))
+    for n, t in zip(("o", "dq", "dk", "dv"), got):
+        within(n, t, ref[n], tol[n])
+
+
 # ---------------------------------------------------------------------------------------------- residual update
 NGR = [  # B, N, D, post, pre, gate, drop
     (1, 1, 8, None, None, None, False), (2, 3, 768, "layer", "layer", "channel", False), (5, 7, 192, "layer", "layer", "sample", True),
@@ -654,3 +705,14 @@ def test_per_sample_passes():
     with per_sample_norms(2, DEV):
         with pytest.raises(NotImplementedError, match="norm_gate_residual"):
             torch.autograd.grad(z.sum(), w)
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(2, 5, 2, 16, device=DEV).requires_grad_()
+    u = torch.randn(2, 5, 16, device=DEV).requires_grad_()
+    pos = torch.arange(5, device=DEV)[:, None]
+    for leaf, f in ((x, lambda: ops().rope_axes(x, None, pos, (8,))), (x, lambda: ops().cross_attn(x, x, x)),
+                    (u, lambda: ops().norm_gate_residual(u, u, post="rms")[0])):
+        grad, = torch.autograd.grad(f().square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grad.sum().backward()

@@ -1029,6 +1029,12 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
     }
     if (!a.dk) return;
     const bool in = key < a.Nk;
+    if (!on) {                                            // a masked key's lane worked on zeros: its gradients are zero
+#pragma unroll
+        for (int d = 0; d < NP; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+    }
     const long long row = (((long long)b * a.Nk + key) * a.Hk + hk) * a.D;
     if (!shared || a.splits == 1) {
         store_acc<T, true, DP>(in ? (T*)a.dk + row : nullptr, dk, a.scale, h, a.D);
@@ -1363,6 +1369,7 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(const float* p, T* o, fl
 
 // ---------------------------------------------------------------------------------------------- host
 constexpr int XA_MAX_D = 128;
+constexpr long long XA_MAX_ROWS = (1ll << 31) - 256, XA_MAX_KEYS = (1ll << 31) - 4096;   // row and key indices are ints, up to 12 key tiles ahead
 
 int xa_check(const char* who, const vitmi_xattn_args* g) {
     VITMI_CHECK_ARG(g, "%s: null arguments", who);
@@ -1376,8 +1383,9 @@ int xa_check(const char* who, const vitmi_xattn_args* g) {
         vitmi_set_error("%s: heads of %d exceed the supported width %d", who, g->D, XA_MAX_D);
         return VITMI_ERR_UNSUPPORTED;
     }
-    const long long lim = 1ll << 31;
-    VITMI_CHECK_ARG((long long)(g->Hq / g->Hk) * g->Nq < lim - 256 && (long long)g->Nk < lim - 256, "%s: lengths beyond one call", who);
+    VITMI_CHECK_ARG((long long)(g->Hq / g->Hk) * g->Nq < XA_MAX_ROWS && (long long)g->Nk < XA_MAX_KEYS, "%s: lengths beyond one call", who);
+    for (int i = 0; i < 3; ++i)
+        VITMI_CHECK_ARG(g->qs[i] >= 0 && g->ks[i] >= 0 && g->vs[i] >= 0 && (!g->dout || g->dos[i] >= 0), "%s: negative strides", who);
     return VITMI_OK;
 }
 
@@ -1579,7 +1587,7 @@ int xa_run_short(const XaArgs& a, long long blocks, hipStream_t s) {
 
 extern "C" long long vitmi_cross_attn_fwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
-    if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
+    if ((long long)(Hq / Hk) * Nq >= XA_MAX_ROWS) return 0;
     const int s = xa_plan(dt, B, Nq, Nk, Hq, Hk, D, true).fwd_splits;
     if (s == 1) return 0;
     const long long rows = (long long)B * Nq * Hq;
@@ -1594,6 +1602,7 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
     const bool vec = xa_vec(g);
     const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D, vec);
     VITMI_CHECK_ARG(p.fwd_splits == 1 || workspace, "%s: this shape needs a workspace", who);
+    VITMI_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be aligned to 16 bytes", who);
     XaArgs a;
     xa_fill(g, &a);
     const long long rows = (long long)g->B * g->Nq * g->Hq;
@@ -1618,7 +1627,7 @@ extern "C" int vitmi_cross_attn_fwd(const vitmi_xattn_args* g, void* workspace, 
 
 extern "C" long long vitmi_cross_attn_bwd_workspace_bytes(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D) {
     if (B <= 0 || Nq <= 0 || Nk <= 0 || Hk <= 0 || Hq <= 0 || D <= 0 || Hq % Hk) return 0;
-    if ((long long)(Hq / Hk) * Nq >= (1ll << 31) - 256) return 0;
+    if ((long long)(Hq / Hk) * Nq >= XA_MAX_ROWS) return 0;
     const long long rows = (long long)B * Nq * Hq;
     long long most = 0;
     for (bool vec : {false, true}) {                      // room for either alignment of the operands
@@ -1637,6 +1646,7 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
     VITMI_CHECK_ARG(g->B > 0 && g->Nq > 0 && g->Nk > 0, "%s: nothing to differentiate", who);
     VITMI_CHECK_ARG(g->q && g->k && g->v && g->o && g->dout && g->lse && workspace, "%s: null pointer", who);
     VITMI_CHECK_ARG((g->dk == nullptr) == (g->dv == nullptr), "%s: dk and dv come together", who);
+    VITMI_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be aligned to 16 bytes", who);
     const bool vec = xa_vec(g);
     const XaPlan p = xa_plan(g->dt, g->B, g->Nq, g->Nk, g->Hq, g->Hk, g->D, vec);
     XaArgs a;

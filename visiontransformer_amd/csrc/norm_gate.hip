@@ -622,6 +622,7 @@ int ng_check(const char* who, const vitmi_ngr_args* g) {
     VITMI_CHECK_ARG(g->B >= 0 && g->N >= 0 && g->D > 0, "%s: bad shape B=%d N=%d D=%d", who, g->B, g->N, g->D);
     VITMI_CHECK_ARG(g->post >= 0 && g->post <= 2 && g->pre >= 0 && g->pre <= 2, "%s: bad norm kind %d / %d", who, g->post, g->pre);
     VITMI_CHECK_ARG(!g->gate || g->gate_dt == VITMI_F32 || g->gate_dt == VITMI_BF16, "%s: bad gate type %d", who, g->gate_dt);
+    VITMI_CHECK_ARG(g->eps >= 0.f, "%s: eps must not be negative", who);
     if (g->D > 8192) {
         vitmi_set_error("%s: D=%d exceeds the supported row length 8192", who, g->D);
         return VITMI_ERR_UNSUPPORTED;
@@ -706,6 +707,7 @@ extern "C" int vitmi_norm_gate_residual_bwd(const vitmi_ngr_args* g, void* works
     VITMI_CHECK_ARG(g->B > 0 && g->N > 0, "%s: no rows", who);
     VITMI_CHECK_ARG(g->x && g->u && g->stats && (g->dy || g->dh) && (workspace || !sums), "%s: null pointer", who);
     VITMI_CHECK_ARG(!g->dgate || g->gate, "%s: gradient of an absent gate", who);
+    VITMI_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be aligned to 16 bytes", who);
     NgPlan p;
     if (!ng_plan(g->D, ng_vec(g), &p)) {
         vitmi_set_error("%s: no plan for D=%d", who, g->D);

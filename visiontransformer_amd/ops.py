@@ -11,6 +11,7 @@ import struct
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import BF16, EPI_DGELU, EPI_GELU, EPI_GELU_D, EPI_MULAUX, EPI_NONE, F32, check, lib
@@ -1736,6 +1737,7 @@ class RopeAxesFn(torch.autograd.Function):
         return outs if k is not None else outs[0]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk=None):
         if _PS2 is not None:                # a replay forms no input gradients
             return tuple(None if g is None else _no_grad_like(g.shape, g.dtype, g.device) for g in (dq, dk)) + (None,) * 5
@@ -1750,6 +1752,16 @@ class RopeAxesFn(torch.autograd.Function):
         return outs[0], outs[1], None, None, None, None, None
 
 
+def _overlap(q, k):
+    """Whether two tensors are known to share memory: one start, or both dense with ranges that meet."""
+    if not q.numel() or not k.numel():
+        return False
+    p, r = q.data_ptr(), k.data_ptr()
+    if q.is_contiguous() and k.is_contiguous():
+        return p < r + k.numel() * k.element_size() and r < p + q.numel() * q.element_size()
+    return p == r
+
+
 def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladder=False, inplace=False):
     """Rotary positions with several axes (time, height, width) on queries [B, N, Hq, D] and, unless None, keys
     [B, N, Hk, D] of the same tokens, in one launch; differentiable.  Returns the rotated (q, k), or q alone.
@@ -1758,8 +1770,8 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     leaves a token as it is (class token).  sections: how many of the head's pairs turn with each axis; pair j of an axis
     with s pairs turns by pos * base^(-j / s) (base a number or one per axis), or, with shared_ladder, pair p of all P by
     pos * base^(-p / P).  A pair is dims (p, P + p), or (2p, 2p + 1) with interleaved; dims from 2P on pass through.
-    q and k may be strided views (the slots of a packed projection); the results are dense.  inplace rotates q and k
-    where they lie, outside of autograd only."""
+    q and k may be strided views (the slots of a packed projection); the results are dense.  inplace rotates q and k,
+    which must not share elements, where they lie, outside of autograd only."""
     xs = (q,) if k is None else (q, k)
     if inplace:
         for t in xs:
@@ -1788,7 +1800,7 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     if inplace:
         if graph:
             raise RuntimeError("rope_axes(inplace=True) is for tensors outside of autograd")
-        if k is not None and q.data_ptr() == k.data_ptr() and q.numel():
+        if k is not None and _overlap(q, k):
             raise ValueError("inplace needs q and k apart")
     device = _one_device(q, k, pos)
     if graph:
@@ -1834,6 +1846,7 @@ class CrossAttnFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, kv_len, key_mask = ctx.saved_tensors
         if _PS2 is not None:                # a replay forms no input gradients
@@ -1931,6 +1944,7 @@ class NormGateResidualFn(torch.autograd.Function):
         return (y, h) if h is not None else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh=None):
         x, u, *params, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -2007,6 +2021,8 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
         x = x if x.stride(2) == 1 else x.contiguous()
         u = u if u.stride(2) == 1 else u.contiguous()
     meta = (float(res_scale), _NORM_KINDS[post], _NORM_KINDS[pre], float(eps))
+    if not meta[3] >= 0.0:
+        raise ValueError(f"eps {eps} must not be negative")
     device = _one_device(x, u, gate, branch_scale, *vectors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, u, gate, *vectors)):
         res = NormGateResidualFn.apply(x, u, gate, branch_scale, *vectors, meta, device)
