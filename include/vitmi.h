@@ -628,8 +628,8 @@ int vitmi_rope_axes(const vitmi_rope_args* args, void* stream);
  * stride over D <= 128.  kv_len [B] (int32, or int64 with kv_len_i64; clamped to 0 .. Nk) or key_mask [B, Nk] bytes
  * (0 = not attended to; rows mask_stride apart, unit stride), or neither.  Masked keys count as absent whatever their
  * rows hold, their gradients are zero; a sample without an allowed key gives o = 0 and zero gradients.
- * lse [B, Hq * Nq] fp32 (log2 domain, +inf for an empty row) is written by the forward call (NULL: not kept) and read by
- * the backward call.  dq may be NULL, and dk with dv. */
+ * Strides are not negative, workspaces are aligned to 16 bytes.  lse [B, Hq * Nq] fp32 (log2 domain, +inf for an empty
+ * row) is written by the forward call (NULL: not kept) and read by the backward call.  dq may be NULL, and dk with dv. */
 typedef struct {
     const void *q, *k, *v;
     void* o;
@@ -656,7 +656,7 @@ int vitmi_cross_attn_bwd(const vitmi_xattn_args* args, void* workspace, void* st
  * absent: y = res_scale * x and u is not read.  x, u have strides in elements (batch, row) and unit stride over D; y, h, dy,
  * dh, dx, du are dense (y, dy, dx of dt_x; h, dh, du of dt_u).  stats fp32 [4][B * N] is written by the forward call (NULL:
  * not kept) and read by the backward call.  Backward: dy or dh may be NULL (zero), any output may be NULL; dgate has the
- * gate's shape (dense) and type. */
+ * gate's shape (dense) and type.  The workspace (NULL without parameter gradients) is aligned to 16 bytes. */
 typedef struct {
     const void *x, *u;
     long long xs[2], us[2];

@@ -11,15 +11,27 @@
 // product as they are.  For bf16 the key rows of the first product are fed in a permuted order (key_of) so that these
 // registers hold eight consecutive keys; the other operand (V^T, K^T, Q^T, dO^T) comes out of a row-major LDS image by
 // transposing reads.  The fp32 form runs the same code over the fp32 matrix instruction.
-//   forward      four waves of 32 rows share double-buffered key tiles; the running maximum is moved only when a row
-//                outgrows it by 2^8, so the rescale of the accumulators almost never runs.
+//   forward      four waves of 32 rows share double-buffered tiles of 64 keys (fp32: 32); the running maximum is moved only
+//                when a row outgrows it by 2^8, so the rescale of the accumulators almost never runs.
 //   few rows     (up to 64 a problem: generation, pooling) the four waves share 32 rows and walk key tiles of their own
-//                without a barrier, bound by the bytes of K and V; their results are joined in LDS.
+//                without a barrier; their results are joined in LDS.
+//   short keys   (bf16, up to 256 keys) the whole backward pass in one launch, every probability formed once.
 //   dq           four waves of 32 rows over all key tiles (S, dP, dq);  dk / dv: four waves of 32 keys over all row tiles
-//                of all heads of the group (S, dP, dv, dk).  Seven products where five would do, and no atomics: every
-//                sum runs in a fixed order, results are bitwise reproducible.
-// Where the tiles of a launch leave compute units idle, the inner loop is split over workgroups that leave fp32 partial
-// results in the workspace, joined by a second launch.
+//                of all heads of the group (S, dP, dv, dk).  Seven products where five would do.
+// No atomics: every sum runs in a fixed order, results are bitwise reproducible.  Where the tiles of a launch leave compute
+// units idle, the inner loop is split over workgroups (dk / dv: equal shares of all tiles) that leave fp32 partial results
+// in the workspace, joined by a second launch.
+// Staging: 16-byte loads that land in LDS without a register between; they cost their issue and nothing else, and the next
+// tile's are on their way during a tile's products.
+// Rounding: in bf16, probabilities and dS are rounded to bf16 before the second product of each pair (the matrix
+// instruction's operands; sums, statistics and delta are 32-bit), which leaves results up to 1.5 times as far from the
+// exact ones as rounding the exact result alone; the row sums add the rounded probabilities, so the weights sum to one.
+// Measured (kernel alone; the chip holds about 1.9 GHz under these products):
+//   2 x 4096 rows, 16 heads over 4 of 128, 4609 and 3457 keys, bf16: forward 317 us (854 TFLOP/s), dq 421, dk / dv 640 + 23 for
+//   the join; bound by the matrix pipes with exponentials and conversions in between, one wave a SIMD of each kind waiting.
+//   32 x 12 heads of 64, 576 rows, 197 keys: forward 31 us, backward 73 + 7; 16 x 8 of 80, 1025 rows, 77 keys: 21, 39 + 7.
+//   8 x 1 row, 32 heads over 8 of 128, about 12800 keys: 83 + 5 us, 5.1 TB/s of keys and values.
+//   fp32, 8 x 6 heads of 64, 333 rows, 257 keys: 32, dq 42, dk / dv 46 + 7: 144 workgroups for 256 compute units.
 // Masked keys: their K and V rows are staged as zeros whatever they hold, their scores are -inf.
 #include <algorithm>
 #include <atomic>
@@ -582,7 +594,8 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// up to 64 rows a problem: every wave walks 32-key tiles of its own for the same 32 rows
+// Up to 64 rows a problem: every wave walks 32-key tiles of its own for the same 32 rows.  Bound by the bytes of K and V, which go
+// through registers: a wave waits for its own loads alone, four of them a SIMD cover for each other (5.1 TB/s at 8 x 8 key heads of 128).
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     constexpr int KT = 32, IMG = KT * DP;
@@ -692,7 +705,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     }
 }
 
-// joins the key splits (at most 64) of a forward launch, one wave a row: lane s holds split s's maximum and sum, the partial rows
+// Joins the key splits (at most 64) of a forward launch, one wave a row: lane s holds split s's maximum and sum, the partial rows
 // are then added in split order, eight loads in flight
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long rows) {
@@ -736,7 +749,8 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long row
     if (a.lse && lane == 0) a.lse[st] = l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
-// dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles
+// dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles, two products of 32 x 32 scores
+// and one that turns them into dq; 421 us at the long shape above, 964 TFLOP/s of its own three products
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xattn_dq_kernel(XaArgs a) {
     constexpr int KT = Mx<T>::KT, IMG = KT * DP, NF = DP / Mx<T>::KD;
@@ -1170,7 +1184,7 @@ __device__ __forceinline__ long long stream_first(const XaArgs& a, int b, int hk
 
 // dk and dv: four waves of 32 keys over the row tiles of the whole group.  At bf16 heads beyond 96 the accumulators and both
 // operands would take more than the 256 registers that two waves a SIMD have: V then stays in LDS and the row tiles are
-// half as long (4096 rows of 16 heads, 2 x ~4000 keys: 636 us, 655 with part of it in scratch memory).
+// half as long (the long shape above: 636 us, 655 with part of it in scratch memory).
 template <typename T, int DP, bool VEC> constexpr bool v_in_lds() { return sizeof(T) == 2 && DP == 128 && VEC; }
 template <typename T, int DP, bool VEC> constexpr int row_tile() { return v_in_lds<T, DP, VEC>() ? 32 : Mx<T>::KT; }
 template <typename T, int DP, bool VEC, bool STREAM>
