@@ -198,6 +198,8 @@ XATTN = [  # B, Nq, Nk, Hq, Hk, D, mask
     # backward passes with all keys in one workgroup (whole and in row shares) and in equal shares of many tiles
     (2, 150, 200, 2, 1, 128, "keys"), (1, 700, 100, 1, 1, 64, "none"), (2, 40, 256, 1, 1, 24, "sparse"), (1, 520, 130, 2, 2, 96, "len"),
     (1, 700, 520, 2, 1, 64, "len"), (3, 300, 900, 4, 2, 96, "len"), (70, 10, 300, 1, 1, 16, "len"), (1, 1030, 260, 1, 1, 128, "sparse"),
+    # more problems than small fp32 launches have
+    (25, 130, 70, 4, 2, 40, "keys"), (33, 100, 65, 4, 4, 64, "len"),
     # up to 32 keys, the gradients' delta from one wave's own scores
     (2, 140, 20, 2, 1, 128, "keys"), (1, 300, 32, 2, 2, 96, "len"), (1, 70, 17, 1, 1, 64, "none"), (2, 33, 7, 4, 2, 24, "empty"),
 ]

@@ -13,8 +13,8 @@
 // transposing reads.  The fp32 form runs the same code over the fp32 matrix instruction.
 //   forward      four waves of 32 rows share double-buffered tiles of 64 keys (fp32: 32); the running maximum is moved only
 //                when a row outgrows it by 2^8, so the rescale of the accumulators almost never runs.
-//   few rows     (up to 64 a problem: generation, pooling) the four waves share 32 rows and walk key tiles of their own
-//                without a barrier; their results are joined in LDS.
+//   few rows     (up to 64 a problem: generation, pooling; small fp32 launches) the four waves share 32 rows and walk key
+//                tiles of their own without a barrier; their results are joined in LDS.
 //   short keys   (bf16, up to 256 keys) the whole backward pass in one launch, every probability formed once.
 //   dq           four waves of 32 rows over all key tiles (S, dP, dq);  dk / dv: four waves of 32 keys over all row tiles
 //                of all heads of the group (S, dP, dv, dk).  Seven products where five would do.
@@ -594,7 +594,7 @@ __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Up to 64 rows a problem: every wave walks 32-key tiles of its own for the same 32 rows.  Bound by the bytes of K and V, which go
+// Few rows: every wave walks 32-key tiles of its own for the same 32 rows.  Bound by the bytes of K and V, which go
 // through registers: a wave waits for its own loads alone, four of them a SIMD cover for each other (5.1 TB/s at 8 x 8 key heads of 128).
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
@@ -1471,7 +1471,10 @@ XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D, bool vec) {
     XaPlan p;
     const int R = Hq / Hk * Nq, KT = dt == VITMI_F32 ? 32 : 64;
     const long long bh = (long long)B * Hk;
-    p.few = R <= 64;
+    // also fp32 launches that would leave most matrix pipes without a wave: up to 384 tiles of 32 rows, up to 512 keys (197 rows and
+    // keys of 64, 48 heads, 336 tiles: 17.7 us, by tiles of 128 rows 23.8; 96 heads, 672 tiles: 26.2 and 24.2; 1000 keys: equal,
+    // 4000: 49 and 32)
+    p.few = R <= 64 || (dt == VITMI_F32 && bh * cdiv(R, 32) <= 384 && Nk <= 512);
     p.fwd_tiles = cdiv(R, p.few ? 32 : 128);
     const long long rows = bh * R;
     p.fwd_splits = p.few ? xa_few_splits(bh * p.fwd_tiles, cdiv(Nk, 32)) : xa_splits(dt, bh * p.fwd_tiles, cdiv(Nk, KT), rows, D);
