@@ -720,3 +720,23 @@ def test_second_derivatives_are_refused():
         grad, = torch.autograd.grad(f().square().sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             grad.sum().backward()
+
+
+def test_saved_tensors_that_come_back_in_another_layout():
+    """Hooks that move saved tensors to the host and back compact strided views."""
+    g = gen(31)
+    packed = torch.randn(2, 40, 3, 4, 16, generator=g).to(DEV, H).requires_grad_()
+    x = torch.randn(2, 40, 2, 64, generator=g).to(DEV).requires_grad_()
+    pos = torch.arange(40, device=DEV)[:, None].expand(40, 2)
+
+    def grads():
+        q, k, v = packed.unbind(2)
+        q, k = ops().rope_axes(q, k, pos, (4, 4))
+        y, h = ops().norm_gate_residual(x[:, :, 0], x[:, :, 1], post="layer", pre="rms")
+        o = ops().cross_attn(packed[:, :, 0], k, v)
+        return torch.autograd.grad((q.float().sum() + (o.float() ** 2).sum() + (y * h).sum()), (packed, x))
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -1716,21 +1716,22 @@ def _rope_ladder(sections, base, shared):
 
 
 def _rope_launch(device, xs, outs, pos, ladder, interleaved, shared, inverse):
-    x = xs[0]
+    x, y = xs[0], outs[0]
     B, N, H, D = x.shape
-    sx, sy = x.stride(), outs[0].stride()
-    first = (x.data_ptr(), outs[0].data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], H, 0)
+    s0, s1, s2, _ = x.stride()
+    r0, r1, r2, _ = y.stride()
     second = _NO_TENSOR
     if len(xs) > 1:
-        x, y = xs[1], outs[1]
-        sx, sy = x.stride(), y.stride()
-        second = (x.data_ptr(), y.data_ptr(), sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], x.shape[2], 0)
+        k, ky = xs[1], outs[1]
+        t0, t1, t2, _ = k.stride()
+        u0, u1, u2, _ = ky.stride()
+        second = (k.data_ptr(), ky.data_ptr(), t0, t1, t2, u0, u1, u2, k.shape[2], 0)
     ps = pos.stride()
     if len(ps) == 2:
-        ps = (0, ps[0], ps[1])
+        ps = (0, *ps)
     _call(device, lib.vitmi_rope_axes, "vitmi_rope_axes",
-          _pack_rope(*first, *second, pos.data_ptr(), *ps, *ladder, _POS_TYPES[pos.dtype], _DT[x.dtype], B, N, D, interleaved,
-                     shared, inverse, 0))
+          _pack_rope(x.data_ptr(), y.data_ptr(), s0, s1, s2, r0, r1, r2, H, 0, *second, pos.data_ptr(), *ps, *ladder,
+                     _POS_TYPES[pos.dtype], _DT[x.dtype], B, N, D, interleaved, shared, inverse, 0))
 
 
 class RopeAxesFn(torch.autograd.Function):
@@ -1739,7 +1740,7 @@ class RopeAxesFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, device, ladder, interleaved, shared):
         xs = (q,) if k is None else (q, k)
-        outs = tuple(_dense(t) for t in xs)
+        outs = (_dense(q),) if k is None else (_dense(q), _dense(k))
         _rope_launch(device, xs, outs, pos, ladder, interleaved, shared, False)
         ctx.save_for_backward(pos)
         ctx.meta = (device, ladder, interleaved, shared)
@@ -1782,15 +1783,15 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     pos * base^(-p / P).  A pair is dims (p, P + p), or (2p, 2p + 1) with interleaved; dims from 2P on pass through.
     q and k may be strided views (the slots of a packed projection); the results are dense.  inplace rotates q and k,
     which must not share elements, where they lie, outside of autograd only."""
-    xs = (q,) if k is None else (q, k)
     if inplace:
+        xs = (q,) if k is None else (q, k)
         for t in xs:
             if t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
                 raise ValueError("inplace needs [batch, tokens, heads, head dim] with unit stride over the head dim")
             if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise ValueError("inplace on a broadcast tensor would turn the same memory several times")
     else:
-        xs = tuple(_heads4(n, t) for n, t in zip("qk", xs))
+        xs = (_heads4("q", q),) if k is None else (_heads4("q", q), _heads4("k", k))
     x = xs[0]
     B, N, _, D = x.shape
     _dt(x)
@@ -1803,9 +1804,9 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
         raise ValueError(f"sections {sections} turn {2 * pairs} dims, the head has {D}")
     if pos.dtype not in _POS_TYPES:
         raise TypeError(f"positions are int32, int64 or float32, not {pos.dtype}")
-    ps = tuple(pos.shape)
+    ps = pos.shape
     if ps != (N, len(sections)) and ps != (B, N, len(sections)):
-        raise ValueError(f"pos {ps} must be [{N}, {len(sections)}] or [{B}, {N}, {len(sections)}]")
+        raise ValueError(f"pos {tuple(ps)} must be [{N}, {len(sections)}] or [{B}, {N}, {len(sections)}]")
     graph = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if inplace:
         if graph:
@@ -1815,7 +1816,7 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     device = _one_device(q, k, pos)
     if graph:
         return RopeAxesFn.apply(x, xs[1] if k is not None else None, pos, device, ladder, interleaved, shared_ladder)
-    outs = xs if inplace else tuple(_dense(t) for t in xs)
+    outs = xs if inplace else (_dense(x),) if k is None else (_dense(x), _dense(xs[1]))
     _rope_launch(device, xs, outs, pos, ladder, interleaved, shared_ladder, False)
     if inplace:
         torch.autograd.graph.increment_version(xs)
@@ -1823,25 +1824,37 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     return outs if k is not None else outs[0]
 
 
-def _xattn_pack(q, k, v, o, kv_len, key_mask, scale, lse, do=None, dq=None, dk=None, dv=None):
-    B, Nq, Hq, D = q.shape
-    _, Nk, Hk, _ = k.shape
+# scratch sizes depend on the sizes of a call alone
+_xattn_fwd_bytes = functools.lru_cache(maxsize=4096)(lambda dims: lib.vitmi_cross_attn_fwd_workspace_bytes(*dims))
+_xattn_bwd_bytes = functools.lru_cache(maxsize=4096)(lambda dims: lib.vitmi_cross_attn_bwd_workspace_bytes(*dims))
+
+
+def _xattn_operands(q, k, v):
+    """q, k, v with unit stride over the head dim and their batch, row and head strides."""
     sq, sk, sv = q.stride(), k.stride(), v.stride()
-    sd = do.stride() if do is not None else (0, 0, 0)
-    ptr = lambda t: 0 if t is None else t.data_ptr()
-    return _pack_xattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2],
-                       ptr(kv_len), ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), ptr(lse), ptr(do), sd[0], sd[1],
-                       sd[2], ptr(dq), ptr(dk), ptr(dv), kv_len is not None and kv_len.dtype == torch.int64, _DT[q.dtype], B, Nq, Nk,
-                       Hq, Hk, D, scale, 0)
+    if not (len(sq) == len(sk) == len(sv) == 4 and sq[3] == sk[3] == sv[3] == 1):
+        q, k, v = _heads4("q", q), _heads4("k", k), _heads4("v", v)
+        sq, sk, sv = q.stride(), k.stride(), v.stride()
+    return q, k, v, (sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
 
 
-def _xattn_fwd(device, q, k, v, kv_len, key_mask, scale, keep_lse):
-    B, Nq, Hq, D = q.shape
+def _xattn_pack(q, k, v, o, strides, kv_len, key_mask, lse, meta, do=None, dq=None, dk=None, dv=None):
+    scale, dims = meta
+    sd = (0, 0, 0) if do is None else do.stride()
+    return _pack_xattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), *strides, 0 if kv_len is None else kv_len.data_ptr(),
+                       0 if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0),
+                       0 if lse is None else lse.data_ptr(), 0 if do is None else do.data_ptr(), sd[0], sd[1], sd[2],
+                       0 if dq is None else dq.data_ptr(), 0 if dk is None else dk.data_ptr(), 0 if dv is None else dv.data_ptr(),
+                       kv_len is not None and kv_len.dtype == torch.int64, *dims, scale, 0)
+
+
+def _xattn_fwd(device, q, k, v, strides, kv_len, key_mask, meta, keep_lse):
+    dims = meta[1]
     o = _dense(q)
-    lse = torch.empty((B, Hq * Nq), dtype=torch.float32, device=q.device) if keep_lse else None
-    n = lib.vitmi_cross_attn_fwd_workspace_bytes(_DT[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D)
+    lse = torch.empty((dims[1], dims[4] * dims[2]), dtype=torch.float32, device=q.device) if keep_lse else None
+    n = _xattn_fwd_bytes(dims)
     ws = _ws(n, q.device) if n else None
-    _call(device, lib.vitmi_cross_attn_fwd, "vitmi_cross_attn_fwd", _xattn_pack(q, k, v, o, kv_len, key_mask, scale, lse), _p(ws))
+    _call(device, lib.vitmi_cross_attn_fwd, "vitmi_cross_attn_fwd", _xattn_pack(q, k, v, o, strides, kv_len, key_mask, lse, meta), _p(ws))
     return o, lse
 
 
@@ -1849,10 +1862,10 @@ class CrossAttnFn(torch.autograd.Function):
     """The node behind cross_attn: keeps q, k, v, the output and a log-sum-exp per row; probabilities are formed again."""
 
     @staticmethod
-    def forward(ctx, q, k, v, kv_len, key_mask, scale, device):
-        o, lse = _xattn_fwd(device, q, k, v, kv_len, key_mask, scale, True)
+    def forward(ctx, q, k, v, strides, kv_len, key_mask, meta, device):
+        o, lse = _xattn_fwd(device, q, k, v, strides, kv_len, key_mask, meta, True)
         ctx.save_for_backward(q, k, v, o, lse, kv_len, key_mask)
-        ctx.meta = (scale, device)
+        ctx.meta = (meta, device)
         return o
 
     @staticmethod
@@ -1860,8 +1873,9 @@ class CrossAttnFn(torch.autograd.Function):
     def backward(ctx, do):
         q, k, v, o, lse, kv_len, key_mask = ctx.saved_tensors
         if _PS2 is not None:                # a replay forms no input gradients
-            return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None,) * 4
-        scale, device = ctx.meta
+            return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None,) * 5
+        meta, device = ctx.meta
+        q, k, v, strides = _xattn_operands(q, k, v)       # of the saved ones: a hook may have laid them out anew
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq = _dense(q) if need_q else None
         dk, dv = (_dense(k), _dense(v)) if need_k or need_v else (None, None)
@@ -1871,11 +1885,10 @@ class CrossAttnFn(torch.autograd.Function):
                     t.zero_()
         else:
             do = _heads4("gradient", do)
-            B, Nq, Hq, D = q.shape
-            ws = _ws(lib.vitmi_cross_attn_bwd_workspace_bytes(_DT[q.dtype], B, Nq, k.shape[1], Hq, k.shape[2], D), q.device)
+            ws = _ws(_xattn_bwd_bytes(meta[1]), q.device)
             _call(device, lib.vitmi_cross_attn_bwd, "vitmi_cross_attn_bwd",
-                  _xattn_pack(q, k, v, o, kv_len, key_mask, scale, lse, do, dq, dk, dv), ws.data_ptr())
-        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None
+                  _xattn_pack(q, k, v, o, strides, kv_len, key_mask, lse, meta, do, dq, dk, dv), ws.data_ptr())
+        return dq, dk if need_k else None, dv if need_v else None, None, None, None, None, None
 
 
 def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
@@ -1886,10 +1899,11 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
     Which keys count: kv_len [B] (int32 / int64), the first kv_len[b] of sample b (values outside 0 .. Nk are taken as
     the nearer end), or key_mask [B, Nk] bool, True = attend, or all.  The rows of other keys may hold anything, their
     gradients are zero.  A sample without a key to attend to gives zeros, and zero gradients."""
-    q, k, v = _heads4("q", q), _heads4("k", k), _heads4("v", v)
-    if not q.dtype == k.dtype == v.dtype:
+    q, k, v, strides = _xattn_operands(q, k, v)
+    dtype = q.dtype
+    if dtype != k.dtype or dtype != v.dtype:
         raise TypeError(f"q, k and v must share a dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    _dt(q)
+    dt = _DT[dtype] if dtype in _DT else _dt(q)
     B, Nq, Hq, D = q.shape
     Bk, Nk, Hk, Dk = k.shape
     if Bk != B or Dk != D or k.shape != v.shape:
@@ -1913,9 +1927,10 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale {scale} must be positive and finite")
     device = _one_device(q, k, v, kv_len, key_mask)
+    meta = (scale, (dt, B, Nq, Nk, Hq, Hk, D))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return CrossAttnFn.apply(q, k, v, kv_len, key_mask, scale, device)
-    return _xattn_fwd(device, q, k, v, kv_len, key_mask, scale, False)[0]
+        return CrossAttnFn.apply(q, k, v, strides, kv_len, key_mask, meta, device)
+    return _xattn_fwd(device, q, k, v, strides, kv_len, key_mask, meta, False)[0]
 
 
 _NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
@@ -1926,10 +1941,9 @@ def _ngr_pack(x, u, params, meta, y, h, stats, dy=None, dh=None, grads=(None,) *
     res_scale, post, pre, eps = meta
     B, N, D = x.shape
     sx, su = x.stride(), u.stride()
-    ptr = lambda t: 0 if t is None else t.data_ptr()
     gate_stride = gate.stride(0) if gate is not None and gate.dim() == 2 else 0
-    return _pack_ngr(x.data_ptr(), u.data_ptr(), sx[0], sx[1], su[0], su[1], ptr(y), ptr(h), ptr(gate), gate_stride, ptr(branch_scale),
-                     ptr(post_w), ptr(post_b), ptr(pre_w), ptr(pre_b), ptr(stats), ptr(dy), ptr(dh), *map(ptr, grads),
+    ptrs = [0 if t is None else t.data_ptr() for t in (y, h, gate, branch_scale, post_w, post_b, pre_w, pre_b, stats, dy, dh, *grads)]
+    return _pack_ngr(x.data_ptr(), u.data_ptr(), sx[0], sx[1], su[0], su[1], *ptrs[:3], gate_stride, *ptrs[3:],
                      0 if gate is None else _DT[gate.dtype], _DT[x.dtype], _DT[u.dtype], B, N, D, post, pre, res_scale, eps)
 
 
@@ -2011,9 +2025,10 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
             if t is not None:
                 if kind is None:
                     raise ValueError(f"{name}_{what} without {name}")
-                if t.dim() != 1 or t.shape[0] != D or t.dtype != torch.float32:
+                if t.shape != (D,) or t.dtype != torch.float32:
                     raise ValueError(f"{name}_{what} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
-                t = t.contiguous()
+                if t.stride(0) != 1:
+                    t = t.contiguous()
             vectors.append(t)
     if gate is not None:
         _dt(gate)
