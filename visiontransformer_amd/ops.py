@@ -1936,15 +1936,36 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
 _NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
 
 
-def _ngr_pack(x, u, params, meta, y, h, stats, dy=None, dh=None, grads=(None,) * 7):
+def _ngr_vector(name, kind, t, D):
+    if t is None:
+        return None
+    if kind is None:
+        raise ValueError(f"{name} without {name.split('_')[0]}")
+    if t.shape != (D,) or t.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
+    return t if t.stride(0) == 1 else t.contiguous()
+
+
+_NGR_NO_GRADS = (0,) * 9
+
+
+def _ngr_pack(x, u, params, meta, y, h, stats, grads=_NGR_NO_GRADS):
     gate, branch_scale, post_w, post_b, pre_w, pre_b = params
     res_scale, post, pre, eps = meta
     B, N, D = x.shape
-    sx, su = x.stride(), u.stride()
-    gate_stride = gate.stride(0) if gate is not None and gate.dim() == 2 else 0
-    ptrs = [0 if t is None else t.data_ptr() for t in (y, h, gate, branch_scale, post_w, post_b, pre_w, pre_b, stats, dy, dh, *grads)]
-    return _pack_ngr(x.data_ptr(), u.data_ptr(), sx[0], sx[1], su[0], su[1], *ptrs[:3], gate_stride, *ptrs[3:],
-                     0 if gate is None else _DT[gate.dtype], _DT[x.dtype], _DT[u.dtype], B, N, D, post, pre, res_scale, eps)
+    x0, x1, _ = x.stride()
+    u0, u1, _ = u.stride()
+    gate_ptr = gate_stride = gate_dt = 0
+    if gate is not None:
+        gate_ptr, gate_dt = gate.data_ptr(), _DT[gate.dtype]
+        if gate.dim() == 2:
+            gate_stride = gate.stride(0)
+    return _pack_ngr(x.data_ptr(), u.data_ptr(), x0, x1, u0, u1, 0 if y is None else y.data_ptr(), 0 if h is None else h.data_ptr(),
+                     gate_ptr, gate_stride, 0 if branch_scale is None else branch_scale.data_ptr(),
+                     0 if post_w is None else post_w.data_ptr(), 0 if post_b is None else post_b.data_ptr(),
+                     0 if pre_w is None else pre_w.data_ptr(), 0 if pre_b is None else pre_b.data_ptr(),
+                     0 if stats is None else stats.data_ptr(), *grads, gate_dt, _DT[x.dtype], _DT[u.dtype], B, N, D, post, pre,
+                     res_scale, eps)
 
 
 def _ngr_fwd(device, x, u, params, meta, keep):
@@ -1995,7 +2016,7 @@ class NormGateResidualFn(torch.autograd.Function):
                 gate = params[0]
                 ws = _ws(lib.vitmi_norm_gate_residual_bwd_workspace_bytes(B, N, D, gate is not None and gate.dim() == 2), x.device)
             _call(device, lib.vitmi_norm_gate_residual_bwd, "vitmi_norm_gate_residual_bwd",
-                  _ngr_pack(x, u, params, meta, None, None, stats, dy, dh, grads), _p(ws))
+                  _ngr_pack(x, u, params, meta, None, None, stats, [0 if t is None else t.data_ptr() for t in (dy, dh, *grads)]), _p(ws))
         return (*grads[:3], None, *grads[3:], None, None)
 
 
@@ -2012,27 +2033,20 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
     if x.dim() != 3 or x.shape != u.shape:
         raise ValueError(f"x and u must be [batch, tokens, dim] alike, got {tuple(x.shape)} and {tuple(u.shape)}")
     B, N, D = x.shape
-    if _dt(x) == BF16 and _dt(u) == F32:
-        raise TypeError("a bf16 residual stream takes bf16 branches")
-    _dt(u)
+    if x.dtype != u.dtype or x.dtype not in _DT:
+        if _dt(x) == BF16 and _dt(u) == F32:
+            raise TypeError("a bf16 residual stream takes bf16 branches")
+        _dt(u)
     if not 1 <= D <= 8192:
         raise ValueError(f"rows of {D} are outside 1 .. 8192")
-    vectors = []
-    for name, kind, w, b in (("post", post, post_weight, post_bias), ("pre", pre, pre_weight, pre_bias)):
-        if kind not in _NORM_KINDS:
-            raise ValueError(f'{name}={kind!r}: "layer", "rms" or None')
-        for what, t in (("weight", w), ("bias", b)):
-            if t is not None:
-                if kind is None:
-                    raise ValueError(f"{name}_{what} without {name}")
-                if t.shape != (D,) or t.dtype != torch.float32:
-                    raise ValueError(f"{name}_{what} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
-                if t.stride(0) != 1:
-                    t = t.contiguous()
-            vectors.append(t)
+    if post not in _NORM_KINDS or pre not in _NORM_KINDS:
+        raise ValueError(f'post={post!r}, pre={pre!r}: "layer", "rms" or None')
+    vectors = (_ngr_vector("post_weight", post, post_weight, D), _ngr_vector("post_bias", post, post_bias, D),
+               _ngr_vector("pre_weight", pre, pre_weight, D), _ngr_vector("pre_bias", pre, pre_bias, D))
     if gate is not None:
-        _dt(gate)
-        if tuple(gate.shape) not in ((D,), (B, D)):
+        if gate.dtype not in _DT:
+            _dt(gate)
+        if gate.shape != (D,) and gate.shape != (B, D):
             raise ValueError(f"gate {tuple(gate.shape)} must be [{D}] or [{B}, {D}]")
         if gate.stride(-1) != 1 or (gate.dim() == 2 and gate.stride(0) < D):
             gate = gate.contiguous()
