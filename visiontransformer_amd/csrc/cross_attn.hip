@@ -117,6 +117,14 @@ __device__ __forceinline__ f32x4 acc_frag(const f32x16& p, int n, float) {
     return f32x4{p[4 * n], p[4 * n + 1], p[4 * n + 2], p[4 * n + 3]};
 }
 
+// what the rounding to `hi` = acc_frag(p, n) left over, rounded in turn
+__device__ __forceinline__ bf16x8 rest_frag(const f32x16& p, int n, const bf16x8& hi) {
+    bf16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (bf16_t)(p[8 * n + j] - (float)hi[j]);
+    return r;
+}
+
 // l plus the sum of a fragment of probabilities: the rounded ones that the output is summed of, two an instruction; fp32 adds its
 // own as they are formed
 __device__ __forceinline__ float add_frag(const bf16x8& p, float l) {
@@ -860,10 +868,11 @@ __device__ __forceinline__ float half_wave_sum(float v) {
 // at heads of 64 they take longer than the products) and feed dk and dv as in xattn_dkv_kernel.  Every wave also leaves its dS
 // as [key][row] in LDS -- the packed fragments as they are, two 16-byte writes a lane -- from where the tile's dq^T =
 // K^T dS^T is formed over all keys, in pieces of 32 dims that the waves take in turns, a tile behind (NOW: a piece a wave, at
-// once, which needs one dS image in place of two).  delta is formed from dO and O on the way in; O is a
-// rounded one, which tells where few keys share it (its half step against dS: at 7 keys the gradients are 0.0030 off, 0.0024 without
-// it, at 77 0.0024 either way), so that with up to 32 keys (ONE), all of one wave, delta = sum_k p dp
-// comes from their own registers.
+// once, which needs one dS image in place of two).  delta is formed from dO and O on the way in.
+// Up to 32 keys (ONE) are all of one wave.  Few keys do not average roundings out, that of O, through delta, among them: with 7 keys
+// gradients would be 0.0030 off, with 77 0.0024, where rounding the exact ones leaves 0.0017.  So delta = sum_k p dp is summed
+// from the scores there, and P and dS enter the products as two bf16 terms each, a rounding and its rest: 0.0018 with 7 keys.
+// The products are a small part of so few keys' work.
 template <int DP, int NW, int SUB, bool ONE>
 __global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
     typedef bf16_t T;
@@ -982,6 +991,10 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
         for (int kb = 0; kb < blocks; ++kb) {
             mma(acc, col_frag<NK>(kimg + kb * 1024, 0, j, lane), col_frag<NK>(di + kb * 1024, 0, 0, lane));
             mma(alt, col_frag<NK>(kimg + kb * 1024, 16, j, lane), col_frag<NK>(di + kb * 1024, 16, 0, lane));
+            if (ONE) {                                    // the rests lie where a second wave's dS would
+                mma(acc, col_frag<NK>(kimg, 0, j, lane), col_frag<NK>(di + 1024, 0, 0, lane));
+                mma(alt, col_frag<NK>(kimg, 16, j, lane), col_frag<NK>(di + 1024, 16, 0, lane));
+            }
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[e] += alt[e];
@@ -1046,6 +1059,15 @@ __global__ __launch_bounds__(64 * NW, 2) void xattn_bwd_short_kernel(XaArgs a) {
                     for (int d = 0; d < NP; ++d) {
                         mma(dv[d], col_frag<QT>(img + IMG, 32 * sub + 16 * g, d, lane), pf);
                         mma(dk[d], col_frag<QT>(img, 32 * sub + 16 * g, d, lane), df);
+                    }
+                    if (ONE) {
+                        const bf16x8 pr = rest_frag(s[sub], g, pf), dr = rest_frag(dp[sub], g, df);
+                        ds_at(pair, sub, 2 * g + h)[32 * 32 / 8] = dr;
+#pragma unroll
+                        for (int d = 0; d < NP; ++d) {
+                            mma(dv[d], col_frag<QT>(img + IMG, 32 * sub + 16 * g, d, lane), pr);
+                            mma(dk[d], col_frag<QT>(img, 32 * sub + 16 * g, d, lane), dr);
+                        }
                     }
                 }
             }
