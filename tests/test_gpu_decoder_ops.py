@@ -740,3 +740,30 @@ def test_saved_tensors_that_come_back_in_another_layout():
         got = grads()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+SHORT = [  # B, Nq, Nk, Hq, Hk, D, dtype, lengths: few or no live keys of many, in launches that the padded sizes give many workgroups
+    (1, 512, 1024, 1, 1, 64, H, (100,)), (2, 576, 4096, 4, 4, 64, H, (300, 200)), (2, 333, 2048, 6, 6, 64, F, (100, 200)),
+    (4, 512, 1024, 2, 2, 64, H, (128,) * 4), (4, 512, 2048, 4, 2, 128, H, (256, 128, 64, 300)), (2, 1030, 2000, 1, 1, 128, H, (100, 0)),
+    (3, 400, 1500, 2, 1, 40, F, (1, 0, 1)), (3, 520, 1500, 2, 2, 64, H, (0, 1, 0)), (2, 520, 1500, 2, 2, 64, H, (0, 0)),
+    (2, 300, 1200, 2, 1, 33, H, (5, 1200)), (130, 300, 600, 1, 1, 16, H, (3,) * 130),
+]
+
+
+@pytest.mark.parametrize("case", SHORT, ids=lambda c: f"{c[:6]}-{'bf16' if c[6] == H else 'f32'}-{sum(c[7])}")
+def test_cross_attn_gradients_of_short_lengths_in_a_dirty_workspace(case, monkeypatch):
+    """Lengths far below the padding; scratch memory holds NaN beforehand, so that nothing may be read that was not written."""
+    B, Nq, Nk, Hq, Hk, D, dtype, lens = case
+    q, kv, do, _, _ = xattn_inputs((B, Nq, Nk, Hq, Hk, D, "none"), dtype, seed=5)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    allowed = orc.allowed_keys(B, Nk, lens)
+    ref, tol = attention_bounds(q.double(), kv[:, :, 0].double(), kv[:, :, 1].double(), allowed, do.double(), dtype, half_step(q))
+    monkeypatch.setattr(ops(), "_ws", lambda n, device: torch.full((max(int(n), 16),), 255, dtype=torch.uint8, device=device))
+    qd, kvd = q.to(DEV).requires_grad_(), kv.to(DEV).requires_grad_()
+    o = ops().cross_attn(qd, kvd[:, :, 0], kvd[:, :, 1], kv_len=lens.to(DEV))
+    within("o", o, ref["o"], tol["o"])
+    dq, dkv = torch.autograd.grad(o, (qd, kvd), do.to(DEV))
+    within("dq", dq, ref["dq"], tol["dq"])
+    within("dk", dkv[:, :, 0], ref["dk"], tol["dk"])
+    within("dv", dkv[:, :, 1], ref["dv"], tol["dv"])
+    assert not dkv[~allowed.to(DEV)].any()

@@ -37,6 +37,7 @@
 #include <atomic>
 
 #include "common.h"
+#include "shares.h"
 
 namespace {
 
@@ -1133,17 +1134,9 @@ __global__ __launch_bounds__(256) void xattn_short_join_kernel(XaArgs a, int per
 
 
 // How the dk / dv launch cuts its work: a unit is one row tile against one live tile of 128 keys.  Streamed, every workgroup
-// takes an equal share of the units in a row -- the end of one key tile, whole ones, the start of another -- because whole
-// key tiles, of which there may be a few more than the chip holds at once, would leave it idle for up to half the time.
-// With three or more workgroups a key tile the shares end at tile borders.  Lengths per sample are only known here, so
-// each wave counts the live tiles itself (64 samples a step).
-struct Stream {
-    long long units;      // in all
-    int rt, nb;           // row tiles a key tile, workgroups that share the units
-    __device__ __forceinline__ long long begin(int i) const { return units * i / nb; }
-    // the workgroup that holds unit x
-    __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * nb + units - 1) / units) - 1; }
-};
+// takes an equal share of the units in a row (shares.h), because whole key tiles, of which there may be a few more than the
+// chip holds at once, would leave it idle for up to half the time.  Lengths per sample are only known here, so each wave
+// counts the live tiles itself (64 samples a step).
 __device__ __forceinline__ int lanes_scan(int v, int lane) {     // inclusive sums over the lanes
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -1153,7 +1146,7 @@ __device__ __forceinline__ int lanes_scan(int v, int lane) {     // inclusive su
     return v;
 }
 __device__ __forceinline__ int live_tiles(const XaArgs& a, int b) { return (keys_of(a, b) + 127) >> 7; }
-__device__ __forceinline__ Stream stream_of(const XaArgs& a, int grid, int row_tiles, int lane) {
+__device__ __forceinline__ Shares stream_of(const XaArgs& a, int grid, int row_tiles, int lane) {
     long long tiles = 0;
     if (!a.kv_len) {
         tiles = (long long)a.B * a.tiles;
@@ -1161,12 +1154,7 @@ __device__ __forceinline__ Stream stream_of(const XaArgs& a, int grid, int row_t
         for (int b0 = 0; b0 < a.B; b0 += 64)
             tiles += __shfl(lanes_scan(b0 + lane < a.B ? live_tiles(a, b0 + lane) : 0, lane), 63, 64);
     }
-    tiles = uniform(tiles * a.Hk);
-    Stream s;
-    s.rt = row_tiles;
-    s.units = tiles * row_tiles;
-    s.nb = tiles > 0 && grid >= 3 * tiles ? (int)(grid / tiles * tiles) : grid;
-    return s;
+    return shares_of(uniform(tiles * a.Hk), grid, row_tiles);
 }
 // sample, key head and key tile of live tile tau (samples in order, then heads, then tiles)
 __device__ __forceinline__ void stream_tile(const XaArgs& a, long long tau, int lane, int& b, int& hk, int& kt) {
@@ -1221,8 +1209,9 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int blk = xa_block(), RT = (a.R + QT - 1) / QT;
     long long u = 0, u1 = 1;                              // not streamed: one key tile a workgroup
+    Shares str = {};
     if (STREAM) {
-        const Stream str = stream_of(a, gridDim.x, RT, lane);
+        str = stream_of(a, gridDim.x, RT, lane);
         if (blk >= str.nb) return;
         u = str.begin(blk);
         u1 = str.begin(blk + 1);
@@ -1231,11 +1220,11 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
     for (int part = 0; u < u1; ++part) {
         int b, hk, kt, t0 = 0, t1 = RT;
         if (STREAM) {
-            const long long tau = u / RT;
-            t0 = (int)(u - tau * RT);
-            t1 = (int)(t0 + (u1 - u) < RT ? t0 + (u1 - u) : RT);
+            const Share now = str.piece(u, u1);
+            t0 = now.t0;
+            t1 = now.t1;
             u += t1 - t0;
-            stream_tile(a, tau, lane, b, hk, kt);
+            stream_tile(a, now.tile, lane, b, hk, kt);
             b = __builtin_amdgcn_readfirstlane(b);
             hk = __builtin_amdgcn_readfirstlane(hk);
             kt = __builtin_amdgcn_readfirstlane(kt);
@@ -1348,7 +1337,7 @@ __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xa
             store_acc<T, VEC, DP>(in ? (T*)a.dk + row : nullptr, dk, a.scale, h, a.D);
             store_acc<T, VEC, DP>(in ? (T*)a.dv + row : nullptr, dv, 1.f, h, a.D);
         } else {                                          // a workgroup's first and its last part may be shares of a tile
-            float* slot = a.part_kv + ((2ll * blk + (part > 0)) * 2 * 128 + wave * 32 + (lane & 31)) * a.D;
+            float* slot = a.part_kv + (Shares::slot(blk, part) * 2 * 128 + wave * 32 + (lane & 31)) * a.D;
             store_acc<float, VEC, DP>(in ? slot : nullptr, dk, 1.f, h, a.D);
             store_acc<float, VEC, DP>(in ? slot + 128ll * a.D : nullptr, dv, 1.f, h, a.D);
         }
@@ -1370,12 +1359,12 @@ __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(XaArgs a, int grid,
     const bool live = kt < live_tiles(a, b);
     int i0 = 0, i1 = -1, part0 = 0;
     if (live) {
-        const Stream str = stream_of(a, grid, row_tiles, lane);
+        const Shares str = stream_of(a, grid, row_tiles, lane);
         const long long x0 = (stream_first(a, b, hk, lane) + kt) * row_tiles;
         i0 = str.owner(x0);
         i1 = str.owner(x0 + row_tiles - 1);
         if (i0 == i1) return;                             // written in full by one workgroup
-        part0 = str.begin(i0) < x0;                       // the tile is the last, not the first, of that workgroup's share
+        part0 = str.part_of(i0, x0);
     }
     const bool v4 = a.D % 4 == 0;
     const int w = v4 ? 4 : 1, per = a.D / w;
@@ -1386,7 +1375,7 @@ __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(XaArgs a, int grid,
             float v[4][4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const float* p = a.part_kv + (((2ll * (i + c) + (i + c == i0 ? part0 : 0)) * 2 + m) * 128 + (blockIdx.x & 15) * 8 + key) * a.D + d;
+                const float* p = a.part_kv + ((Shares::slot(i + c, i + c == i0 ? part0 : 0) * 2 + m) * 128 + (blockIdx.x & 15) * 8 + key) * a.D + d;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) v[c][q] = 0.f;
                 if (i + c <= i1) {
