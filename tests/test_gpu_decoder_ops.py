@@ -767,3 +767,19 @@ def test_cross_attn_gradients_of_short_lengths_in_a_dirty_workspace(case, monkey
     within("dk", dkv[:, :, 0], ref["dk"], tol["dk"])
     within("dv", dkv[:, :, 1], ref["dv"], tol["dv"])
     assert not dkv[~allowed.to(DEV)].any()
+
+
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,D,mask", [(2, 1, 7, 2, 2, 64, "none"), (3, 1, 197, 3, 3, 64, "none"), (2, 1, 5000, 8, 2, 128, "len"),
+                                                 (2, 5, 77, 4, 1, 40, "keys"), (2, 60, 300, 1, 1, 33, "none"), (1, 1, 3, 1, 1, 96, "none")])
+def test_cross_attn_of_few_rows_rounds_nothing_but_its_result(B, Nq, Nk, Hq, Hk, D, mask):
+    """bf16, up to 64 rows a key head: P enters its product as two bf16 terms, off by at most 2^-8 of a rest that is at most 2^-8
+    of P, and the row sums add the 32-bit P; so the bound is that of 32-bit arithmetic plus 2^-16 of P |v|."""
+    q, kv, do, lens, keep = xattn_inputs((B, Nq, Nk, Hq, Hk, D, mask), H, seed=9)
+    allowed = orc.allowed_keys(B, Nk, lens, keep)
+    q64, k64, v64 = q.double(), kv[:, :, 0].double(), kv[:, :, 1].double()
+    ref, tol = attention_bounds(q64, k64, v64, allowed, do.double(), F, half_step(q))
+    weight = torch.zeros_like(ref["o"])
+    for b in range(B):
+        weight[b:b + 1] = orc.cross_attn(q64[b:b + 1], k64[b:b + 1], v64[b:b + 1].abs(), allowed[b:b + 1])
+    m = dict(kv_len=None if lens is None else lens.to(DEV), key_mask=None if keep is None else keep.to(DEV))
+    within("o", ops().cross_attn(q.to(DEV), kv[:, :, 0].to(DEV), kv[:, :, 1].to(DEV), **m), ref["o"], tol["o"] + 2.0 ** -16 * weight)

@@ -410,8 +410,9 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned m, int h) {
         if (!((m >> key_of<T>(e, h)) & 1)) s[e] = -INFINITY;
 }
 
-// 32 staged keys (their images' rows from kimg, vimg on) against the lane's query: running softmax and o^T += V^T P^T
-template <typename T, int DP, int KT>
+// 32 staged keys (their images' rows from kimg, vimg on) against the lane's query: running softmax and o^T += V^T P^T.  TWO: P as a
+// rounding and its rest, and its own sum in 32 bits, so that nothing but the result is rounded.
+template <typename T, int DP, int KT, bool TWO = false>
 __device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typename Mx<T>::frag (&qf)[DP / Mx<T>::KD], unsigned mask, float c,
                                        f32x16 (&o)[DP / 32], float& m, float& l, int lane) {
     f32x16 s;
@@ -434,14 +435,24 @@ __device__ __forceinline__ void attend(const T* kimg, const T* vimg, const typen
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -m));
-        if (sizeof(T) == 4) l += s[e];
+        if (sizeof(T) == 4 || TWO) l += s[e];
     }
 #pragma unroll
     for (int n = 0; n < 32 / Mx<T>::KD; ++n) {
         const typename Mx<T>::frag pf = acc_frag(s, n, T());
-        l = add_frag(pf, l);
+        if constexpr (TWO) {
+            const typename Mx<T>::frag pr = rest_frag(s, n, pf);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<KT>(vimg, n * Mx<T>::KD, d, lane), pf);
+            for (int d = 0; d < DP / 32; ++d) {
+                const typename Mx<T>::frag vf = col_frag<KT>(vimg, n * Mx<T>::KD, d, lane);
+                mma(o[d], vf, pf);
+                mma(o[d], vf, pr);
+            }
+        } else {
+            l = add_frag(pf, l);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) mma(o[d], col_frag<KT>(vimg, n * Mx<T>::KD, d, lane), pf);
+        }
     }
 }
 
@@ -653,7 +664,7 @@ __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
             st.fetch(kp, a.ks[1], vp, a.vs[1], (kt + 4) * KT, mw.next, nullptr, nullptr, a.D, lane, false);
             mw.advance(a, kt, lane);
         }
-        if (mk) attend<T, DP, KT>(img, img + IMG, qf, (unsigned)mk, a.c, o, m, l, lane);
+        if (mk) attend<T, DP, KT, sizeof(T) == 2>(img, img + IMG, qf, (unsigned)mk, a.c, o, m, l, lane);
         wave_fence();
     }
     l += other_half(l);
