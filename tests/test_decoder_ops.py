@@ -399,3 +399,14 @@ def test_shares_of_live_tiles_are_all_written_before_they_are_joined(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", str(src), "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout == "ok\n", r.stdout
+
+
+def test_tracing_is_refused():
+    """A traced program would hold the empty result tensors alone, or nodes for the sizes of the traced call, unchecked."""
+    x, pos = torch.zeros(2, 3, 4, 16), torch.zeros(3, 2, dtype=torch.int64)
+    for grad in (False, True):
+        a, u = x.clone().requires_grad_(grad), torch.zeros(2, 3, 8).requires_grad_(grad)
+        for f, t in ((lambda t: ops.rope_axes(t, None, pos, (4, 4)), a), (lambda t: ops.rope_axes(t, None, pos, (4, 4), inplace=True), a),
+                     (lambda t: ops.cross_attn(t, t, t), a), (lambda t: ops.norm_gate_residual(t, t)[0], u)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                torch.jit.trace(f, (t,), check_trace=False)

@@ -783,3 +783,29 @@ def test_cross_attn_of_few_rows_rounds_nothing_but_its_result(B, Nq, Nk, Hq, Hk,
         weight[b:b + 1] = orc.cross_attn(q64[b:b + 1], k64[b:b + 1], v64[b:b + 1].abs(), allowed[b:b + 1])
     m = dict(kv_len=None if lens is None else lens.to(DEV), key_mask=None if keep is None else keep.to(DEV))
     within("o", ops().cross_attn(q.to(DEV), kv[:, :, 0].to(DEV), kv[:, :, 1].to(DEV), **m), ref["o"], tol["o"] + 2.0 ** -16 * weight)
+
+
+@pytest.mark.parametrize("record", [True, False])
+def test_forward_mode_and_functional_transforms_are_refused(record):
+    """A tangent or a batch must not be dropped without a word, with or without recording; without either the results are
+    the usual ones."""
+    from torch.autograd import forward_ad
+    x, u, pos = torch.randn(2, 5, 2, 16, device=DEV), torch.randn(2, 5, 16, device=DEV), torch.arange(5, device=DEV)[:, None]
+    calls = ((lambda t: ops().rope_axes(t, None, pos, (8,)), x), (lambda t: ops().cross_attn(x, t, x), x),
+             (lambda t: ops().norm_gate_residual(u, t, post="rms")[0], u), (lambda t: ops().norm_gate_residual(u, u, gate=t[0, 0])[0], u))
+    with torch.set_grad_enabled(record):
+        for f, t in calls:
+            want = f(t)
+            with forward_ad.dual_level():
+                assert torch.equal(f(t), want)
+                with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+                    f(forward_ad.make_dual(t, torch.ones_like(t)))
+            for transform in (lambda: torch.func.vmap(f)(t[None]), lambda: torch.func.jvp(f, (t,), (t,)),
+                              lambda: torch.func.grad(lambda a: f(a).sum())(t)):
+                with pytest.raises(RuntimeError, match="functorch|vmap|jvp|setup_context"):
+                    transform()
+        buf = x.clone()
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="outside of autograd"):
+                ops().rope_axes(forward_ad.make_dual(buf, x), None, pos, (8,), inplace=True)
+        assert torch.equal(buf, x)

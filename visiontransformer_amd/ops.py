@@ -11,6 +11,7 @@ import struct
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -1685,6 +1686,17 @@ def _one_device(first, *rest):
     return d
 
 
+def _through_node(name, *ts):
+    """Whether a call goes through its autograd node: where a gradient is wanted, and where forward-mode or functional
+    transforms are at work, whose tangents or batches a launch would drop and the node refuses.  A traced program would lose
+    the launch, or keep the node with the sizes of the call it saw and without the checks of later ones."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{name} cannot be traced")
+    if forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active():
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
 def _dense(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
@@ -1783,6 +1795,7 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     pos * base^(-p / P).  A pair is dims (p, P + p), or (2p, 2p + 1) with interleaved; dims from 2P on pass through.
     q and k may be strided views (the slots of a packed projection); the results are dense.  inplace rotates q and k,
     which must not share elements, where they lie, outside of autograd only."""
+    node = _through_node("rope_axes", q, k)
     if inplace:
         xs = (q,) if k is None else (q, k)
         for t in xs:
@@ -1807,14 +1820,13 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     ps = pos.shape
     if ps != (N, len(sections)) and ps != (B, N, len(sections)):
         raise ValueError(f"pos {tuple(ps)} must be [{N}, {len(sections)}] or [{B}, {N}, {len(sections)}]")
-    graph = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if inplace:
-        if graph:
+        if node:
             raise RuntimeError("rope_axes(inplace=True) is for tensors outside of autograd")
         if k is not None and _overlap(q, k):
             raise ValueError("inplace needs q and k apart")
     device = _one_device(q, k, pos)
-    if graph:
+    if node:
         return RopeAxesFn.apply(x, xs[1] if k is not None else None, pos, device, ladder, interleaved, shared_ladder)
     outs = xs if inplace else (_dense(x),) if k is None else (_dense(x), _dense(xs[1]))
     _rope_launch(device, xs, outs, pos, ladder, interleaved, shared_ladder, False)
@@ -1899,6 +1911,7 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
     Which keys count: kv_len [B] (int32 / int64), the first kv_len[b] of sample b (values outside 0 .. Nk are taken as
     the nearer end), or key_mask [B, Nk] bool, True = attend, or all.  The rows of other keys may hold anything, their
     gradients are zero.  A sample without a key to attend to gives zeros, and zero gradients."""
+    node = _through_node("cross_attn", q, k, v)
     q, k, v, strides = _xattn_operands(q, k, v)
     dtype = q.dtype
     if dtype != k.dtype or dtype != v.dtype:
@@ -1928,7 +1941,7 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
         raise ValueError(f"scale {scale} must be positive and finite")
     device = _one_device(q, k, v, kv_len, key_mask)
     meta = (scale, (dt, B, Nq, Nk, Hq, Hk, D))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if node:
         return CrossAttnFn.apply(q, k, v, strides, kv_len, key_mask, meta, device)
     return _xattn_fwd(device, q, k, v, strides, kv_len, key_mask, meta, False)[0]
 
@@ -2030,6 +2043,7 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
     per sample [B, D] (fp32 or bf16).  branch_scale [B] fp32, not differentiated: stochastic depth; a sample at 0 is
     y = res_scale * x, whatever u holds.  post, pre: "layer" (LayerNorm), "rms" or None, with optional fp32 weight and
     (LayerNorm or RMS) bias [D].  D up to 8192."""
+    node = _through_node("norm_gate_residual", x, u, gate, post_weight, post_bias, pre_weight, pre_bias)
     if x.dim() != 3 or x.shape != u.shape:
         raise ValueError(f"x and u must be [batch, tokens, dim] alike, got {tuple(x.shape)} and {tuple(u.shape)}")
     B, N, D = x.shape
@@ -2063,7 +2077,7 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
     if not meta[3] >= 0.0:
         raise ValueError(f"eps {eps} must not be negative")
     device = _one_device(x, u, gate, branch_scale, *vectors)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, u, gate, *vectors)):
+    if node:
         res = NormGateResidualFn.apply(x, u, gate, branch_scale, *vectors, meta, device)
         return res if pre is not None else (res, None)
     return _ngr_fwd(device, x, u, (gate, branch_scale, *vectors), meta, False)[:2]
