@@ -410,3 +410,19 @@ def test_tracing_is_refused():
                      (lambda t: ops.cross_attn(t, t, t), a), (lambda t: ops.norm_gate_residual(t, t)[0], u)):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 torch.jit.trace(f, (t,), check_trace=False)
+
+
+def test_arguments_without_a_gradient_do_not_drop_one():
+    """Positions and plain numbers are not differentiated: such an argument that wants a gradient is refused while one would be
+    recorded."""
+    x, u = torch.zeros(2, 3, 4, 16), torch.zeros(2, 3, 8)
+    pos, one = torch.zeros(3, 2, requires_grad=True), torch.ones((), requires_grad=True)
+    calls = (lambda: ops.rope_axes(x, None, pos, (4, 4)), lambda: ops.rope_axes(x, x.clone(), pos, (4, 4), inplace=True),
+             lambda: ops.rope_axes(x, None, pos.detach(), (4, 4), base=one * 100.0),
+             lambda: ops.rope_axes(x, None, pos.detach(), (4, 4), base=(one * 100.0, 10.0)), lambda: ops.cross_attn(x, x, x, scale=one),
+             lambda: ops.norm_gate_residual(u, u, res_scale=one), lambda: ops.norm_gate_residual(u, u, post="rms", eps=one))
+    for f in calls:
+        with pytest.raises(ValueError, match="not differentiated"):
+            f()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm device tensors"):      # nothing to lose: the next check speaks
+            f()

@@ -1697,6 +1697,13 @@ def _through_node(name, *ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def _number(name, v):
+    """v as a Python number; one that wants a gradient would lose it here."""
+    if isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} is not differentiated")
+    return float(v)
+
+
 def _dense(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
@@ -1789,7 +1796,7 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
     """Rotary positions with several axes (time, height, width) on queries [B, N, Hq, D] and, unless None, keys
     [B, N, Hk, D] of the same tokens, in one launch; differentiable.  Returns the rotated (q, k), or q alone.
 
-    pos [N, A] or [B, N, A] (int32, int64 or float32) holds a token's position on each axis; position 0 on every axis
+    pos [N, A] or [B, N, A] (int32, int64 or float32, not differentiated) holds a token's position on each axis; position 0 on every axis
     leaves a token as it is (class token).  sections: how many of the head's pairs turn with each axis; pair j of an axis
     with s pairs turns by pos * base^(-j / s) (base a number or one per axis), or, with shared_ladder, pair p of all P by
     pos * base^(-p / P).  A pair is dims (p, P + p), or (2p, 2p + 1) with interleaved; dims from 2P on pass through.
@@ -1812,9 +1819,13 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
         bk, nk, _, d_k = xs[1].shape
         if bk != B or nk != N or d_k != D or k.dtype != q.dtype:
             raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in everything but heads")
+    for b in base if isinstance(base, (tuple, list)) else (base,):
+        _number("base", b)
     sections, ladder, pairs = _rope_ladder(tuple(sections), tuple(base) if isinstance(base, list) else base, shared_ladder)
     if 2 * pairs > D:
         raise ValueError(f"sections {sections} turn {2 * pairs} dims, the head has {D}")
+    if pos.requires_grad and torch.is_grad_enabled():
+        raise ValueError("positions are not differentiated")
     if pos.dtype not in _POS_TYPES:
         raise TypeError(f"positions are int32, int64 or float32, not {pos.dtype}")
     ps = pos.shape
@@ -1936,7 +1947,7 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
             raise ValueError(f"key_mask must be bool [{B}, {Nk}], got {key_mask.dtype} {tuple(key_mask.shape)}")
         if Nk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    scale = float(D) ** -0.5 if scale is None else float(scale)
+    scale = float(D) ** -0.5 if scale is None else _number("scale", scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale {scale} must be positive and finite")
     device = _one_device(q, k, v, kv_len, key_mask)
@@ -2073,7 +2084,7 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
     if D > 1:
         x = x if x.stride(2) == 1 else x.contiguous()
         u = u if u.stride(2) == 1 else u.contiguous()
-    meta = (float(res_scale), _NORM_KINDS[post], _NORM_KINDS[pre], float(eps))
+    meta = (_number("res_scale", res_scale), _NORM_KINDS[post], _NORM_KINDS[pre], _number("eps", eps))
     if not meta[3] >= 0.0:
         raise ValueError(f"eps {eps} must not be negative")
     device = _one_device(x, u, gate, branch_scale, *vectors)
