@@ -426,3 +426,20 @@ def test_arguments_without_a_gradient_do_not_drop_one():
             f()
         with torch.no_grad(), pytest.raises(RuntimeError, match="ROCm device tensors"):      # nothing to lose: the next check speaks
             f()
+
+
+def test_rotary_arguments_are_kept_by_value(monkeypatch):
+    """A base or a section count that lies in a tensor and changes between two calls must not meet the first call's ladder."""
+    seen = []
+    monkeypatch.setattr(ops, "_one_device", lambda *t: 0)
+    monkeypatch.setattr(ops, "_rope_launch", lambda device, xs, outs, pos, ladder, *rest: seen.append(ladder))
+    x, pos = torch.zeros(2, 3, 4, 16), torch.zeros(3, 2)
+    n, base = torch.tensor(4), torch.tensor(100.0)
+    for _ in range(2):
+        ops.rope_axes(x, None, pos, (n, 2), base)
+        ops.rope_axes(x, None, pos, (n, 2), [base, 10.0])
+        ops.rope_axes(x, None, pos, [int(n), 2], float(base))
+        ops.rope_axes(x, None, pos, (int(n), 2), (float(base), 10.0))
+        n += 1
+        base *= 10
+    assert seen[0] == seen[2] and seen[1] == seen[3] and seen[4] == seen[6] and seen[5] == seen[7] and seen[0] != seen[4]

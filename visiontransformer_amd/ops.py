@@ -1721,8 +1721,8 @@ _NO_TENSOR = (0,) * 10
 
 @functools.lru_cache(maxsize=256)
 def _rope_ladder(sections, base, shared):
-    """(sections, log2 of the bases, pairs) of checked arguments, as the argument struct takes them."""
-    sections = tuple(int(s) for s in sections)
+    """(sections, log2 of the bases, pairs) of checked arguments, as the argument struct takes them; plain numbers alone, the
+    cache would know tensors by their identity."""
     if not 1 <= len(sections) <= 4 or min(sections) < 1 or sum(sections) > 256:
         raise ValueError(f"sections {sections}: one to four axes of at least one pair each, at most 256 pairs")
     bases = base if isinstance(base, tuple) else (base,) * len(sections)
@@ -1819,9 +1819,8 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
         bk, nk, _, d_k = xs[1].shape
         if bk != B or nk != N or d_k != D or k.dtype != q.dtype:
             raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must agree in everything but heads")
-    for b in base if isinstance(base, (tuple, list)) else (base,):
-        _number("base", b)
-    sections, ladder, pairs = _rope_ladder(tuple(sections), tuple(base) if isinstance(base, list) else base, shared_ladder)
+    base = tuple(_number("base", b) for b in base) if isinstance(base, (tuple, list)) else _number("base", base)
+    sections, ladder, pairs = _rope_ladder(tuple(map(int, sections)), base, shared_ladder)
     if 2 * pairs > D:
         raise ValueError(f"sections {sections} turn {2 * pairs} dims, the head has {D}")
     if pos.requires_grad and torch.is_grad_enabled():
