@@ -809,3 +809,38 @@ def test_forward_mode_and_functional_transforms_are_refused(record):
             with pytest.raises(RuntimeError, match="outside of autograd"):
                 ops().rope_axes(forward_ad.make_dual(buf, x), None, pos, (8,), inplace=True)
         assert torch.equal(buf, x)
+
+
+def all_three_kept(g, B=2, N=40):
+    """A loss through the three operators with every kind of tensor that they keep, and its leaves."""
+    r = lambda *s, dt=F: torch.randn(*s, generator=g).to(DEV, dt).requires_grad_()
+    leaves = dict(qkv=r(B, N, 3, 4, 16, dt=H), x=r(B, N, 64), u=r(B, N, 64), gate=r(B, 64), w=r(64), b=r(64), pw=r(64), far=r(B, 300, 2, 4, 16))
+    pos = torch.randint(0, 50, (B, N, 2), generator=g).to(DEV)
+    lens, keep = torch.tensor([17, 290], device=DEV)[:B], (torch.rand(B, N, generator=g) < 0.6).to(DEV)
+    scale = torch.tensor([1.25, 0.0], device=DEV)[:B]
+
+    def loss():
+        q, k, v = leaves["qkv"].unbind(2)
+        q, k = ops().rope_axes(q, k, pos, (4, 4))
+        o = ops().cross_attn(q, k, v, key_mask=keep)
+        y, h = ops().norm_gate_residual(leaves["x"], leaves["u"], leaves["gate"], scale, post="layer", post_weight=leaves["w"],
+                                        post_bias=leaves["b"], pre="rms", pre_weight=leaves["pw"])
+        far = ops().cross_attn(h.unflatten(-1, (4, 16)), *leaves["far"].unbind(2), kv_len=lens)
+        return (o.float() ** 2).sum() + (far ** 2).sum() + (y * h).sum()
+    return loss, list(leaves.values())
+
+
+def laid_out_anew(t):
+    """The same values with no unit stride anywhere."""
+    return torch.stack((t.detach().movedim(-1, 0).contiguous(),) * 2, -1)[..., 0].movedim(0, -1)
+
+
+def test_saved_tensors_that_come_back_strided():
+    loss, leaves = all_three_kept(gen(41))
+    want = torch.autograd.grad(loss(), leaves)
+    kinds = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: (kinds.append(t.dim()), laid_out_anew(t))[1]):
+        got = torch.autograd.grad(loss(), leaves)
+    assert {1, 2, 3, 4} <= set(kinds)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

@@ -1860,6 +1860,15 @@ def _xattn_operands(q, k, v):
     return q, k, v, (sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2])
 
 
+def _xattn_masks(kv_len, key_mask):
+    """The lengths dense and the mask with unit stride over the keys."""
+    if kv_len is not None:
+        kv_len = kv_len.contiguous()
+    if key_mask is not None and key_mask.shape[1] > 1 and key_mask.stride(1) != 1:
+        key_mask = key_mask.contiguous()
+    return kv_len, key_mask
+
+
 def _xattn_pack(q, k, v, o, strides, kv_len, key_mask, lse, meta, do=None, dq=None, dk=None, dv=None):
     scale, dims = meta
     sd = (0, 0, 0) if do is None else do.stride()
@@ -1898,6 +1907,8 @@ class CrossAttnFn(torch.autograd.Function):
             return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None,) * 5
         meta, device = ctx.meta
         q, k, v, strides = _xattn_operands(q, k, v)       # of the saved ones: a hook may have laid them out anew
+        o, lse = o.contiguous(), lse.contiguous()
+        kv_len, key_mask = _xattn_masks(kv_len, key_mask)
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq = _dense(q) if need_q else None
         dk, dv = (_dense(k), _dense(v)) if need_k or need_v else (None, None)
@@ -1940,12 +1951,10 @@ def cross_attn(q, k, v, kv_len=None, key_mask=None, scale=None):
             raise ValueError("give key lengths or a key mask, not both")
         if kv_len.dtype not in (torch.int32, torch.int64) or tuple(kv_len.shape) != (B,):
             raise ValueError(f"kv_len must be int32 or int64 [{B}], got {kv_len.dtype} {tuple(kv_len.shape)}")
-        kv_len = kv_len.contiguous()
     if key_mask is not None:
         if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, Nk):
             raise ValueError(f"key_mask must be bool [{B}, {Nk}], got {key_mask.dtype} {tuple(key_mask.shape)}")
-        if Nk > 1 and key_mask.stride(1) != 1:
-            key_mask = key_mask.contiguous()
+    kv_len, key_mask = _xattn_masks(kv_len, key_mask)
     scale = float(D) ** -0.5 if scale is None else _number("scale", scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"scale {scale} must be positive and finite")
@@ -1966,7 +1975,20 @@ def _ngr_vector(name, kind, t, D):
         raise ValueError(f"{name} without {name.split('_')[0]}")
     if t.shape != (D,) or t.dtype != torch.float32:
         raise ValueError(f"{name} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
-    return t if t.stride(0) == 1 else t.contiguous()
+    return t
+
+
+def _ngr_layout(x, u, gate, branch_scale, *vectors):
+    """Unit stride over the columns, a gate per sample by rows of its own."""
+    D = x.shape[2]
+    if D > 1:
+        x = x if x.stride(2) == 1 else x.contiguous()
+        u = u if u.stride(2) == 1 else u.contiguous()
+    if gate is not None and (gate.stride(-1) != 1 or (gate.dim() == 2 and gate.stride(0) < D)):
+        gate = gate.contiguous()
+    if branch_scale is not None:
+        branch_scale = branch_scale.contiguous()
+    return x, u, (gate, branch_scale, *(t if t is None or t.stride(0) == 1 else t.contiguous() for t in vectors))
 
 
 _NGR_NO_GRADS = (0,) * 9
@@ -2023,6 +2045,8 @@ class NormGateResidualFn(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 10
         meta, device = ctx.meta
+        x, u, params = _ngr_layout(x, u, *params)
+        stats = stats.contiguous()
         # dx, du, dgate and the norms' parameters; branch_scale has none
         grads = [_dense(t) if need[i] else None for i, t in ((0, x), (1, u), (2, params[0]), (4, params[2]), (5, params[3]),
                                                              (6, params[4]), (7, params[5]))]
@@ -2072,22 +2096,17 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
             _dt(gate)
         if gate.shape != (D,) and gate.shape != (B, D):
             raise ValueError(f"gate {tuple(gate.shape)} must be [{D}] or [{B}, {D}]")
-        if gate.stride(-1) != 1 or (gate.dim() == 2 and gate.stride(0) < D):
-            gate = gate.contiguous()
     if branch_scale is not None:
         if branch_scale.dtype != torch.float32 or tuple(branch_scale.shape) != (B,):
             raise ValueError(f"branch_scale must be float32 [{B}], got {branch_scale.dtype} {tuple(branch_scale.shape)}")
         if branch_scale.requires_grad:
             raise ValueError("branch_scale is not differentiated")
-        branch_scale = branch_scale.contiguous()
-    if D > 1:
-        x = x if x.stride(2) == 1 else x.contiguous()
-        u = u if u.stride(2) == 1 else u.contiguous()
+    x, u, params = _ngr_layout(x, u, gate, branch_scale, *vectors)
     meta = (_number("res_scale", res_scale), _NORM_KINDS[post], _NORM_KINDS[pre], _number("eps", eps))
     if not meta[3] >= 0.0:
         raise ValueError(f"eps {eps} must not be negative")
-    device = _one_device(x, u, gate, branch_scale, *vectors)
+    device = _one_device(x, u, *params)
     if node:
-        res = NormGateResidualFn.apply(x, u, gate, branch_scale, *vectors, meta, device)
+        res = NormGateResidualFn.apply(x, u, *params, meta, device)
         return res if pre is not None else (res, None)
-    return _ngr_fwd(device, x, u, (gate, branch_scale, *vectors), meta, False)[:2]
+    return _ngr_fwd(device, x, u, params, meta, False)[:2]
