@@ -844,3 +844,16 @@ def test_saved_tensors_that_come_back_strided():
     assert {1, 2, 3, 4} <= set(kinds)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("change", [lambda t: t.cpu(), lambda t: t[:1], lambda t: t.to(torch.float64)], ids=["host", "shape", "type"])
+def test_saved_tensors_that_come_back_as_something_else_are_refused(change):
+    g = gen(42)
+    x, u = torch.randn(2, 9, 2, 16, generator=g).to(DEV).requires_grad_(), torch.randn(2, 9, 32, generator=g).to(DEV).requires_grad_()
+    pos = torch.arange(9, device=DEV)[:, None]
+    for f, t in ((lambda: ops().rope_axes(x, None, pos, (8,)), x), (lambda: ops().cross_attn(x, x, x), x),
+                 (lambda: ops().norm_gate_residual(u, u, post="rms")[0], u)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda s: s.detach(), change):
+            y = f()
+            with pytest.raises(RuntimeError, match="came back"):
+                torch.autograd.grad(y.sum(), t)

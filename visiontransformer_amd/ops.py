@@ -1715,6 +1715,14 @@ def _heads4(name, t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 or t.numel() == 0 else t.contiguous()
 
 
+def _came_back(device, *saved):
+    """Saved tensors may come back from a hook in another layout, but with the (shape, type) and on the device that the launch
+    is made for."""
+    for t, shape, dtype in saved:
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != device):
+            raise RuntimeError(f"a saved tensor of shape {tuple(shape)} and type {dtype} came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _NO_TENSOR = (0,) * 10
 
@@ -1762,7 +1770,7 @@ class RopeAxesFn(torch.autograd.Function):
         outs = (_dense(q),) if k is None else (_dense(q), _dense(k))
         _rope_launch(device, xs, outs, pos, ladder, interleaved, shared, False)
         ctx.save_for_backward(pos)
-        ctx.meta = (device, ladder, interleaved, shared)
+        ctx.meta = (device, ladder, interleaved, shared, pos.dtype)
         ctx.set_materialize_grads(False)
         return outs if k is not None else outs[0]
 
@@ -1772,12 +1780,14 @@ class RopeAxesFn(torch.autograd.Function):
         if _PS2 is not None:                # a replay forms no input gradients
             return tuple(None if g is None else _no_grad_like(g.shape, g.dtype, g.device) for g in (dq, dk)) + (None,) * 5
         pos, = ctx.saved_tensors
-        device, ladder, interleaved, shared = ctx.meta
+        device, ladder, interleaved, shared, pos_type = ctx.meta
         gs = [None if g is None or not need else _heads4("gradient", g)
               for g, need in zip((dq, dk), ctx.needs_input_grad)]
         outs = [None if g is None else _dense(g) for g in gs]
         live = [i for i in (0, 1) if gs[i] is not None]
         if live:
+            B, N = gs[live[0]].shape[:2]
+            _came_back(device, (pos, (B, N, ladder[-1]) if pos.dim() == 3 else (N, ladder[-1]), pos_type))
             _rope_launch(device, [gs[i] for i in live], [outs[i] for i in live], pos, ladder, interleaved, shared, True)
         return outs[0], outs[1], None, None, None, None, None
 
@@ -1897,6 +1907,7 @@ class CrossAttnFn(torch.autograd.Function):
         o, lse = _xattn_fwd(device, q, k, v, strides, kv_len, key_mask, meta, True)
         ctx.save_for_backward(q, k, v, o, lse, kv_len, key_mask)
         ctx.meta = (meta, device)
+        ctx.len_type = None if kv_len is None else kv_len.dtype
         return o
 
     @staticmethod
@@ -1906,7 +1917,11 @@ class CrossAttnFn(torch.autograd.Function):
         if _PS2 is not None:                # a replay forms no input gradients
             return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None,) * 5
         meta, device = ctx.meta
-        q, k, v, strides = _xattn_operands(q, k, v)       # of the saved ones: a hook may have laid them out anew
+        _, B, Nq, Nk, Hq, Hk, D = meta[1]
+        dtype = do.dtype
+        _came_back(device, (q, (B, Nq, Hq, D), dtype), (k, (B, Nk, Hk, D), dtype), (v, (B, Nk, Hk, D), dtype), (o, (B, Nq, Hq, D), dtype),
+                   (lse, (B, Hq * Nq), torch.float32), (kv_len, (B,), ctx.len_type), (key_mask, (B, Nk), torch.bool))
+        q, k, v, strides = _xattn_operands(q, k, v)
         o, lse = o.contiguous(), lse.contiguous()
         kv_len, key_mask = _xattn_masks(kv_len, key_mask)
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
@@ -2028,8 +2043,9 @@ class NormGateResidualFn(torch.autograd.Function):
     def forward(ctx, x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, device):
         params = (gate, branch_scale, post_w, post_b, pre_w, pre_b)
         y, h, stats = _ngr_fwd(device, x, u, params, meta, True)
-        ctx.save_for_backward(x, u, *params, stats)
-        ctx.meta = (meta, device)
+        kept = (x, u, *params, stats)
+        ctx.save_for_backward(*kept)
+        ctx.meta = (meta, device, [None if t is None else (t.shape, t.dtype) for t in kept])
         ctx.set_materialize_grads(False)
         return (y, h) if h is not None else y
 
@@ -2044,7 +2060,8 @@ class NormGateResidualFn(torch.autograd.Function):
             return (_no_grad_like(x.shape, x.dtype, x.device), _no_grad_like(u.shape, u.dtype, u.device)) + (None,) * 8
         if dy is None and dh is None:
             return (None,) * 10
-        meta, device = ctx.meta
+        meta, device, kept = ctx.meta
+        _came_back(device, *((t, *like) for t, like in zip((x, u, *params, stats), kept) if t is not None))
         x, u, params = _ngr_layout(x, u, *params)
         stats = stats.contiguous()
         # dx, du, dgate and the norms' parameters; branch_scale has none
