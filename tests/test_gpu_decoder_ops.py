@@ -857,3 +857,20 @@ def test_saved_tensors_that_come_back_as_something_else_are_refused(change):
             y = f()
             with pytest.raises(RuntimeError, match="came back"):
                 torch.autograd.grad(y.sum(), t)
+
+
+def test_cross_attn_without_a_query_gradient_forms_no_parts_of_it(monkeypatch):
+    """Frozen queries: the launch that splits dq over the keys has only delta to form, and the scratch memory of the parts, which
+    the size query makes room for, stays as it was."""
+    g = gen(51)
+    q, k, v, do = (torch.randn(1, n, 1, 64, generator=g).to(DEV, H) for n in (512, 8192, 8192, 512))
+    made = []
+    monkeypatch.setattr(ops(), "_ws", lambda n, device: made.append(torch.full((max(int(n), 16),), 255, dtype=torch.uint8, device=device)) or made[-1])
+    got = []
+    for need in (True, False):
+        args = [q.clone().requires_grad_(need), k.clone().requires_grad_(), v.clone().requires_grad_()]
+        o = ops().cross_attn(*args)
+        got.append(torch.autograd.grad(o, [t for t in args if t.requires_grad], do))
+    for a, b in zip(got[0][1:], got[1]):
+        assert torch.equal(a, b)
+    assert (made[-1][-(1 << 20):] == 255).all()

@@ -1733,13 +1733,13 @@ extern "C" int vitmi_cross_attn_bwd(const vitmi_xattn_args* g, void* workspace, 
     char* w = (char*)workspace;
     a.delta = (float*)w;
     w += up256(rows * 4);
-    if (p.dq_splits > 1) {
+    a.tiles = p.dq_tiles;
+    a.splits = g->dq ? p.dq_splits : 1;                   // without dq the launch forms delta alone
+    if (a.splits > 1) {
         a.part_dq = (float*)w;
-        w += up256(p.dq_splits * a.n_q * 4);
+        w += up256(a.splits * a.n_q * 4);
     }
     a.part_kv = (float*)w;
-    a.tiles = p.dq_tiles;
-    a.splits = p.dq_splits;
     if (int rc = xa_run(XK_DQ, g->dt, a, vec, (long long)g->B * g->Hk * a.tiles * a.splits, s)) return rc;
     if (g->dq && a.splits > 1)
         if (int rc = xa_sum(g->dt, a.part_dq, g->dq, g->scale, a.n_q, a.splits, s)) return rc;
