@@ -66,7 +66,7 @@ struct XaArgs {
     float *part_dq;
     float* part_kv;                       // [workgroups][first, last share][dk, dv][128][D]
     int B;
-    long long n_q, n_k;                   // elements of q and of k
+    long long n_q;                        // elements of q
 };
 
 template <typename T> struct Mx;
@@ -1546,7 +1546,6 @@ void xa_fill(const vitmi_xattn_args* g, XaArgs* a) {
     a->dq = g->dq; a->dk = g->dk; a->dv = g->dv;
     a->n_q = (long long)g->B * g->Nq * g->Hq * g->D;
     a->B = g->B;
-    a->n_k = (long long)g->B * g->Nk * g->Hk * g->D;
 }
 
 // more than 64 KB of LDS a workgroup is asked for once per kernel and device (a bit of *done each)
