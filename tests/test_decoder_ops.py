@@ -443,3 +443,43 @@ def test_rotary_arguments_are_kept_by_value(monkeypatch):
         n += 1
         base *= 10
     assert seen[0] == seen[2] and seen[1] == seen[3] and seen[4] == seen[6] and seen[5] == seen[7] and seen[0] != seen[4]
+
+
+def test_in_place_rotation_of_interleaved_views_that_share_elements_is_refused():
+    """Slots of a packed projection are apart though their ranges meet; slots that share a head, a dim or a row are not, nor is a
+    window view of its own memory."""
+    pos = torch.zeros(5, 1)
+    buf = torch.zeros(2, 5, 6, 16)
+    for a, b in (((0, 3), (2, 6)), ((1, 5), (0, 2)), ((0, 6), (3, 4))):
+        with pytest.raises(ValueError, match="apart"):
+            ops.rope_axes(buf[:, :, slice(*a)], buf[:, :, slice(*b)], pos, (2,), inplace=True)
+    with pytest.raises(ValueError, match="apart"):
+        ops.rope_axes(buf[..., :9], buf[..., 7:], pos, (2,), inplace=True)
+    rows = torch.zeros(2, 6, 3, 16)
+    with pytest.raises(ValueError, match="apart"):
+        ops.rope_axes(rows[:, :5], rows[:, 1:], pos, (2,), inplace=True)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.rope_axes(torch.zeros(20).as_strided((1, 5, 1, 8), (20, 2, 8, 1)), None, pos, (2,), inplace=True)
+    for a, b in ((buf[:, :, :4], buf[:, :, 4:]), (buf[..., :8], buf[..., 8:]), (buf[:1], buf[1:]), (buf.transpose(0, 1)[:2].transpose(0, 1), buf[:, 3:]),
+                 (buf[:, :, ::2], buf[:, :, 1::2])):
+        with pytest.raises(RuntimeError, match="ROCm device tensors"):           # apart: the next check speaks
+            ops.rope_axes(a, b, torch.zeros(a.shape[1], 1), (2,), inplace=True)
+
+
+def test_whether_strided_tensors_meet_against_counting():
+    rng = torch.Generator().manual_seed(2)
+    pick = lambda lo, hi: int(torch.randint(lo, hi + 1, (), generator=rng))
+    met = 0
+    for _ in range(3000):
+        size = (2, 4)[pick(0, 1)]
+        shapes = [tuple(pick(1, 4) for _ in range(3)) for _ in range(2)]
+        strides = [tuple(pick(0, 30) if pick(0, 2) else pick(1, 4) for _ in range(3)) for _ in range(2)]
+        apart = pick(-80, 80)
+        places = [[sum(i * s for i, s in zip(ix, st)) * size for ix in torch.cartesian_prod(*(torch.arange(n) for n in sh)).tolist()]
+                  for sh, st in zip(shapes, strides)]
+        want = any(abs(a - b - apart) < size for a in places[0] for b in places[1])
+        assert ops._meet(apart, size, shapes[0], strides[0], shapes[1], strides[1]) == want
+        met += want
+        if 0 not in strides[0]:
+            assert ops._meets_itself(size, shapes[0], strides[0]) == (len(set(places[0])) < len(places[0]))
+    assert 300 < met < 2700

@@ -1792,14 +1792,53 @@ class RopeAxesFn(torch.autograd.Function):
         return outs[0], outs[1], None, None, None, None, None
 
 
+def _reaches(offset, dims, moved=False, budget=None):
+    """Whether whole numbers i_d, lo_d <= i_d <= hi_d, make sum(i_d * stride_d) == offset, for dims of (stride, lo, hi) in order
+    of falling strides; with moved, other than by zeros in all but the last.  A search that layouts of nested strides
+    keep to a few steps; where it takes thousands the answer is yes."""
+    budget = [10000] if budget is None else budget
+    budget[0] -= 1
+    if budget[0] < 0:
+        return True
+    (s, lo, hi), rest = dims[0], dims[1:]
+    if not rest:
+        return not moved and offset % s == 0 and lo <= offset // s <= hi
+    low, high = sum(t * n for t, n, _ in rest), sum(t * n for t, _, n in rest)
+    return any(_reaches(offset - i * s, rest, moved and not i, budget)
+               for i in range(max(lo, -((high - offset) // s)), min(hi, (offset - low) // s) + 1))
+
+
+def _steps(size, *layouts):
+    """The dims of _reaches, in bytes, of (shape, strides, sign) layouts of elements of `size` bytes: steps forwards (1),
+    backwards (-1) or both ways (0).  Two elements meet where their first bytes are less than `size` apart."""
+    dims = {}
+    for shape, strides, sign in layouts:
+        for n, s in zip(shape, strides):
+            if n > 1 and s > 0:
+                lo, hi = dims.get(s * size, (0, 0))
+                dims[s * size] = (lo - (sign <= 0) * (n - 1), hi + (sign >= 0) * (n - 1))
+    return [(s, *r) for s, r in sorted(dims.items(), reverse=True)] + [(1, 1 - size, size - 1)]
+
+
+@functools.lru_cache(maxsize=256)
+def _meet(apart, size, q_shape, q_strides, k_shape, k_strides):
+    return _reaches(apart, _steps(size, (q_shape, q_strides, 1), (k_shape, k_strides, -1)))
+
+
+@functools.lru_cache(maxsize=256)
+def _meets_itself(size, shape, strides):
+    used = [s for n, s in zip(shape, strides) if n > 1]
+    return len(set(used)) < len(used) or _reaches(0, _steps(size, (shape, strides, 0)), moved=True)
+
+
 def _overlap(q, k):
-    """Whether two tensors are known to share memory: one start, or both dense with ranges that meet."""
+    """Whether two tensors of one type share memory."""
     if not q.numel() or not k.numel():
         return False
-    p, r = q.data_ptr(), k.data_ptr()
+    apart = k.data_ptr() - q.data_ptr()
     if q.is_contiguous() and k.is_contiguous():
-        return p < r + k.numel() * k.element_size() and r < p + q.numel() * q.element_size()
-    return p == r
+        return -k.numel() * k.element_size() < apart < q.numel() * q.element_size()
+    return _meet(apart, q.element_size(), q.shape, q.stride(), k.shape, k.stride())
 
 
 def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladder=False, inplace=False):
@@ -1820,6 +1859,8 @@ def rope_axes(q, k, pos, sections, base=10000.0, interleaved=False, shared_ladde
                 raise ValueError("inplace needs [batch, tokens, heads, head dim] with unit stride over the head dim")
             if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise ValueError("inplace on a broadcast tensor would turn the same memory several times")
+            if t.numel() and not t.is_contiguous() and _meets_itself(t.element_size(), t.shape, t.stride()):
+                raise ValueError("inplace on a tensor whose elements overlap would turn the same memory several times")
     else:
         xs = (_heads4("q", q),) if k is None else (_heads4("q", q), _heads4("k", k))
     x = xs[0]
