@@ -874,3 +874,18 @@ def test_cross_attn_without_a_query_gradient_forms_no_parts_of_it(monkeypatch):
     for a, b in zip(got[0][1:], got[1]):
         assert torch.equal(a, b)
     assert (made[-1][-(1 << 20):] == 255).all()
+
+
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hk,D,mask", [(30, 130, 70, 4, 2, 40, "keys"), (16, 128, 33, 8, 8, 64, "len"), (13, 129, 65, 8, 8, 64, "none"),
+                                                 (16, 128, 40, 4, 4, 96, "keys"), (13, 130, 40, 4, 4, 128, "len"), (1, 70, 480, 2, 2, 32, "len"),
+                                                 (1, 70, 481, 2, 2, 32, "len"), (1, 70, 384, 1, 1, 96, "keys"), (1, 70, 385, 1, 1, 96, "keys")])
+def test_cross_attn_fp32_on_both_sides_of_the_small_launches(B, Nq, Nk, Hq, Hk, D, mask):
+    """fp32 launches of few tiles take the form of few rows: numbers of tiles and of keys at the ends of that rule."""
+    q, kv, do, lens, keep = xattn_inputs((B, Nq, Nk, Hq, Hk, D, mask), F, seed=13)
+    ref, tol = attention_bounds(q.double(), kv[:, :, 0].double(), kv[:, :, 1].double(), orc.allowed_keys(B, Nk, lens, keep), do.double(), F,
+                                half_step(q))
+    m = dict(kv_len=None if lens is None else lens.to(DEV), key_mask=None if keep is None else keep.to(DEV))
+    args = [t.to(DEV).requires_grad_() for t in (q, kv[:, :, 0], kv[:, :, 1])]
+    o = ops().cross_attn(*args, **m)
+    for n, t in zip(("o", "dq", "dk", "dv"), (o,) + torch.autograd.grad(o, args, do.to(DEV))):
+        within(n, t, ref[n], tol[n])

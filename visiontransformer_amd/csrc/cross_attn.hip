@@ -1493,10 +1493,12 @@ XaPlan xa_plan(int dt, int B, int Nq, int Nk, int Hq, int Hk, int D, bool vec) {
     XaPlan p;
     const int R = Hq / Hk * Nq, KT = dt == VITMI_F32 ? 32 : 64;
     const long long bh = (long long)B * Hk;
-    // also fp32 launches that would leave most matrix pipes without a wave: up to 384 tiles of 32 rows, up to 512 keys (197 rows and
-    // keys of 64, 48 heads, 336 tiles: 17.7 us, by tiles of 128 rows 23.8; 96 heads, 672 tiles: 26.2 and 24.2; 1000 keys: equal,
-    // 4000: 49 and 32)
-    p.few = R <= 64 || (dt == VITMI_F32 && bh * cdiv(R, 32) <= 384 && Nk <= 512);
+    // also fp32 launches that would leave most matrix pipes without a wave, while all their tiles of 32 rows are at work at once: two
+    // workgroups of this form fit a compute unit at heads up to 64, one at wider ones (LDS).  By tiles of 32 rows / of 128, us:
+    // heads of 64, 257 keys, 128 tiles 15 / 18, 384 21 / 29, 512 21 / 29, 520 33 / 29; 100 keys, 512 tiles 12 / 16; 480 keys, 260 tiles
+    // 28 / 27, 512 30 / 37; 512 keys (two splits) 384 tiles 36 / 35.  Heads of 128, 257 keys, 256 tiles 26 / 30, 260 48 / 31; 384
+    // keys, 64 tiles 25 / 21, 256 27 / 30; 480 keys, 64 tiles 30 / 25.
+    p.few = R <= 64 || (dt == VITMI_F32 && (D <= 64 ? bh * cdiv(R, 32) <= 512 && Nk <= 480 : bh * cdiv(R, 32) <= 256 && Nk <= 384));
     p.fwd_tiles = cdiv(R, p.few ? 32 : 128);
     const long long rows = bh * R;
     p.fwd_splits = p.few ? xa_few_splits(bh * p.fwd_tiles, cdiv(Nk, 32)) : xa_splits(dt, bh * p.fwd_tiles, cdiv(Nk, KT), rows, D);
