@@ -1686,19 +1686,29 @@ def _one_device(first, *rest):
     return d
 
 
+_tracing_state, _transforms_active = torch._C._get_tracing_state, torch._C._are_functorch_transforms_active
+_saved_hooks = torch._C._autograd._top_saved_tensors_default_hooks
+
+
 def _through_node(name, *ts):
     """Whether a call goes through its autograd node: where a gradient is wanted, and where forward-mode or functional
     transforms are at work, whose tangents or batches a launch would drop and the node refuses.  A traced program would lose
     the launch, or keep the node with the sizes of the call it saw and without the checks of later ones."""
-    if torch._C._get_tracing_state() is not None:
+    if _tracing_state() is not None:
         raise RuntimeError(f"{name} cannot be traced")
-    if forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active():
+    if forward_ad._current_level >= 0 or _transforms_active():
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _number(name, v):
     """v as a Python number; one that wants a gradient would lose it here."""
+    if type(v) is float:
+        return v
     if isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} is not differentiated")
     return float(v)
@@ -1715,12 +1725,22 @@ def _heads4(name, t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 or t.numel() == 0 else t.contiguous()
 
 
-def _came_back(device, *saved):
-    """Saved tensors may come back from a hook in another layout, but with the (shape, type) and on the device that the launch
-    is made for."""
-    for t, shape, dtype in saved:
-        if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != device):
-            raise RuntimeError(f"a saved tensor of shape {tuple(shape)} and type {dtype} came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+def _save(ctx, *tensors):
+    """save_for_backward; where hooks take the tensors, also what they have to hand back."""
+    ctx.save_for_backward(*tensors)
+    ctx.like = None
+    if _saved_hooks(False) is not None:
+        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _saved(ctx):
+    """The saved tensors: hooks may lay them out anew, but shape, type and device are those that the launch is made for."""
+    tensors = ctx.saved_tensors
+    if ctx.like is not None:
+        for t, like in zip(tensors, ctx.like):
+            if like is not None and (t.shape, t.dtype, t.device) != like:
+                raise RuntimeError(f"a saved tensor {tuple(like[0])} {like[1]} on {like[2]} came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+    return tensors
 
 
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -1769,8 +1789,8 @@ class RopeAxesFn(torch.autograd.Function):
         xs = (q,) if k is None else (q, k)
         outs = (_dense(q),) if k is None else (_dense(q), _dense(k))
         _rope_launch(device, xs, outs, pos, ladder, interleaved, shared, False)
-        ctx.save_for_backward(pos)
-        ctx.meta = (device, ladder, interleaved, shared, pos.dtype)
+        _save(ctx, pos)
+        ctx.meta = (device, ladder, interleaved, shared)
         ctx.set_materialize_grads(False)
         return outs if k is not None else outs[0]
 
@@ -1779,15 +1799,13 @@ class RopeAxesFn(torch.autograd.Function):
     def backward(ctx, dq, dk=None):
         if _PS2 is not None:                # a replay forms no input gradients
             return tuple(None if g is None else _no_grad_like(g.shape, g.dtype, g.device) for g in (dq, dk)) + (None,) * 5
-        pos, = ctx.saved_tensors
-        device, ladder, interleaved, shared, pos_type = ctx.meta
+        pos, = _saved(ctx)
+        device, ladder, interleaved, shared = ctx.meta
         gs = [None if g is None or not need else _heads4("gradient", g)
               for g, need in zip((dq, dk), ctx.needs_input_grad)]
         outs = [None if g is None else _dense(g) for g in gs]
         live = [i for i in (0, 1) if gs[i] is not None]
         if live:
-            B, N = gs[live[0]].shape[:2]
-            _came_back(device, (pos, (B, N, ladder[-1]) if pos.dim() == 3 else (N, ladder[-1]), pos_type))
             _rope_launch(device, [gs[i] for i in live], [outs[i] for i in live], pos, ladder, interleaved, shared, True)
         return outs[0], outs[1], None, None, None, None, None
 
@@ -1946,23 +1964,18 @@ class CrossAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, strides, kv_len, key_mask, meta, device):
         o, lse = _xattn_fwd(device, q, k, v, strides, kv_len, key_mask, meta, True)
-        ctx.save_for_backward(q, k, v, o, lse, kv_len, key_mask)
+        _save(ctx, q, k, v, o, lse, kv_len, key_mask)
         ctx.meta = (meta, device)
-        ctx.len_type = None if kv_len is None else kv_len.dtype
         return o
 
     @staticmethod
     @_once
     def backward(ctx, do):
-        q, k, v, o, lse, kv_len, key_mask = ctx.saved_tensors
+        q, k, v, o, lse, kv_len, key_mask = _saved(ctx)
         if _PS2 is not None:                # a replay forms no input gradients
             return tuple(_no_grad_like(t.shape, t.dtype, t.device) for t in (q, k, v)) + (None,) * 5
         meta, device = ctx.meta
-        _, B, Nq, Nk, Hq, Hk, D = meta[1]
-        dtype = do.dtype
-        _came_back(device, (q, (B, Nq, Hq, D), dtype), (k, (B, Nk, Hk, D), dtype), (v, (B, Nk, Hk, D), dtype), (o, (B, Nq, Hq, D), dtype),
-                   (lse, (B, Hq * Nq), torch.float32), (kv_len, (B,), ctx.len_type), (key_mask, (B, Nk), torch.bool))
-        q, k, v, strides = _xattn_operands(q, k, v)
+        q, k, v, strides = _xattn_operands(q, k, v)       # of the saved ones: a hook may have laid them out anew
         o, lse = o.contiguous(), lse.contiguous()
         kv_len, key_mask = _xattn_masks(kv_len, key_mask)
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
@@ -2031,10 +2044,14 @@ def _ngr_vector(name, kind, t, D):
         raise ValueError(f"{name} without {name.split('_')[0]}")
     if t.shape != (D,) or t.dtype != torch.float32:
         raise ValueError(f"{name} must be float32 [{D}], got {t.dtype} {tuple(t.shape)}")
-    return t
+    return _unit(t)
 
 
-def _ngr_layout(x, u, gate, branch_scale, *vectors):
+def _unit(t):
+    return t if t is None or t.stride(0) == 1 else t.contiguous()
+
+
+def _ngr_layout(x, u, gate, branch_scale):
     """Unit stride over the columns, a gate per sample by rows of its own."""
     D = x.shape[2]
     if D > 1:
@@ -2044,7 +2061,7 @@ def _ngr_layout(x, u, gate, branch_scale, *vectors):
         gate = gate.contiguous()
     if branch_scale is not None:
         branch_scale = branch_scale.contiguous()
-    return x, u, (gate, branch_scale, *(t if t is None or t.stride(0) == 1 else t.contiguous() for t in vectors))
+    return x, u, gate, branch_scale
 
 
 _NGR_NO_GRADS = (0,) * 9
@@ -2084,16 +2101,15 @@ class NormGateResidualFn(torch.autograd.Function):
     def forward(ctx, x, u, gate, branch_scale, post_w, post_b, pre_w, pre_b, meta, device):
         params = (gate, branch_scale, post_w, post_b, pre_w, pre_b)
         y, h, stats = _ngr_fwd(device, x, u, params, meta, True)
-        kept = (x, u, *params, stats)
-        ctx.save_for_backward(*kept)
-        ctx.meta = (meta, device, [None if t is None else (t.shape, t.dtype) for t in kept])
+        _save(ctx, x, u, *params, stats)
+        ctx.meta = (meta, device)
         ctx.set_materialize_grads(False)
         return (y, h) if h is not None else y
 
     @staticmethod
     @_once
     def backward(ctx, dy, dh=None):
-        x, u, *params, stats = ctx.saved_tensors
+        x, u, *params, stats = _saved(ctx)
         need = ctx.needs_input_grad
         if (_PS is not None or _PS2 is not None) and any(need[i] for i in (2, 4, 5, 6, 7)):
             raise NotImplementedError("per-sample norms of norm_gate_residual's gate and norm parameters")
@@ -2101,9 +2117,9 @@ class NormGateResidualFn(torch.autograd.Function):
             return (_no_grad_like(x.shape, x.dtype, x.device), _no_grad_like(u.shape, u.dtype, u.device)) + (None,) * 8
         if dy is None and dh is None:
             return (None,) * 10
-        meta, device, kept = ctx.meta
-        _came_back(device, *((t, *like) for t, like in zip((x, u, *params, stats), kept) if t is not None))
-        x, u, params = _ngr_layout(x, u, *params)
+        meta, device = ctx.meta
+        params[2:] = map(_unit, params[2:])
+        x, u, *params[:2] = _ngr_layout(x, u, *params[:2])
         stats = stats.contiguous()
         # dx, du, dgate and the norms' parameters; branch_scale has none
         grads = [_dense(t) if need[i] else None for i, t in ((0, x), (1, u), (2, params[0]), (4, params[2]), (5, params[3]),
@@ -2159,12 +2175,12 @@ def norm_gate_residual(x, u, gate=None, branch_scale=None, res_scale=1.0, post=N
             raise ValueError(f"branch_scale must be float32 [{B}], got {branch_scale.dtype} {tuple(branch_scale.shape)}")
         if branch_scale.requires_grad:
             raise ValueError("branch_scale is not differentiated")
-    x, u, params = _ngr_layout(x, u, gate, branch_scale, *vectors)
+    x, u, gate, branch_scale = _ngr_layout(x, u, gate, branch_scale)
     meta = (_number("res_scale", res_scale), _NORM_KINDS[post], _NORM_KINDS[pre], _number("eps", eps))
     if not meta[3] >= 0.0:
         raise ValueError(f"eps {eps} must not be negative")
-    device = _one_device(x, u, *params)
+    device = _one_device(x, u, gate, branch_scale, *vectors)
     if node:
-        res = NormGateResidualFn.apply(x, u, *params, meta, device)
+        res = NormGateResidualFn.apply(x, u, gate, branch_scale, *vectors, meta, device)
         return res if pre is not None else (res, None)
-    return _ngr_fwd(device, x, u, params, meta, False)[:2]
+    return _ngr_fwd(device, x, u, (gate, branch_scale, *vectors), meta, False)[:2]
