@@ -23,15 +23,24 @@
 // in the workspace, joined by a second launch.
 // Staging: 16-byte loads that land in LDS without a register between; they cost their issue and nothing else, and the next
 // tile's are on their way during a tile's products.
-// Rounding: in bf16, probabilities and dS are rounded to bf16 before the second product of each pair (the matrix
-// instruction's operands; sums, statistics and delta are 32-bit), which leaves results up to 1.5 times as far from the
-// exact ones as rounding the exact result alone; the row sums add the rounded probabilities, so the weights sum to one.
+// Rounding: in bf16, probabilities and dS are rounded to bf16 before the second product of each pair (the matrix instruction's
+// operands; sums and statistics are 32-bit), which leaves results up to 1.5 times as far from the exact ones as rounding the
+// exact result alone.  Two terms of P in the row form cost 19 % at 197 keys, 7 % at 77 and 32 % in the long shape below.  The
+// few-row form, which waits for memory, and the backward pass of up to 32 keys have them.  delta is formed from the rounded
+// output: gradients of few ALLOWED keys among more than 32, where dP and delta nearly cancel, are up to 2.3 times as far off
+// (0.0038 with two, 0.0027 with eight, 0.0025 with 32; rounding alone 0.0017).  One-term row sums add the rounded
+// probabilities, so the weights sum to one.
 // Measured (kernel alone; the chip holds about 1.9 GHz under these products):
-//   2 x 4096 rows, 16 heads over 4 of 128, 4609 and 3457 keys, bf16: forward 317 us (854 TFLOP/s), dq 421, dk / dv 640 + 23 for
-//   the join; bound by the matrix pipes with exponentials and conversions in between, one wave a SIMD of each kind waiting.
+//   2 x 4096 rows, 16 heads over 4 of 128, 4609 and 3457 keys, bf16: forward 316 us (857 TFLOP/s), dq 415, dk / dv 632 + 24 for
+//   the join.  Matrix instructions run 48 % (forward), 49 % (dk / dv) and 56 % (dq) of the busy time: with two waves a SIMD the
+//   exponentials, conversions and staging between the products are not covered in full.
 //   32 x 12 heads of 64, 576 rows, 197 keys: forward 31 us, backward 73 + 7; 16 x 8 of 80, 1025 rows, 77 keys: 21, 39 + 7.
-//   8 x 1 row, 32 heads over 8 of 128, about 12800 keys: 83 + 5 us, 5.1 TB/s of keys and values.
-//   fp32, 8 x 6 heads of 64, 333 rows, 257 keys: 32, dq 42, dk / dv 46 + 7: 144 workgroups for 256 compute units.
+//   8 x 1 row, 32 heads over 8 of 128, about 12800 keys: 85 + 5 us, 5.0 TB/s of keys and values.
+//   fp32, 8 x 6 heads of 64, 333 rows, 257 keys: 33, dq 43, dk / dv 48 + 8: 144 workgroups for 256 compute units, and matrix
+//   instructions run 44 to 55 % of the busy time of those, one wave a SIMD with nothing to cover its waits.
+//   Heads off the vector size (8 bf16 or 4 fp32 elements) and operands off a 16-byte border take element loads and the width of
+//   128 throughout: 32 x 12 heads, 576 rows, 197 keys in bf16, forward 178 us with heads of 66, 157 of 36, 185 of 64 off a
+//   border; backward 770, 641, 755.
 // Masked keys: their K and V rows are staged as zeros whatever they hold, their scores are -inf.
 #include <algorithm>
 #include <atomic>
@@ -615,7 +624,8 @@ __device__ __forceinline__ void wave_fence() {
 }
 
 // Few rows: every wave walks 32-key tiles of its own for the same 32 rows.  Bound by the bytes of K and V, which go
-// through registers: a wave waits for its own loads alone, four of them a SIMD cover for each other (5.1 TB/s at 8 x 8 key heads of 128).
+// through registers: a wave waits for its own loads alone, four of them a SIMD cover for each other (5.0 TB/s at 8 x 8 key heads of
+// 128).  P enters its product as two bf16 terms, which costs nothing beside the loads (82 us either way).
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS) void xattn_few_kernel(XaArgs a) {
     constexpr int KT = 32, IMG = KT * DP;
@@ -770,7 +780,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaArgs a, long long row
 }
 
 // dq (and delta, which the dk / dv launch reads): four waves of 32 rows over the key tiles, two products of 32 x 32 scores
-// and one that turns them into dq; 421 us at the long shape above, 964 TFLOP/s of its own three products
+// and one that turns them into dq; 415 us at the long shape above, 977 TFLOP/s of its own three products
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(XA_THREADS, sizeof(T) == 4 || !VEC ? 1 : 2) void xattn_dq_kernel(XaArgs a) {
     constexpr int KT = Mx<T>::KT, IMG = KT * DP, NF = DP / Mx<T>::KD;
