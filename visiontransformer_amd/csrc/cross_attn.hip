@@ -26,8 +26,8 @@
 // Rounding: in bf16, probabilities and dS are rounded to bf16 before the second product of each pair (the matrix instruction's
 // operands; sums and statistics are 32-bit), which leaves results up to 1.5 times as far from the exact ones as rounding the
 // exact result alone.  Two terms of P in the row form cost 19 % at 197 keys, 7 % at 77 and 32 % in the long shape below.  The
-// few-row form, which waits for memory, and the backward pass of up to 32 keys have them.  delta is formed from the rounded
-// output: gradients of few ALLOWED keys among more than 32, where dP and delta nearly cancel, are up to 2.3 times as far off
+// few-row form, which waits for memory, and the one-launch backward pass of up to 32 keys have them.  delta is formed from the
+// rounded output elsewhere: gradients of few ALLOWED keys there, where dP and delta nearly cancel, are up to 2.3 times as far off
 // (0.0038 with two, 0.0027 with eight, 0.0025 with 32; rounding alone 0.0017).  One-term row sums add the rounded
 // probabilities, so the weights sum to one.
 // Measured (kernel alone; the chip holds about 1.9 GHz under these products):
